@@ -1,0 +1,559 @@
+// Kernels of the fp8 linear and the linears of experts; see expert_ops.hpp.
+#include "expert_ops.hpp"
+
+#include <algorithm>
+
+#include "fp8.cuh"
+#include "launch.hpp"
+
+namespace cq {
+
+namespace {
+
+// ------------------------------------------------------------------ rows to e4m3
+
+// One block of 128 values per half warp, eight values a lane: the largest
+// magnitude by shuffles, then the codes, eight bytes a lane.  Bound by memory:
+// (2 + 1) bytes a value for 16-bit rows.
+constexpr int kQuantThreads = 256;
+
+template <int DT>
+__device__ __forceinline__ void load8(const void* row, int k, int cols, bool aligned, float (&v)[8]) {
+  if (aligned && k + 8 <= cols) {
+    if constexpr (DT == kF32) {
+      const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + k);
+      const float4 a = p[0], b = p[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+      v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + k);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (DT == kBF16) {
+          v[2 * j] = __uint_as_float(w[j] << 16);
+          v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+          v[2 * j] = f.x, v[2 * j + 1] = f.y;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = 0.0f;
+      if (k + j < cols) v[j] = ld_t<DT>(row, k + j);
+    }
+  }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const QuantizeRowsArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int kSize = DT == kF32 ? 4 : 2;
+  const int blocks = (a.cols + kFp8Block - 1) / kFp8Block;
+  const int64_t items = static_cast<int64_t>(a.rows) * blocks;
+  const bool aligned = ((a.ldx * kSize) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+  const int half = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  constexpr int kHalves = kQuantThreads / 16;
+  // every lane of a warp makes the same number of turns: the shuffles below
+  // are the warp's
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kHalves; base < items;
+       base += static_cast<int64_t>(gridDim.x) * kHalves) {
+    const int64_t item = base + half;
+    bool live = item < items;
+    const int64_t row = live ? item / blocks : 0;
+    const int block = live ? static_cast<int>(item - row * blocks) : 0;
+    int64_t src = row;
+    if (live && a.row_index != nullptr) {
+      src = a.row_index[row];
+      live = src >= 0 && src < a.x_rows;
+    }
+    const int k = block * kFp8Block + lane * 8;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    if (live) load8<DT>(reinterpret_cast<const char*>(a.x) + src * a.ldx * kSize, k, a.cols, aligned, v);
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, finite_magnitude(v[j]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if (!live) continue;
+    const int e = fp8_scale_exponent(top);
+    const float inv = pow2f(-e);
+    uint2 out;
+    out.x = e4m3x2(v[0] * inv, v[1] * inv) | (e4m3x2(v[2] * inv, v[3] * inv) << 16);
+    out.y = e4m3x2(v[4] * inv, v[5] * inv) | (e4m3x2(v[6] * inv, v[7] * inv) << 16);
+    if (k < a.ld) *reinterpret_cast<uint2*>(a.codes + row * a.ld + k) = out;
+    if (lane == 0) a.scales[static_cast<int64_t>(block) * a.rows + row] = pow2f(e);
+  }
+}
+
+// One CTA per 128 x 128 block of a weight; used when a layer is made.
+__global__ void __launch_bounds__(kQuantThreads)
+    quantize_weight_kernel(const float* w, int rows, int cols, uint8_t* codes, float* scales) {
+  const int n0 = blockIdx.y * kFp8Block, k0 = blockIdx.x * kFp8Block;
+  const int n1 = min(n0 + kFp8Block, rows), k1 = min(k0 + kFp8Block, cols);
+  __shared__ uint32_t most;
+  if (threadIdx.x == 0) most = 0;
+  __syncthreads();
+  const int c = threadIdx.x % kFp8Block, r0 = threadIdx.x / kFp8Block;
+  constexpr int kStep = kQuantThreads / kFp8Block;
+  uint32_t top = 0;
+  if (k0 + c < k1)
+    for (int n = n0 + r0; n < n1; n += kStep)
+      top = max(top, finite_magnitude(w[static_cast<int64_t>(n) * cols + k0 + c]));
+  atomicMax(&most, top);
+  __syncthreads();
+  const int e = fp8_scale_exponent(most);
+  const float inv = pow2f(-e);
+  if (k0 + c < k1)
+    for (int n = n0 + r0; n < n1; n += kStep) {
+      const int64_t i = static_cast<int64_t>(n) * cols + k0 + c;
+      codes[i] = static_cast<uint8_t>(e4m3x2(w[i] * inv, 0.0f));
+    }
+  if (threadIdx.x == 0) scales[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = pow2f(e);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) round_kernel(const float* v, int64_t n, void* out) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256)
+    st_t<DT>(out, i, v[i]);
+}
+
+// ------------------------------------------------------------------ the product
+
+// offsets[e] kept inside [0, rows] and rising, whatever the array holds.
+__device__ __forceinline__ int group_end(const int32_t* offsets, int e, int begin, int rows) {
+  return min(max(offsets[e + 1], begin), rows);
+}
+
+constexpr int kTile = 64, kStepK = 16;
+
+template <int DT, bool F8>
+__global__ void __launch_bounds__(256) expert_product_kernel(const ExpertProductArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  // the blockIdx.y-th tile of 64 rows over all groups; the rows past the last
+  // group are a group of their own, whose tiles are zeros
+  int e = 0, begin = 0, end = 0, tile = blockIdx.y;
+  if (a.offsets == nullptr) {
+    end = a.rows;
+    begin = tile * kTile;
+    if (begin >= end) return;
+  } else {
+    int at = 0;
+    for (e = 0; e <= a.experts; ++e) {
+      const int next = e < a.experts ? group_end(a.offsets, e, at, a.rows) : a.rows;
+      const int tiles = (next - at + kTile - 1) / kTile;
+      if (tile < tiles) {
+        begin = at + tile * kTile;
+        end = next;
+        break;
+      }
+      tile -= tiles;
+      at = next;
+    }
+    if (e > a.experts) return;
+  }
+  const int n0 = blockIdx.x * kTile;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float acc[4][4] = {};
+  const int KB = (a.K + kFp8Block - 1) / kFp8Block, NB = (a.N + kFp8Block - 1) / kFp8Block;
+  __shared__ float xs[kStepK][kTile + 1], ws[kStepK][kTile + 1];
+  if (e < a.experts) {
+    for (int k0 = 0; k0 < a.K; k0 += kStepK) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < kTile * kStepK; i += 256) {
+        const int r = i / kStepK, k = k0 + i % kStepK;
+        float xv = 0.0f, wv = 0.0f;
+        const int row = begin + r, n = n0 + r;
+        if (row < end && k < a.K) {
+          if constexpr (F8) {
+            xv = e4m3_to_float(reinterpret_cast<const uint8_t*>(a.x)[row * a.ldx + k]) *
+                 a.x_scales[static_cast<int64_t>(k / kFp8Block) * a.rows + row];
+          } else {
+            const int64_t src = a.row_index ? a.row_index[row] : row;
+            if (src >= 0 && src < a.x_rows) xv = ld_t<DT>(a.x, src * a.ldx + k);
+          }
+        }
+        if (n < a.N && k < a.K) {
+          const int64_t i_w = (static_cast<int64_t>(e) * a.N + n) * a.ldw + k;
+          if constexpr (F8) {
+            wv = e4m3_to_float(reinterpret_cast<const uint8_t*>(a.w)[i_w]) *
+                 a.w_scales[(static_cast<int64_t>(e) * NB + n / kFp8Block) * KB + k / kFp8Block];
+          } else {
+            wv = ld_t<DT>(a.w, i_w);
+          }
+        }
+        xs[i % kStepK][r] = xv;
+        ws[i % kStepK][r] = wv;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kStepK; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[k][ty + 16 * i], ws[k][tx + 16 * j], acc[i][j]);
+    }
+  }
+  for (int i = 0; i < 4; ++i) {
+    const int row = begin + ty + 16 * i;
+    if (row >= end) continue;
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + tx + 16 * j;
+      if (n >= a.N) continue;
+      float v = 0.0f;
+      if (e < a.experts) {
+        v = acc[i][j];
+        if (a.bias != nullptr) v += ld_t<DT>(a.bias, static_cast<int64_t>(e) * a.N + n);
+        v = activate(v, a.act);
+      }
+      if (a.y_f32) st_t<kF32>(a.y, row * a.ldy + n, v);
+      else st_t<DT>(a.y, row * a.ldy + n, v);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ router
+
+// A block takes kRouteTokens tokens, a warp one token at a time.  A token's
+// logits live as order-preserving integers in the warp's lanes; each of the
+// `top` rounds is a warp maximum, then the lowest index that holds it.  Which
+// tokens of the block chose an expert is a bit mask per expert in shared
+// memory, so that a pair's rank inside the block is a population count, the
+// same in every run.  One block does it all where the tokens fit one;
+// otherwise a second kernel adds up the blocks' counts.
+constexpr int kRouteTokens = 128;
+constexpr int kRouteThreads = 1024;
+constexpr int kRouteWords = kRouteTokens / 32;
+
+// Unsigned order of the key = order of the value; 0 for -inf and NaN.
+__device__ __forceinline__ uint32_t route_key(float v) {
+  if (!(v > -INFINITY)) return 0u;
+  const uint32_t u = __float_as_uint(v + 0.0f);  // -0 and +0 are equal
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float route_value(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
+}
+
+template <int DT, int PER>
+__device__ __forceinline__ void route_token(const RouteArgs& a, int t, int slot, int lane, uint32_t* masks,
+                                            int16_t* chosen) {
+  uint32_t key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = i * 32 + lane;
+    key[i] = e < a.experts ? route_key(ld_t<DT>(a.logits, t * a.ld + e)) : 0u;
+  }
+  uint32_t first = 0;
+  float total = 0.0f, mine = 0.0f;
+  int mine_e = -1;
+  for (int j = 0; j < a.top; ++j) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) best = max(best, key[i]);
+    best = __reduce_max_sync(0xFFFFFFFFu, best);
+    if (best == 0) break;
+    if (j == 0) {
+      first = best;
+      if (!a.renormalize) {
+        // the denominator over every expert that can be taken
+        float sum = 0.0f;
+        const float m = route_value(first);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (key[i] != 0u) sum += m == INFINITY ? (key[i] == first ? 1.0f : 0.0f) : expf(route_value(key[i]) - m);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        total = sum;
+      }
+    }
+    uint32_t at = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = PER - 1; i >= 0; --i)
+      if (key[i] == best) at = i * 32 + lane;
+    at = __reduce_min_sync(0xFFFFFFFFu, at);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (static_cast<uint32_t>(i * 32 + lane) == at) key[i] = 0u;
+    const float m = route_value(first);
+    const float share = m == INFINITY ? (best == first ? 1.0f : 0.0f) : expf(route_value(best) - m);
+    if (a.renormalize) total += share;
+    if (lane == j) {
+      mine = share;
+      mine_e = static_cast<int>(at);
+    }
+  }
+  if (lane < a.top) {
+    const int64_t p = static_cast<int64_t>(t) * a.top + lane;
+    a.expert[p] = mine_e;
+    a.weight[p] = mine_e >= 0 ? mine / total : 0.0f;
+    if (chosen != nullptr) chosen[slot * a.top + lane] = static_cast<int16_t>(mine_e);
+    if (mine_e >= 0) atomicOr(&masks[mine_e * kRouteWords + (slot >> 5)], 1u << (slot & 31));
+  }
+}
+
+__device__ __forceinline__ int mask_count(const uint32_t* m) {
+  int n = 0;
+#pragma unroll
+  for (int w = 0; w < kRouteWords; ++w) n += __popc(m[w]);
+  return n;
+}
+
+__device__ __forceinline__ int mask_rank(const uint32_t* m, int slot) {
+  int n = 0;
+#pragma unroll
+  for (int w = 0; w < kRouteWords; ++w) {
+    if (w < (slot >> 5)) n += __popc(m[w]);
+    else if (w == (slot >> 5)) n += __popc(m[w] & ((1u << (slot & 31)) - 1u));
+  }
+  return n;
+}
+
+// base[e] (shared, kMaxExperts values) -> the exclusive sum before e; returns
+// the total.  All threads of the block; experts <= kRouteThreads.
+__device__ __forceinline__ int exclusive_sum(int* base, int experts, int* scratch) {
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  int v = t < experts ? base[t] : 0, sum = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+    if (lane >= o) sum += up;
+  }
+  if (lane == 31) scratch[warp] = sum;
+  __syncthreads();
+  if (warp == 0) {
+    int s = lane < kRouteThreads / 32 ? scratch[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xFFFFFFFFu, s, o);
+      if (lane >= o) s += up;
+    }
+    scratch[lane] = s;
+  }
+  __syncthreads();
+  const int before = warp ? scratch[warp - 1] : 0;
+  if (t < experts) base[t] = before + sum - v;
+  const int total = scratch[31];
+  __syncthreads();
+  return total;
+}
+
+// Writes the sorted rows of the block's pairs from base[e], the first row that
+// the block has in expert e.
+__device__ __forceinline__ void place_pairs(const RouteArgs& a, int t0, int n, const int* base, const uint32_t* masks,
+                                            const int16_t* chosen) {
+  for (int i = threadIdx.x; i < n * a.top; i += kRouteThreads) {
+    const int slot = i / a.top;
+    const int e = chosen[i];
+    int row = -1;
+    if (e >= 0) {
+      row = base[e] + mask_rank(masks + e * kRouteWords, slot);
+      a.token[row] = t0 + slot;
+    }
+    a.position[static_cast<int64_t>(t0) * a.top + i] = row;
+  }
+}
+
+__device__ __forceinline__ void write_tail(const RouteArgs& a, int total, int first, int step) {
+  for (int64_t p = static_cast<int64_t>(total) + first; p < static_cast<int64_t>(a.tokens) * a.top; p += step)
+    a.token[p] = -1;
+}
+
+template <int DT, int PER, bool ONE>
+__global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const RouteArgs a) {
+  extern __shared__ uint32_t route_smem[];
+  uint32_t* masks = route_smem;                                           // [experts][kRouteWords]
+  int* base = reinterpret_cast<int*>(masks + a.experts * kRouteWords);    // [experts] (ONE)
+  int16_t* chosen = reinterpret_cast<int16_t*>(base + (ONE ? a.experts : 0));  // [kRouteTokens][top] (ONE)
+  __shared__ int scratch[32];
+  pdl_launch_dependents();
+  for (int i = threadIdx.x; i < a.experts * kRouteWords; i += kRouteThreads) masks[i] = 0u;
+  __syncthreads();
+  pdl_wait();
+  const int t0 = blockIdx.x * kRouteTokens;
+  const int n = min(kRouteTokens, a.tokens - t0);
+  for (int slot = threadIdx.x >> 5; slot < n; slot += kRouteThreads / 32)
+    route_token<DT, PER>(a, t0 + slot, slot, threadIdx.x & 31, masks, ONE ? chosen : nullptr);
+  __syncthreads();
+  if constexpr (ONE) {
+    for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) base[e] = mask_count(masks + e * kRouteWords);
+    __syncthreads();
+    const int total = exclusive_sum(base, a.experts, scratch);
+    for (int e = threadIdx.x; e <= a.experts; e += kRouteThreads) a.offsets[e] = e < a.experts ? base[e] : total;
+    place_pairs(a, t0, n, base, masks, chosen);
+    write_tail(a, total, threadIdx.x, kRouteThreads);
+  } else {
+    for (int e = threadIdx.x; e < a.experts; e += kRouteThreads)
+      a.counts[static_cast<int64_t>(blockIdx.x) * a.experts + e] = mask_count(masks + e * kRouteWords);
+  }
+}
+
+// The rows of each block's pairs: the counts of the blocks before it and of
+// all experts before, from the counts of all blocks.
+__global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteArgs a) {
+  extern __shared__ uint32_t route_smem[];
+  uint32_t* masks = route_smem;
+  int* base = reinterpret_cast<int*>(masks + a.experts * kRouteWords);  // [experts]
+  int* before = base + a.experts;                                       // [experts]
+  int16_t* chosen = reinterpret_cast<int16_t*>(before + a.experts);
+  __shared__ int scratch[32];
+  pdl_launch_dependents();
+  for (int i = threadIdx.x; i < a.experts * kRouteWords; i += kRouteThreads) masks[i] = 0u;
+  for (int i = threadIdx.x; i < a.experts; i += kRouteThreads) base[i] = before[i] = 0;
+  __syncthreads();
+  pdl_wait();
+  const int t0 = blockIdx.x * kRouteTokens;
+  const int n = min(kRouteTokens, a.tokens - t0);
+  for (int i = threadIdx.x; i < n * a.top; i += kRouteThreads) {
+    const int e = a.expert[static_cast<int64_t>(t0) * a.top + i], slot = i / a.top;
+    chosen[i] = static_cast<int16_t>(e);
+    if (e >= 0) atomicOr(&masks[e * kRouteWords + (slot >> 5)], 1u << (slot & 31));
+  }
+  // threads that share an expert split the blocks
+  const int lanes = kRouteThreads / a.experts;
+  if (static_cast<int>(threadIdx.x) < lanes * a.experts) {
+    const int e = threadIdx.x % a.experts;
+    int all = 0, mine = 0;
+    for (int b = threadIdx.x / a.experts; b < static_cast<int>(gridDim.x); b += lanes) {
+      const int c = a.counts[static_cast<int64_t>(b) * a.experts + e];
+      all += c;
+      mine += b < static_cast<int>(blockIdx.x) ? c : 0;
+    }
+    atomicAdd(&base[e], all);
+    atomicAdd(&before[e], mine);
+  }
+  __syncthreads();
+  const int total = exclusive_sum(base, a.experts, scratch);
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e <= a.experts; e += kRouteThreads) a.offsets[e] = e < a.experts ? base[e] : total;
+  for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) before[e] += base[e];
+  __syncthreads();
+  place_pairs(a, t0, n, before, masks, chosen);
+  write_tail(a, total, blockIdx.x * kRouteThreads + threadIdx.x, gridDim.x * kRouteThreads);
+}
+
+template <int DT, int PER>
+cudaError_t route_typed(const RouteArgs& a, cudaStream_t stream, bool pdl) {
+  const int blocks = (a.tokens + kRouteTokens - 1) / kRouteTokens;
+  const size_t masks = static_cast<size_t>(a.experts) * kRouteWords * 4;
+  const size_t chosen = static_cast<size_t>(kRouteTokens) * a.top * 2;
+  if (blocks <= 1)
+    return launch(route_choose_kernel<DT, PER, true>, dim3(1), dim3(kRouteThreads), masks + a.experts * 4 + chosen,
+                  stream, pdl, a);
+  cudaError_t e = launch(route_choose_kernel<DT, PER, false>, dim3(blocks), dim3(kRouteThreads), masks, stream, pdl, a);
+  if (e != cudaSuccess) return e;
+  return launch(route_place_kernel, dim3(blocks), dim3(kRouteThreads), masks + a.experts * 8 + chosen, stream, pdl, a);
+}
+
+template <int DT>
+cudaError_t route_dtype(const RouteArgs& a, cudaStream_t stream, bool pdl) {
+  if (a.experts <= 32) return route_typed<DT, 1>(a, stream, pdl);
+  if (a.experts <= 128) return route_typed<DT, 4>(a, stream, pdl);
+  if (a.experts <= 512) return route_typed<DT, 16>(a, stream, pdl);
+  return route_typed<DT, 32>(a, stream, pdl);
+}
+
+// ------------------------------------------------------------------ combine
+
+// A thread sums eight columns of one token.  Bound by memory: the rows of z
+// once, y once.
+template <int DT>
+__global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int chunks = (a.dims + 7) / 8;
+  const bool zv = (a.ldz & 7) == 0 && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0;
+  const bool yv = (a.ldy & 7) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
+  const int64_t items = static_cast<int64_t>(a.tokens) * chunks;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < items;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t t = i / chunks;
+    const int d = static_cast<int>(i - t * chunks) * 8;
+    float acc[8] = {};
+    for (int j = 0; j < a.top; ++j) {
+      const int p = __ldg(a.position + t * a.top + j);
+      if (p < 0 || p >= a.rows) continue;
+      const float w = __ldg(a.weight + t * a.top + j);
+      float v[8];
+      load8<DT>(reinterpret_cast<const uint16_t*>(a.z) + p * a.ldz, d, a.dims, zv, v);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) acc[c] = fmaf(w, v[c], acc[c]);
+    }
+    uint16_t* out = reinterpret_cast<uint16_t*>(a.y) + t * a.ldy + d;
+    if (yv && d + 8 <= a.dims) {
+      uint32_t u[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) u[c] = pack_t<DT>(acc[2 * c], acc[2 * c + 1]);
+      *reinterpret_cast<uint4*>(out) = make_uint4(u[0], u[1], u[2], u[3]);
+    } else {
+      for (int c = 0; c < 8; ++c)
+        if (d + c < a.dims) st_t<DT>(out, c, acc[c]);
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_quantize_rows(int dtype, const QuantizeRowsArgs& a, cudaStream_t stream, bool pdl) {
+  const int64_t items = static_cast<int64_t>(a.rows) * ((a.cols + kFp8Block - 1) / kFp8Block);
+  if (items == 0) return cudaSuccess;
+  const int grid = static_cast<int>(std::min<int64_t>((items + 15) / 16, 148 * 8 * 4));
+  switch (dtype) {
+    case kF16: return launch(quantize_rows_kernel<kF16>, dim3(grid), dim3(kQuantThreads), 0, stream, pdl, a);
+    case kBF16: return launch(quantize_rows_kernel<kBF16>, dim3(grid), dim3(kQuantThreads), 0, stream, pdl, a);
+    case kF32: return launch(quantize_rows_kernel<kF32>, dim3(grid), dim3(kQuantThreads), 0, stream, pdl, a);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t launch_quantize_weight(const float* w, int rows, int cols, uint8_t* codes, float* scales,
+                                   cudaStream_t stream) {
+  const dim3 grid((cols + kFp8Block - 1) / kFp8Block, (rows + kFp8Block - 1) / kFp8Block);
+  return launch(quantize_weight_kernel, grid, dim3(kQuantThreads), 0, stream, false, w, rows, cols, codes, scales);
+}
+
+cudaError_t launch_round(int dtype, const float* v, int64_t n, void* out, cudaStream_t stream) {
+  const int grid = static_cast<int>(std::min<int64_t>((n + 255) / 256, 1024));
+  return dtype == kF16 ? launch(round_kernel<kF16>, dim3(grid), dim3(256), 0, stream, false, v, n, out)
+                       : launch(round_kernel<kBF16>, dim3(grid), dim3(256), 0, stream, false, v, n, out);
+}
+
+cudaError_t launch_expert_product(int dtype, bool e4m3, const ExpertProductArgs& a, cudaStream_t stream, bool pdl) {
+  const dim3 grid((a.N + kTile - 1) / kTile, (a.rows + kTile - 1) / kTile + (a.offsets ? a.experts + 1 : 0));
+  if (dtype == kF16)
+    return e4m3 ? launch(expert_product_kernel<kF16, true>, grid, dim3(256), 0, stream, pdl, a)
+                : launch(expert_product_kernel<kF16, false>, grid, dim3(256), 0, stream, pdl, a);
+  return e4m3 ? launch(expert_product_kernel<kBF16, true>, grid, dim3(256), 0, stream, pdl, a)
+              : launch(expert_product_kernel<kBF16, false>, grid, dim3(256), 0, stream, pdl, a);
+}
+
+size_t route_workspace(int tokens, int experts) {
+  const size_t blocks = (static_cast<size_t>(tokens) + kRouteTokens - 1) / kRouteTokens;
+  return blocks <= 1 ? 0 : blocks * experts * sizeof(int32_t);
+}
+
+cudaError_t launch_route(int dtype, const RouteArgs& a, cudaStream_t stream, bool pdl) {
+  switch (dtype) {
+    case kF16: return route_dtype<kF16>(a, stream, pdl);
+    case kBF16: return route_dtype<kBF16>(a, stream, pdl);
+    case kF32: return route_dtype<kF32>(a, stream, pdl);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t launch_combine(int dtype, const CombineArgs& a, cudaStream_t stream, bool pdl) {
+  const int64_t items = static_cast<int64_t>(a.tokens) * ((a.dims + 7) / 8);
+  if (items == 0) return cudaSuccess;
+  const int grid = static_cast<int>(std::min<int64_t>((items + 255) / 256, 1 << 20));
+  return dtype == kF16 ? launch(combine_kernel<kF16>, dim3(grid), dim3(256), 0, stream, pdl, a)
+                       : launch(combine_kernel<kBF16>, dim3(grid), dim3(256), 0, stream, pdl, a);
+}
+
+}  // namespace cq

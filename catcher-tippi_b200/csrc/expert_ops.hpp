@@ -1,0 +1,83 @@
+// Kernels of the fp8 linear and of the linears of experts: bringing rows and
+// weights to e4m3, the grouped product, the router and the combine.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace cq {
+
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxTop = 32;
+
+// x rows -> e4m3 codes [rows][ld] (ld a multiple of 16; zero from cols to the
+// next multiple of 128 or ld) and scales [ceil(cols / 128)][rows].  With
+// row_index, row r is x row row_index[r]; rows whose index is outside
+// [0, x_rows) are left as they are.
+struct QuantizeRowsArgs {
+  const void* x;
+  int64_t ldx;
+  const int32_t* row_index;
+  int x_rows, rows, cols;
+  uint8_t* codes;
+  int64_t ld;
+  float* scales;
+};
+cudaError_t launch_quantize_rows(int dtype, const QuantizeRowsArgs& a, cudaStream_t stream, bool pdl);
+
+// Weight f32 [rows, cols] -> codes and the scales of 128 x 128 blocks.
+cudaError_t launch_quantize_weight(const float* w, int rows, int cols, uint8_t* codes, float* scales,
+                                   cudaStream_t stream);
+
+// f32 -> T (kF16 or kBF16), to nearest.
+cudaError_t launch_round(int dtype, const float* v, int64_t n, void* out, cudaStream_t stream);
+
+// The grouped product: rows [offsets[e], offsets[e + 1]) of x by the weights
+// of expert e; without offsets all rows meet expert 0.  Rows past
+// offsets[experts] are set to zero.
+struct ExpertProductArgs {
+  const void* x;  // T [rows][ldx], or e4m3 codes [rows][ldx]
+  int64_t ldx;
+  const int32_t* row_index;  // T only: row r is x row row_index[r]; outside [0, x_rows) reads as zero
+  int x_rows;
+  const float* x_scales;  // e4m3: [ceil(K / 128)][rows]
+  int rows;
+  const void* w;  // T or codes [experts][N][ldw]
+  int64_t ldw;
+  const float* w_scales;  // e4m3: [experts][ceil(N / 128)][ceil(K / 128)]
+  const void* bias;       // T [experts][N] or null
+  const int32_t* offsets;
+  int experts, N, K, act;
+  void* y;  // T, or f32 with y_f32
+  int64_t ldy;
+  int y_f32;
+};
+cudaError_t launch_expert_product(int dtype, bool e4m3, const ExpertProductArgs& a, cudaStream_t stream,
+                                  bool pdl);
+
+struct RouteArgs {
+  const void* logits;
+  int64_t ld;
+  int tokens, experts, top, renormalize;
+  int32_t* expert;
+  float* weight;
+  int32_t* offsets;
+  int32_t* token;
+  int32_t* position;
+  int32_t* counts;  // workspace: route_workspace bytes
+};
+size_t route_workspace(int tokens, int experts);
+cudaError_t launch_route(int dtype, const RouteArgs& a, cudaStream_t stream, bool pdl);
+
+struct CombineArgs {
+  const void* z;
+  int64_t ldz;
+  const int32_t* position;
+  const float* weight;
+  int rows, tokens, top, dims;
+  void* y;
+  int64_t ldy;
+};
+cudaError_t launch_combine(int dtype, const CombineArgs& a, cudaStream_t stream, bool pdl);
+
+}  // namespace cq

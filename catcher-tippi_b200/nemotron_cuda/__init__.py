@@ -39,7 +39,7 @@ def lib() -> ctypes.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is missing; run catcher-tippi_b200/build.py")
     L = ctypes.CDLL(LIB_PATH)
-    vp, i32, sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_size_t
+    vp, i32, i64, sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t
     pp = ctypes.POINTER(ctypes.c_void_p)
     sig = {
         "cq_last_error": ([], ctypes.c_char_p),
@@ -131,6 +131,31 @@ def lib() -> ctypes.CDLL:
         "cq_logmel_filters": ([vp, vp, sz], i32),
         "cq_logmel_extract": ([vp, vp, i32, ctypes.c_int64, ctypes.c_int64, i32, vp, vp], i32),
         "cq_logmel_destroy": ([vp], None),
+        # 8-bit floating-point linear (include/cqfp8.h)
+        "cq_fp8_linear_create": ([vp, vp, vp, i32, i32, i32, i32, pp], i32),
+        "cq_fp8_linear_create_from_f32": ([vp, vp, i32, i32, i32, i32, pp], i32),
+        "cq_fp8_linear_workspace": ([vp, i32], sz),
+        "cq_fp8_linear_forward": ([vp, vp, i64, i32, vp, i64, i32, vp, sz, vp], i32),
+        "cq_fp8_linear_forward_codes": ([vp, vp, i64, vp, i32, vp, i64, i32, vp], i32),
+        "cq_fp8_linear_input_dims": ([vp], i32),
+        "cq_fp8_linear_output_dims": ([vp], i32),
+        "cq_fp8_linear_destroy": ([vp], None),
+        "cq_fp8_quantize_rows": ([vp, i64, i32, i32, i32, vp, i64, vp, vp], i32),
+        "cq_fp8_quantize_weight": ([vp, i32, i32, vp, vp, vp], i32),
+        # linears of experts (include/cqexperts.h)
+        "cq_expert_linear_create": ([vp, vp, vp, i32, i32, i32, i32, i32, i32, pp], i32),
+        "cq_expert_linear_workspace": ([vp, i32], sz),
+        "cq_expert_linear_forward": ([vp, vp, i64, i32, vp, vp, i64, i32, vp, sz, vp], i32),
+        "cq_expert_linear_experts": ([vp], i32),
+        "cq_expert_linear_input_dims": ([vp], i32),
+        "cq_expert_linear_output_dims": ([vp], i32),
+        "cq_expert_linear_destroy": ([vp], None),
+        "cq_route_workspace": ([i32, i32, i32], sz),
+        "cq_route": ([vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, sz, vp], i32),
+        "cq_expert_combine": ([vp, i64, i32, vp, vp, i32, i32, i32, i32, vp, i64, vp], i32),
+        "cq_expert_ffn_workspace": ([vp, vp, i32, i32], sz),
+        "cq_expert_ffn_forward": ([vp, vp, vp, i64, i32, vp, i64, i32, i32, i32, i32, vp, i64, vp, sz,
+                                   vp], i32),
         # streaming scheduler and tokenizer (include/cqstream.h)
         "cq_chunk_scheduler_create": ([i32, pp], i32),
         "cq_chunk_scheduler_push": ([vp, vp, sz, ctypes.POINTER(ctypes.c_int32)], i32),

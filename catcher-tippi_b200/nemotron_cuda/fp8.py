@@ -1,0 +1,221 @@
+"""Python bindings of the 8-bit floating-point linear (include/cqfp8.h).
+
+``Fp8Linear`` holds e4m3 weights with an f32 scale for each 128 x 128 block;
+``forward`` brings the rows of x to e4m3 (a power-of-two scale for each 128
+values), multiplies and applies bias and activation in f32.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import numpy as np
+
+from . import ACTS, CQ_INVALID_ARGUMENT, DTYPES, CQError, _check, _ptr, lib
+
+BLOCK = 128
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _types():
+    torch = _torch()
+    return {torch.float16: "f16", torch.bfloat16: "bf16", torch.float32: "f32"}
+
+
+def _refuse(message: str):
+    raise CQError(CQ_INVALID_ARGUMENT, message)
+
+
+def _stream_of(stream, device) -> int:
+    if stream is None:
+        return _torch().cuda.current_stream(device).cuda_stream
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _allocating(stream, device):
+    """The context in which a call's tensors are allocated: torch's memory pool goes by the stream that uses it."""
+    if stream is None:
+        return contextlib.nullcontext()
+    cuda = _torch().cuda
+    return cuda.stream(cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream)
+
+
+def _contiguous(a):
+    """The array without gaps: numpy or torch, on the host or the device."""
+    return np.ascontiguousarray(a) if isinstance(a, np.ndarray) else a.contiguous()
+
+
+def _packed(a, *shape):
+    """An array argument of a layer: its shape checked, without gaps."""
+    if tuple(a.shape) != shape:
+        _refuse(f"array has shape {tuple(a.shape)}, expected {shape}")
+    return _contiguous(a)
+
+
+def _bytes(a) -> int:
+    return a.itemsize if isinstance(a, np.ndarray) else a.element_size()
+
+
+def blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _rows_of(x, dims: int, what: str = "input"):
+    if not x.is_cuda:
+        _refuse(f"{what} must be on the device, got {x.device}")
+    if x.dim() != 2 or x.shape[1] != dims or (dims > 1 and x.stride(1) != 1):
+        _refuse(f"{what} must be rows of {dims} values next to each other, got shape {tuple(x.shape)} "
+                f"with strides {tuple(x.stride())}")
+
+
+class _Layer:
+    """A handle of the library and what its calls need to know."""
+
+    _destroy = ""
+
+    def __init__(self, handle: ctypes.c_void_p, experts: int, output_dims: int, input_dims: int, dtype: str,
+                 device: int):
+        self._h = handle
+        self.experts, self.output_dims, self.input_dims = experts, output_dims, input_dims
+        self.dtype, self.device = dtype, device
+        torch = _torch()
+        self._type = {"f16": torch.float16, "bf16": torch.bfloat16}[dtype]
+        self._torch_device = torch.device("cuda", device)
+        self._sizes: dict[int, int] = {}
+
+    def _output(self, x, y):
+        torch = _torch()
+        if x.device != self._torch_device:
+            _refuse(f"input is on {x.device}, the layer on {self._torch_device}")
+        if x.dtype != self._type:
+            _refuse(f"input has type {x.dtype}, expected {self._type}")
+        if y is None:
+            return torch.empty((x.shape[0], self.output_dims), dtype=self._type, device=x.device)
+        if y.dtype != self._type or y.shape[0] != x.shape[0]:
+            _refuse(f"output must be {self._type} with {x.shape[0]} rows")
+        _rows_of(y, self.output_dims, "output")
+        return y
+
+    def _workspace(self, entry, rows: int):
+        """(tensor that keeps the memory, pointer, bytes) for a call on `rows` rows."""
+        n = self._sizes.get(rows)
+        if n is None:
+            if len(self._sizes) > 256:
+                self._sizes.clear()
+            n = self._sizes[rows] = entry(self._h, rows)
+        if n == 0:
+            return None, None, 0
+        w = _torch().empty(n, dtype=_torch().uint8, device=self._torch_device)
+        return w, w.data_ptr(), n
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            try:
+                getattr(lib(), self._destroy)(self._h)
+            except TypeError:  # interpreter shutdown
+                pass
+            self._h = None
+
+    def __del__(self):
+        self.close()
+
+
+class Fp8Linear(_Layer):
+    """y = act(x^ . w^T + b) with e4m3 weights in blocks of 128 x 128."""
+
+    _destroy = "cq_fp8_linear_destroy"
+
+    @classmethod
+    def from_codes(cls, codes, scales, bias=None, dtype: str = "bf16", device: int = 0) -> "Fp8Linear":
+        """codes [N, K] of one byte (torch float8_e4m3fn or uint8, or numpy uint8), scales f32
+        [ceil(N / 128), ceil(K / 128)], bias T [N] or None; host or device arrays."""
+        n, k = codes.shape
+        if _bytes(codes) != 1:
+            _refuse("codes must have one byte each")
+        if _bytes(scales) != 4 or (bias is not None and _bytes(bias) != 2):
+            _refuse("scales must be f32 and the bias of the layer's 16-bit type")
+        c, s = _packed(codes, n, k), _packed(scales, blocks(n), blocks(k))
+        b = None if bias is None else _packed(bias, n)
+        h = ctypes.c_void_p()
+        _check(lib().cq_fp8_linear_create(_ptr(c), _ptr(s), _ptr(b), n, k, DTYPES[dtype], device, ctypes.byref(h)))
+        return cls(h, 1, n, k, dtype, device)
+
+    @classmethod
+    def from_f32(cls, weight, bias=None, dtype: str = "bf16", device: int = 0) -> "Fp8Linear":
+        """An f32 weight [N, K] and bias [N] (numpy or torch, host or device), brought to e4m3 on the device."""
+        n, k = weight.shape
+        if _bytes(weight) != 4 or (bias is not None and _bytes(bias) != 4):
+            _refuse("weight and bias must be f32")
+        w, b = _contiguous(weight), None if bias is None else _packed(bias, n)
+        h = ctypes.c_void_p()
+        _check(lib().cq_fp8_linear_create_from_f32(_ptr(w), _ptr(b), n, k, DTYPES[dtype], device, ctypes.byref(h)))
+        return cls(h, 1, n, k, dtype, device)
+
+    def forward(self, x, y=None, act: str = "none", stream=None):
+        """x torch [rows, K] of T on the layer's device -> y [rows, N]."""
+        _rows_of(x, self.input_dims)
+        L = lib()
+        with _allocating(stream, x.device):
+            y = self._output(x, y)
+            keep, ws, n = self._workspace(L.cq_fp8_linear_workspace, x.shape[0])
+            _check(L.cq_fp8_linear_forward(self._h, x.data_ptr(), x.stride(0), x.shape[0], y.data_ptr(), y.stride(0),
+                                           ACTS[act], ws, n, _stream_of(stream, x.device)))
+        return y
+
+    def forward_codes(self, codes, scales, y=None, act: str = "none", stream=None):
+        """forward on rows that quantize_rows made: codes [rows, >= K], scales [ceil(K / 128), rows]."""
+        torch = _torch()
+        if codes.device != self._torch_device or scales.device != self._torch_device:
+            _refuse(f"codes and scales must be on {self._torch_device}")
+        rows = codes.shape[0]
+        if codes.dim() != 2 or codes.shape[1] < self.input_dims or codes.stride(1) != 1 or _bytes(codes) != 1:
+            _refuse(f"codes must be rows of at least {self.input_dims} bytes, got shape {tuple(codes.shape)}")
+        if scales.dtype != torch.float32 or tuple(scales.shape) != (blocks(self.input_dims), rows) or \
+                not scales.is_contiguous():
+            _refuse(f"scales must be f32 [{blocks(self.input_dims)}, {rows}] without gaps")
+        if y is None:
+            with _allocating(stream, codes.device):
+                y = torch.empty((rows, self.output_dims), dtype=self._type, device=codes.device)
+        elif y.dtype != self._type or y.shape[0] != rows:
+            _refuse(f"output must be {self._type} with {rows} rows")
+        _rows_of(y, self.output_dims, "output")
+        _check(lib().cq_fp8_linear_forward_codes(self._h, codes.data_ptr(), codes.stride(0), scales.data_ptr(), rows,
+                                                 y.data_ptr(), y.stride(0), ACTS[act],
+                                                 _stream_of(stream, codes.device)))
+        return y
+
+
+def quantize_rows(x, stream=None):
+    """x torch [rows, K] (f16, bf16 or f32) -> (e4m3 codes [rows, 128 ceil(K / 128)], scales f32 [ceil(K / 128), rows])."""
+    torch = _torch()
+    if x.dim() != 2:
+        _refuse(f"input must be rows, got shape {tuple(x.shape)}")
+    rows, k = x.shape
+    _rows_of(x, k)
+    kind = _types().get(x.dtype)
+    if kind is None:
+        _refuse(f"input has type {x.dtype}, expected f16, bf16 or f32")
+    with _allocating(stream, x.device):
+        codes = torch.empty((rows, BLOCK * blocks(k)), dtype=torch.float8_e4m3fn, device=x.device)
+        scales = torch.empty((blocks(k), rows), dtype=torch.float32, device=x.device)
+    _check(lib().cq_fp8_quantize_rows(x.data_ptr(), x.stride(0), rows, k, DTYPES[kind], codes.data_ptr(),
+                                      codes.stride(0), scales.data_ptr(), _stream_of(stream, x.device)))
+    return codes, scales
+
+
+def quantize_weight(w, stream=None):
+    """w torch f32 [N, K] on the device -> (e4m3 codes [N, K], scales f32 [ceil(N / 128), ceil(K / 128)])."""
+    torch = _torch()
+    if not w.is_cuda or w.dim() != 2 or w.dtype != torch.float32 or not w.is_contiguous():
+        _refuse("weight must be f32 [N, K] without gaps on the device")
+    n, k = w.shape
+    with _allocating(stream, w.device):
+        codes = torch.empty((n, k), dtype=torch.float8_e4m3fn, device=w.device)
+        scales = torch.empty((blocks(n), blocks(k)), dtype=torch.float32, device=w.device)
+    _check(lib().cq_fp8_quantize_weight(w.data_ptr(), n, k, codes.data_ptr(), scales.data_ptr(),
+                                        _stream_of(stream, w.device)))
+    return codes, scales
