@@ -1,0 +1,46 @@
+// The grouped product on the 5th-generation tensor cores: see expert_gemm.cu.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "expert_ops.hpp"
+
+namespace cq {
+
+constexpr int kGemmRows = 128;  // rows of x per CTA
+
+// How one call is cut: CTAs per MMA (1, or 2 sharing one of 256 rows), weight
+// rows per tile (64, 128 or 256), and CTAs that share a tile's k (with pairs
+// and 256-wide tiles: 1).
+struct ExpertGemmConfig {
+  int pair, bn, splits;
+};
+
+// What a value of y becomes: T, f32, or e4m3 codes with their scales.
+enum ExpertOut : int { kOutT = 0, kOutF32 = 1, kOutCodes = 2 };
+
+struct ExpertGemmArgs {
+  const float* x_scales;  // e4m3: [k blocks][rows]
+  const float* w_scales;  // e4m3: [experts][n blocks][k blocks]
+  const void* bias;       // T [experts][N] or null
+  const int32_t* offsets; // null: all rows meet expert 0
+  int rows, experts, N, K, act;
+  int out;
+  void* y;  // T, f32 or codes, row stride ldy
+  int64_t ldy;
+  float* y_scales;  // kOutCodes: [ceil(N / 128)][rows]
+  int* status;
+  int splits;
+};
+
+// xmap: [rows, K] of x, box 128 bytes x 128 rows; wmap: [experts * N, K], box
+// 128 bytes x bn / pair rows; both with the 128-byte swizzle.
+cudaError_t launch_expert_gemm(int dtype, bool e4m3, const CUtensorMap& xmap, const CUtensorMap& wmap,
+                               const ExpertGemmConfig& cfg, ExpertGemmArgs a, int num_sms, cudaStream_t stream,
+                               bool pdl);
+
+ExpertGemmConfig plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, bool codes_out, int num_sms);
+
+}  // namespace cq

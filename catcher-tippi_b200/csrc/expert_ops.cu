@@ -124,98 +124,33 @@ __global__ void __launch_bounds__(256) round_kernel(const float* v, int64_t n, v
     st_t<DT>(out, i, v[i]);
 }
 
-// ------------------------------------------------------------------ the product
+// ------------------------------------------------------------------ gather
 
-// offsets[e] kept inside [0, rows] and rising, whatever the array holds.
-__device__ __forceinline__ int group_end(const int32_t* offsets, int e, int begin, int rows) {
-  return min(max(offsets[e + 1], begin), rows);
-}
-
-constexpr int kTile = 64, kStepK = 16;
-
-template <int DT, bool F8>
-__global__ void __launch_bounds__(256) expert_product_kernel(const ExpertProductArgs a) {
+// 16-bit rows to 16-byte aligned rows, eight values a thread: the order of a
+// row list, or rows whose own alignment a tile copy cannot take.
+__global__ void __launch_bounds__(256) gather_rows_kernel(const GatherRowsArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  // the blockIdx.y-th tile of 64 rows over all groups; the rows past the last
-  // group are a group of their own, whose tiles are zeros
-  int e = 0, begin = 0, end = 0, tile = blockIdx.y;
-  if (a.offsets == nullptr) {
-    end = a.rows;
-    begin = tile * kTile;
-    if (begin >= end) return;
-  } else {
-    int at = 0;
-    for (e = 0; e <= a.experts; ++e) {
-      const int next = e < a.experts ? group_end(a.offsets, e, at, a.rows) : a.rows;
-      const int tiles = (next - at + kTile - 1) / kTile;
-      if (tile < tiles) {
-        begin = at + tile * kTile;
-        end = next;
-        break;
-      }
-      tile -= tiles;
-      at = next;
-    }
-    if (e > a.experts) return;
-  }
-  const int n0 = blockIdx.x * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  const int KB = (a.K + kFp8Block - 1) / kFp8Block, NB = (a.N + kFp8Block - 1) / kFp8Block;
-  __shared__ float xs[kStepK][kTile + 1], ws[kStepK][kTile + 1];
-  if (e < a.experts) {
-    for (int k0 = 0; k0 < a.K; k0 += kStepK) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < kTile * kStepK; i += 256) {
-        const int r = i / kStepK, k = k0 + i % kStepK;
-        float xv = 0.0f, wv = 0.0f;
-        const int row = begin + r, n = n0 + r;
-        if (row < end && k < a.K) {
-          if constexpr (F8) {
-            xv = e4m3_to_float(reinterpret_cast<const uint8_t*>(a.x)[row * a.ldx + k]) *
-                 a.x_scales[static_cast<int64_t>(k / kFp8Block) * a.rows + row];
-          } else {
-            const int64_t src = a.row_index ? a.row_index[row] : row;
-            if (src >= 0 && src < a.x_rows) xv = ld_t<DT>(a.x, src * a.ldx + k);
-          }
-        }
-        if (n < a.N && k < a.K) {
-          const int64_t i_w = (static_cast<int64_t>(e) * a.N + n) * a.ldw + k;
-          if constexpr (F8) {
-            wv = e4m3_to_float(reinterpret_cast<const uint8_t*>(a.w)[i_w]) *
-                 a.w_scales[(static_cast<int64_t>(e) * NB + n / kFp8Block) * KB + k / kFp8Block];
-          } else {
-            wv = ld_t<DT>(a.w, i_w);
-          }
-        }
-        xs[i % kStepK][r] = xv;
-        ws[i % kStepK][r] = wv;
-      }
-      __syncthreads();
+  const int chunks = (a.cols + 7) / 8;
+  const bool aligned = (a.ldx & 7) == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+  const int64_t items = static_cast<int64_t>(a.rows) * chunks;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < items;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / chunks;
+    const int c = static_cast<int>(i - row * chunks) * 8;
+    const int64_t src = a.row_index != nullptr ? a.row_index[row] : row;
+    if (src < 0 || src >= a.x_rows) continue;
+    const uint16_t* from = reinterpret_cast<const uint16_t*>(a.x) + src * a.ldx + c;
+    uint4 v;
+    if (aligned && c + 8 <= a.cols) {
+      v = *reinterpret_cast<const uint4*>(from);
+    } else {
+      uint16_t h[8];
 #pragma unroll
-      for (int k = 0; k < kStepK; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[k][ty + 16 * i], ws[k][tx + 16 * j], acc[i][j]);
+      for (int j = 0; j < 8; ++j) h[j] = c + j < a.cols ? from[j] : static_cast<uint16_t>(0);
+      v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
     }
-  }
-  for (int i = 0; i < 4; ++i) {
-    const int row = begin + ty + 16 * i;
-    if (row >= end) continue;
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + tx + 16 * j;
-      if (n >= a.N) continue;
-      float v = 0.0f;
-      if (e < a.experts) {
-        v = acc[i][j];
-        if (a.bias != nullptr) v += ld_t<DT>(a.bias, static_cast<int64_t>(e) * a.N + n);
-        v = activate(v, a.act);
-      }
-      if (a.y_f32) st_t<kF32>(a.y, row * a.ldy + n, v);
-      else st_t<DT>(a.y, row * a.ldy + n, v);
-    }
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + row * a.ld + c) = v;
   }
 }
 
@@ -464,11 +399,12 @@ cudaError_t route_dtype(const RouteArgs& a, cudaStream_t stream, bool pdl) {
 
 // A thread sums eight columns of one token.  Bound by memory: the rows of z
 // once, y once.
-template <int DT>
+template <int DT, int ZT>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const int chunks = (a.dims + 7) / 8;
+  constexpr int kSize = ZT == kF32 ? 4 : 2;
   const bool zv = (a.ldz & 7) == 0 && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0;
   const bool yv = (a.ldy & 7) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
   const int64_t items = static_cast<int64_t>(a.tokens) * chunks;
@@ -482,7 +418,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
       if (p < 0 || p >= a.rows) continue;
       const float w = __ldg(a.weight + t * a.top + j);
       float v[8];
-      load8<DT>(reinterpret_cast<const uint16_t*>(a.z) + p * a.ldz, d, a.dims, zv, v);
+      load8<ZT>(reinterpret_cast<const char*>(a.z) + p * a.ldz * kSize, d, a.dims, zv, v);
 #pragma unroll
       for (int c = 0; c < 8; ++c) acc[c] = fmaf(w, v[c], acc[c]);
     }
@@ -525,13 +461,11 @@ cudaError_t launch_round(int dtype, const float* v, int64_t n, void* out, cudaSt
                        : launch(round_kernel<kBF16>, dim3(grid), dim3(256), 0, stream, false, v, n, out);
 }
 
-cudaError_t launch_expert_product(int dtype, bool e4m3, const ExpertProductArgs& a, cudaStream_t stream, bool pdl) {
-  const dim3 grid((a.N + kTile - 1) / kTile, (a.rows + kTile - 1) / kTile + (a.offsets ? a.experts + 1 : 0));
-  if (dtype == kF16)
-    return e4m3 ? launch(expert_product_kernel<kF16, true>, grid, dim3(256), 0, stream, pdl, a)
-                : launch(expert_product_kernel<kF16, false>, grid, dim3(256), 0, stream, pdl, a);
-  return e4m3 ? launch(expert_product_kernel<kBF16, true>, grid, dim3(256), 0, stream, pdl, a)
-              : launch(expert_product_kernel<kBF16, false>, grid, dim3(256), 0, stream, pdl, a);
+cudaError_t launch_gather_rows(const GatherRowsArgs& a, cudaStream_t stream, bool pdl) {
+  const int64_t items = static_cast<int64_t>(a.rows) * ((a.cols + 7) / 8);
+  if (items == 0) return cudaSuccess;
+  const int grid = static_cast<int>(std::min<int64_t>((items + 255) / 256, 148 * 16));
+  return launch(gather_rows_kernel, dim3(grid), dim3(256), 0, stream, pdl, a);
 }
 
 size_t route_workspace(int tokens, int experts) {
@@ -552,8 +486,11 @@ cudaError_t launch_combine(int dtype, const CombineArgs& a, cudaStream_t stream,
   const int64_t items = static_cast<int64_t>(a.tokens) * ((a.dims + 7) / 8);
   if (items == 0) return cudaSuccess;
   const int grid = static_cast<int>(std::min<int64_t>((items + 255) / 256, 1 << 20));
-  return dtype == kF16 ? launch(combine_kernel<kF16>, dim3(grid), dim3(256), 0, stream, pdl, a)
-                       : launch(combine_kernel<kBF16>, dim3(grid), dim3(256), 0, stream, pdl, a);
+  if (a.z_f32)
+    return dtype == kF16 ? launch(combine_kernel<kF16, kF32>, dim3(grid), dim3(256), 0, stream, pdl, a)
+                         : launch(combine_kernel<kBF16, kF32>, dim3(grid), dim3(256), 0, stream, pdl, a);
+  return dtype == kF16 ? launch(combine_kernel<kF16, kF16>, dim3(grid), dim3(256), 0, stream, pdl, a)
+                       : launch(combine_kernel<kBF16, kBF16>, dim3(grid), dim3(256), 0, stream, pdl, a);
 }
 
 }  // namespace cq

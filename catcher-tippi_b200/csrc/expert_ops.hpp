@@ -32,28 +32,17 @@ cudaError_t launch_quantize_weight(const float* w, int rows, int cols, uint8_t* 
 // f32 -> T (kF16 or kBF16), to nearest.
 cudaError_t launch_round(int dtype, const float* v, int64_t n, void* out, cudaStream_t stream);
 
-// The grouped product: rows [offsets[e], offsets[e + 1]) of x by the weights
-// of expert e; without offsets all rows meet expert 0.  Rows past
-// offsets[experts] are set to zero.
-struct ExpertProductArgs {
-  const void* x;  // T [rows][ldx], or e4m3 codes [rows][ldx]
+// 16-bit rows x[row_index[r]] (or x[r]) -> out rows of stride ld, a multiple
+// of 8 at least cols; rows whose index is outside [0, x_rows) are left as they are.
+struct GatherRowsArgs {
+  const void* x;
   int64_t ldx;
-  const int32_t* row_index;  // T only: row r is x row row_index[r]; outside [0, x_rows) reads as zero
-  int x_rows;
-  const float* x_scales;  // e4m3: [ceil(K / 128)][rows]
-  int rows;
-  const void* w;  // T or codes [experts][N][ldw]
-  int64_t ldw;
-  const float* w_scales;  // e4m3: [experts][ceil(N / 128)][ceil(K / 128)]
-  const void* bias;       // T [experts][N] or null
-  const int32_t* offsets;
-  int experts, N, K, act;
-  void* y;  // T, or f32 with y_f32
-  int64_t ldy;
-  int y_f32;
+  const int32_t* row_index;
+  int x_rows, rows, cols;
+  void* out;
+  int64_t ld;
 };
-cudaError_t launch_expert_product(int dtype, bool e4m3, const ExpertProductArgs& a, cudaStream_t stream,
-                                  bool pdl);
+cudaError_t launch_gather_rows(const GatherRowsArgs& a, cudaStream_t stream, bool pdl);
 
 struct RouteArgs {
   const void* logits;
@@ -77,6 +66,7 @@ struct CombineArgs {
   int rows, tokens, top, dims;
   void* y;
   int64_t ldy;
+  int z_f32;  // z is f32 instead of T
 };
 cudaError_t launch_combine(int dtype, const CombineArgs& a, cudaStream_t stream, bool pdl);
 

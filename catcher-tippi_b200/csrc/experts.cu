@@ -3,6 +3,7 @@
 
 #include <string>
 
+#include "expert_gemm.hpp"
 #include "expert_ops.hpp"
 #include "qlinear.hpp"
 
@@ -69,18 +70,37 @@ int device_of(const void* p, const char* what) {
   return attr.device;
 }
 
-// Scratch of a product with e4m3 weights: the rows' codes and scales.
-struct CodeRows {
-  uint8_t* codes;
+// Rows in a workspace, as the product takes them: codes and scales, or T.
+struct StagedRows {
+  void* x;
   float* scales;
   int64_t ld;
 };
-CodeRows take_codes(Arena& arena, int64_t rows, int cols) {
-  CodeRows c{};
-  c.ld = round_up(cols, kBlock);
-  c.codes = arena.take<uint8_t>(rows * c.ld);
-  c.scales = arena.take<float>(rows * (c.ld / kBlock));
-  return c;
+StagedRows take_rows(Arena& arena, int64_t rows, int cols, bool e4m3) {
+  StagedRows s{};
+  if (e4m3) {
+    s.ld = round_up(cols, kBlock);
+    s.x = arena.take<uint8_t>(rows * s.ld);
+    s.scales = arena.take<float>(rows * (s.ld / kBlock));
+  } else {
+    s.ld = round_up(cols, 8);
+    s.x = arena.take<uint16_t>(rows * s.ld);
+  }
+  return s;
+}
+
+// Brings rows of T (in the order of row_index where given) to the form that
+// the product takes.
+ExpertLinear::Rows stage_rows(const StagedRows& s, const void* x, int64_t ldx, const int32_t* row_index, int x_rows,
+                              int rows, int cols, cq_dtype dtype, bool e4m3, cudaStream_t stream) {
+  if (e4m3) {
+    const cq::QuantizeRowsArgs q{x, ldx, row_index, x_rows, rows, cols, static_cast<uint8_t*>(s.x), s.ld, s.scales};
+    check_cuda(cq::launch_quantize_rows(dtype, q, stream, pdl_enabled()), "quantize rows");
+  } else {
+    const cq::GatherRowsArgs g{x, ldx, row_index, x_rows, rows, cols, s.x, s.ld};
+    check_cuda(cq::launch_gather_rows(g, stream, pdl_enabled()), "gather rows");
+  }
+  return {s.x, s.ld, s.scales};
 }
 
 }  // namespace
@@ -154,9 +174,9 @@ std::unique_ptr<ExpertLinear> ExpertLinear::from_f32(const float* weight, const 
 }
 
 size_t ExpertLinear::workspace(int rows) const {
-  if (rows == 0 || !e4m3()) return 0;
+  if (rows == 0) return 0;
   Arena arena(nullptr);
-  take_codes(arena, rows, K_);
+  take_rows(arena, rows, K_, e4m3());
   return arena.used();
 }
 
@@ -169,28 +189,30 @@ void ExpertLinear::check_rows(const void* x, int64_t ldx, int rows, const void* 
   check_act(act);
 }
 
-void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, void* y, int64_t ldy, bool y_f32, int act,
+void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, int out, void* y, int64_t ldy, int act,
                            cudaStream_t stream) const {
-  cq::ExpertProductArgs a{};
-  a.x = x.x;
-  a.ldx = x.ldx;
-  a.row_index = x.row_index;
-  a.x_rows = x.x_rows;
+  DeviceContext& ctx = device_context(device_);
+  cq::ExpertGemmArgs a{};
   a.x_scales = x.scales;
-  a.rows = rows;
-  a.w = weight_.get();
-  a.ldw = ldw_;
   a.w_scales = scales_.as<float>();
   a.bias = bias_.get();
   a.offsets = offsets;
+  a.rows = rows;
   a.experts = experts_;
   a.N = N_;
   a.K = K_;
   a.act = act;
+  a.out = out;
   a.y = y;
   a.ldy = ldy;
-  a.y_f32 = y_f32 ? 1 : 0;
-  check_cuda(cq::launch_expert_product(dtype_, e4m3(), a, stream, pdl_enabled()), "expert product");
+  a.status = ctx.status;
+  const cq::ExpertGemmConfig cfg = cq::plan_expert_gemm(e4m3(), rows, experts_, N_, K_, false, ctx.num_sms);
+  const int size = e4m3() ? 1 : 2, k = 128 / size;
+  const CUtensorMap xmap = make_map_2d(x.x, size, rows, K_, x.ld, cq::kGemmRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
+  const CUtensorMap wmap =
+      make_map_2d(weight_.get(), size, experts_ * N_, K_, ldw_, cfg.bn / cfg.pair, k, CU_TENSOR_MAP_SWIZZLE_128B);
+  check_cuda(cq::launch_expert_gemm(dtype_, e4m3(), xmap, wmap, cfg, a, ctx.num_sms, stream, pdl_enabled()),
+             "expert product");
 }
 
 void ExpertLinear::forward(const void* x, int64_t ldx, int rows, const int32_t* offsets, void* y, int64_t ldy, int act,
@@ -200,15 +222,12 @@ void ExpertLinear::forward(const void* x, int64_t ldx, int rows, const int32_t* 
   if (rows == 0) return;
   check_workspace(workspace, workspace_bytes, this->workspace(rows));
   DeviceGuard guard(device_);
-  Rows r{x, ldx, nullptr, rows, nullptr};
-  if (e4m3()) {
+  Rows r{x, ldx, nullptr};
+  if (e4m3() || ldx % 8 != 0 || (reinterpret_cast<uintptr_t>(x) & 15) != 0) {
     Arena arena(workspace);
-    const CodeRows c = take_codes(arena, rows, K_);
-    const cq::QuantizeRowsArgs q{x, ldx, nullptr, rows, rows, K_, c.codes, c.ld, c.scales};
-    check_cuda(cq::launch_quantize_rows(dtype_, q, stream, pdl_enabled()), "quantize rows");
-    r = Rows{c.codes, c.ld, nullptr, rows, c.scales};
+    r = stage_rows(take_rows(arena, rows, K_, e4m3()), x, ldx, nullptr, rows, rows, K_, dtype_, e4m3(), stream);
   }
-  product(r, rows, offsets, y, ldy, false, act, stream);
+  product(r, rows, offsets, cq::kOutT, y, ldy, act, stream);
 }
 
 void ExpertLinear::forward_codes(const uint8_t* codes, int64_t ld, const float* scales, int rows, void* y, int64_t ldy,
@@ -220,7 +239,7 @@ void ExpertLinear::forward_codes(const uint8_t* codes, int64_t ld, const float* 
   if (scales == nullptr) throw_invalid("scales must not be null");
   check_aligned(scales, 4, "scales");
   DeviceGuard guard(device_);
-  product(Rows{codes, ld, nullptr, rows, scales}, rows, nullptr, y, ldy, false, act, stream);
+  product({codes, ld, scales}, rows, nullptr, cq::kOutT, y, ldy, act, stream);
 }
 
 void quantize_rows(const void* x, int64_t ldx, const int32_t* row_index, int x_rows, int rows, int cols,
@@ -307,7 +326,7 @@ void combine(const void* z, int64_t ldz, int rows, const int32_t* position, cons
   check_aligned(position, 4, "positions");
   check_aligned(weight, 4, "weights");
   DeviceGuard guard(device_of(y, "output"));
-  const cq::CombineArgs a{z, ldz, position, weight, rows, tokens, top, dims, y, ldy};
+  const cq::CombineArgs a{z, ldz, position, weight, rows, tokens, top, dims, y, ldy, 0};
   check_cuda(cq::launch_combine(dtype, a, stream, pdl_enabled()), "combine");
 }
 
@@ -320,10 +339,9 @@ struct FfnScratch {
   float* weight;
   void* route;
   size_t route_bytes;
-  CodeRows x, h;  // e4m3
-  float* h_f32;   // e4m3: up's result, before it goes to codes
-  uint16_t* h_t;  // T
-  uint16_t* z;
+  StagedRows x, h;
+  float* h_f32;  // e4m3: up's result, before it goes to codes
+  float* z;      // f32: the sum over a token's experts is rounded once
 };
 
 FfnScratch take_ffn(Arena& arena, const ExpertLinear& up, const ExpertLinear& down, int tokens, int top) {
@@ -336,14 +354,10 @@ FfnScratch take_ffn(Arena& arena, const ExpertLinear& up, const ExpertLinear& do
   s.position = arena.take<int32_t>(pairs);
   s.route_bytes = route_workspace_bytes(tokens, up.experts(), top);
   s.route = arena.take<uint8_t>(s.route_bytes);
-  if (up.e4m3()) {
-    s.x = take_codes(arena, pairs, up.input_dims());
-    s.h_f32 = arena.take<float>(pairs * up.output_dims());
-    s.h = take_codes(arena, pairs, up.output_dims());
-  } else {
-    s.h_t = arena.take<uint16_t>(pairs * up.output_dims());
-  }
-  s.z = arena.take<uint16_t>(pairs * down.output_dims());
+  s.x = take_rows(arena, pairs, up.input_dims(), up.e4m3());
+  s.h = take_rows(arena, pairs, up.output_dims(), up.e4m3());
+  if (up.e4m3()) s.h_f32 = arena.take<float>(pairs * up.output_dims());
+  s.z = arena.take<float>(pairs * down.output_dims());
   return s;
 }
 
@@ -386,17 +400,18 @@ void expert_ffn(const ExpertLinear& up, const ExpertLinear& down, const void* x,
   DeviceGuard guard(up.device());
   route(logits, ld_logits, logits_dtype, tokens, up.experts(), top, renormalize, s.expert, s.weight, s.offsets,
         s.token, s.position, s.route, s.route_bytes, stream);
+  const ExpertLinear::Rows rows =
+      stage_rows(s.x, x, ldx, s.token, tokens, pairs, d, up.dtype(), up.e4m3(), stream);
+  ExpertLinear::Rows h{s.h.x, s.h.ld, s.h.scales};
   if (up.e4m3()) {
-    quantize_rows(x, ldx, s.token, tokens, pairs, d, up.dtype(), s.x.codes, s.x.ld, s.x.scales, stream);
-    up.product({s.x.codes, s.x.ld, nullptr, pairs, s.x.scales}, pairs, s.offsets, s.h_f32, ff, true, act, stream);
-    quantize_rows(s.h_f32, ff, nullptr, pairs, pairs, ff, CQ_F32, s.h.codes, s.h.ld, s.h.scales, stream);
-    down.product({s.h.codes, s.h.ld, nullptr, pairs, s.h.scales}, pairs, s.offsets, s.z, out, false, CQ_ACT_NONE,
-                 stream);
+    up.product(rows, pairs, s.offsets, cq::kOutF32, s.h_f32, ff, act, stream);
+    h = stage_rows(s.h, s.h_f32, ff, nullptr, pairs, pairs, ff, CQ_F32, true, stream);
   } else {
-    up.product({x, ldx, s.token, tokens, nullptr}, pairs, s.offsets, s.h_t, ff, false, act, stream);
-    down.product({s.h_t, ff, nullptr, pairs, nullptr}, pairs, s.offsets, s.z, out, false, CQ_ACT_NONE, stream);
+    up.product(rows, pairs, s.offsets, cq::kOutT, s.h.x, s.h.ld, act, stream);
   }
-  combine(s.z, out, pairs, s.position, s.weight, tokens, top, out, up.dtype(), y, ldy, stream);
+  down.product(h, pairs, s.offsets, cq::kOutF32, s.z, out, CQ_ACT_NONE, stream);
+  const cq::CombineArgs c{s.z, out, s.position, s.weight, pairs, tokens, top, out, y, ldy, 1};
+  check_cuda(cq::launch_combine(up.dtype(), c, stream, pdl_enabled()), "combine");
 }
 
 }  // namespace nemotron_cuda

@@ -37,16 +37,15 @@ class ExpertLinear {
   cq_dtype dtype() const { return dtype_; }
   int device() const { return device_; }
 
-  // The product alone, arguments checked: x is T rows (gathered by row_index
-  // where given) or the codes of rows with their scales.
+  // Rows as the product's tile copies take them: 16-byte aligned rows of T, or
+  // of codes with their scales [k blocks][rows].
   struct Rows {
     const void* x;
-    int64_t ldx;
-    const int32_t* row_index;
-    int x_rows;
+    int64_t ld;
     const float* scales;
   };
-  void product(const Rows& x, int rows, const int32_t* offsets, void* y, int64_t ldy, bool y_f32, int act,
+  // The product alone, arguments checked; out: a cq::ExpertOut.
+  void product(const Rows& x, int rows, const int32_t* offsets, int out, void* y, int64_t ldy, int act,
                cudaStream_t stream) const;
 
  private:

@@ -135,7 +135,7 @@ CUtensorMap encode_map(CUtensorMapDataType dt, int rank, const void* base, const
 
 }  // namespace
 
-CUtensorMap make_map_2d(const void* base, int elem_bytes, int rows, int cols, int ld,
+CUtensorMap make_map_2d(const void* base, int elem_bytes, int rows, int cols, int64_t ld,
                         int box_rows, int box_cols, CUtensorMapSwizzle swizzle) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * elem_bytes};  // bytes per row

@@ -56,7 +56,7 @@ class DeviceGuard {
 
 // 2-D tiled tensor map over a row-major [rows, cols] matrix of 1- or 2-byte
 // elements (row stride in elements), box [box_rows, box_cols].
-CUtensorMap make_map_2d(const void* base, int elem_bytes, int rows, int cols, int ld,
+CUtensorMap make_map_2d(const void* base, int elem_bytes, int rows, int cols, int64_t ld,
                         int box_rows, int box_cols, CUtensorMapSwizzle swizzle);
 
 // The K2 GEMM's activation maps over f16 [rows, K] with row stride ld.
