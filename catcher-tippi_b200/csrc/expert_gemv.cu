@@ -1,0 +1,428 @@
+// The grouped product for few rows an expert: y[r] = act(W[e] x[r] + b[e]).
+//
+// Bound by the bytes of the weights, so everything serves their stream: a warp
+// owns 16 weight rows and a slice of k and asks for all of it at once, 32 bytes
+// a lane and row (a quad reads the 128 bytes of one k block of one row), before
+// it looks at x.  The lane's bytes are used as the A fragment of mma.sync as
+// they come: which k a fragment slot holds does not matter as long as x, the B
+// fragment, is permuted alike, and both are read as the same 32 bytes of a
+// block.  mma.sync, not tcgen05: at 32 rows or fewer the products take less
+// than a tenth of the time of the weights' bytes, and this path has no
+// tensor-memory set-up and no copy into shared memory before it can start.
+//
+// A CTA is kBands bands of 16 weight rows times kSlices slices of k; with few
+// bands a cluster splits k further, the partial sums meeting in the first
+// CTA's shared memory.  Each CTA brings its slice of its expert's rows of x to
+// e4m3 itself (a few KB from L2), which saves a launch.
+#include "expert_gemv.hpp"
+
+#include <algorithm>
+
+#include "fp8.cuh"
+#include "launch.hpp"
+
+namespace cq {
+
+namespace {
+
+constexpr int kThreads = 256, kWarps = 8;
+constexpr int kPassRows = 32;   // rows of x that one turn over the weights serves
+constexpr int kAhead = 4;       // k blocks a warp has in flight
+constexpr int kSmemMax = 200 * 1024;
+
+
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void st_dsmem_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+struct Group {
+  int expert, begin, end;
+};
+
+// The slot-th expert that has rows, and the first row past all experts; every
+// warp for itself.  Offsets are cut to [0, rows] and made to rise.
+__device__ __forceinline__ Group find_group(const ExpertGemvArgs& a, int slot, int lane, int& past) {
+  Group g{-1, 0, 0};
+  if (a.offsets == nullptr) {
+    past = a.rows;
+    return slot == 0 ? Group{0, 0, a.rows} : g;
+  }
+  int row = 0;
+  for (int e0 = 0; e0 < a.experts; e0 += 32) {
+    const int e = e0 + lane;
+    int end = e < a.experts ? min(max(a.offsets[e + 1], row), a.rows) : row;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xFFFFFFFFu, end, o);
+      if (lane >= o) end = max(end, up);
+    }
+    int begin = __shfl_up_sync(0xFFFFFFFFu, end, 1);
+    if (lane == 0) begin = row;
+    const uint32_t has = __ballot_sync(0xFFFFFFFFu, end > begin);
+    const int count = __popc(has);
+    if (g.expert < 0) {
+      if (slot < count) {
+        const bool me = (has >> lane & 1u) && __popc(has & ((1u << lane) - 1u)) == slot;
+        const int at = __ffs(__ballot_sync(0xFFFFFFFFu, me)) - 1;
+        g.expert = e0 + at;
+        g.begin = __shfl_sync(0xFFFFFFFFu, begin, at);
+        g.end = __shfl_sync(0xFFFFFFFFu, end, at);
+      }
+      slot -= count;
+    }
+    row = __shfl_sync(0xFFFFFFFFu, end, 31);
+  }
+  past = row;
+  return g;
+}
+
+template <int DT, int SRC>
+__device__ __forceinline__ void load_x8(const ExpertGemvArgs& a, int64_t src, int k, bool aligned, float (&v)[8]) {
+  constexpr int T = SRC == kSourceF32 ? static_cast<int>(kF32) : DT;
+  const char* row = reinterpret_cast<const char*>(a.x) + src * a.ldx * (SRC == kSourceF32 ? 4 : 2);
+  if (aligned && k + 8 <= a.K) {
+    if constexpr (T == kF32) {
+      const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + k);
+      const float4 lo = p[0], hi = p[1];
+      v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w;
+      v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + k);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (T == kBF16) {
+          v[2 * j] = __uint_as_float(w[j] << 16);
+          v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+          v[2 * j] = f.x, v[2 * j + 1] = f.y;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = 0.0f;
+      if (k + j < a.K) v[j] = ld_t<T>(row, k + j);
+    }
+  }
+}
+
+// Rows [begin, begin + n) of x, blocks [kb0, kb1), into shared memory: codes
+// (or T), `pitch` bytes a row, and for codes their scales [block][kPassRows].
+template <bool F8, int DT, int SRC>
+__device__ __forceinline__ void stage_x(const ExpertGemvArgs& a, int begin, int n, int kb0, int kb1, uint8_t* xs,
+                                        int pitch, float* sx) {
+  const int blocks = kb1 - kb0;
+  if constexpr (F8 && SRC != kSourceCodes) {
+    constexpr int kSize = SRC == kSourceF32 ? 4 : 2;
+    const bool aligned = ((a.ldx * kSize) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+    const int half = threadIdx.x >> 4, lane = threadIdx.x & 15;
+    const int items = n * blocks;
+    for (int base = 0; base < items; base += kThreads / 16) {
+      const int item = base + half;
+      const bool live = item < items;
+      const int r = live ? item / blocks : 0, b = live ? item - r * blocks : 0;
+      const int64_t src = !live ? -1 : a.row_index != nullptr ? a.row_index[begin + r] : begin + r;
+      float v[8] = {};
+      if (src >= 0 && src < a.x_rows) load_x8<DT, SRC>(a, src, (kb0 + b) * kFp8Block + lane * 8, aligned, v);
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, finite_magnitude(v[j]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      if (!live) continue;
+      const int e = fp8_scale_exponent(top);
+      const float inv = pow2f(-e);
+      uint2 out;
+      out.x = e4m3x2(v[0] * inv, v[1] * inv) | (e4m3x2(v[2] * inv, v[3] * inv) << 16);
+      out.y = e4m3x2(v[4] * inv, v[5] * inv) | (e4m3x2(v[6] * inv, v[7] * inv) << 16);
+      *reinterpret_cast<uint2*>(xs + r * pitch + b * 128 + lane * 8) = out;
+      if (lane == 0) sx[b * kPassRows + r] = pow2f(e);
+    }
+  } else {
+    // 16 bytes a thread
+    constexpr int kSize = F8 ? 1 : 2, kPer = 16 / kSize;
+    const bool aligned = ((a.ldx * kSize) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+    const int pieces = blocks * 8;
+    for (int i = threadIdx.x; i < n * pieces; i += kThreads) {
+      const int r = i / pieces, p = i - r * pieces;
+      const int k = kb0 * (128 / kSize) + p * kPer;
+      const int64_t src = a.row_index != nullptr ? a.row_index[begin + r] : begin + r;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (src >= 0 && src < a.x_rows) {
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(a.x) + (src * a.ldx + k) * kSize;
+        if (aligned && k + kPer <= a.K) {
+          v = *reinterpret_cast<const uint4*>(from);
+        } else {
+          uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            if (k + j >= a.K) continue;
+            if constexpr (F8) w[j / 4] |= static_cast<uint32_t>(from[j]) << (8 * (j & 3));
+            else w[j / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(from)[j]) << (16 * (j & 1));
+          }
+          v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      *reinterpret_cast<uint4*>(xs + r * pitch + p * 16) = v;
+    }
+    if constexpr (F8) {
+      for (int i = threadIdx.x; i < n * blocks; i += kThreads) {
+        const int b = i / n, r = i - b * n;
+        sx[b * kPassRows + r] = a.x_scales[static_cast<int64_t>(kb0 + b) * a.rows + begin + r];
+      }
+    }
+  }
+}
+
+__host__ __device__ inline int x_pitch(int blocks) { return blocks * 128 + 16; }  // quads of a row pair miss each other's banks
+
+template <bool F8, int DT, int SRC, int BANDS>
+__global__ void __launch_bounds__(kThreads) expert_gemv_kernel(const ExpertGemvArgs a, int splits) {
+  constexpr int SLICES = kWarps / BANDS, ROWS = 16 * BANDS;
+  constexpr int kElems = F8 ? 128 : 64;
+  extern __shared__ __align__(16) uint8_t gemv_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int band = warp % BANDS, slice = warp / BANDS;
+  const int g = lane >> 2, q = lane & 3;
+  const int KB = (a.K + kElems - 1) / kElems;
+  const int rank = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int per = (KB + splits - 1) / splits;
+  const int kb0 = rank * per, kb1 = min(KB, kb0 + per);
+  // this warp's blocks of the CTA's
+  const int wper = (per + SLICES - 1) / SLICES;
+  const int wb0 = min(kb0 + slice * wper, kb1), wb1 = min(wb0 + wper, kb1);
+  const int n0 = blockIdx.x / splits * ROWS;
+  const int pass_rows = min(kPassRows, a.rows), staged = (pass_rows + 7) & ~7;
+  const int pitch = x_pitch(per);
+  uint8_t* xs = gemv_smem;
+  float* sx = reinterpret_cast<float*>(xs + staged * pitch);       // [per][kPassRows]
+  float* red = sx + (F8 ? per * kPassRows : 0);                    // [SLICES][kPassRows][ROWS + 1]
+  float* clus = red + SLICES * kPassRows * (ROWS + 1);             // [splits][kPassRows][ROWS], in rank 0
+  if (splits > 1) cluster_arrive();  // the CTAs of the cluster run
+
+  pdl_launch_dependents();
+  Group grp{0, 0, a.rows};
+  int past = a.rows;
+  if (a.offsets != nullptr) {
+    pdl_wait();
+    grp = find_group(a, blockIdx.y, lane, past);
+  }
+  // all of the warp's first blocks at once
+  const char* w_lo = nullptr;
+  const char* w_hi = nullptr;
+  const float* sw = nullptr;
+  uint4 w[kAhead][4];
+  if (grp.expert >= 0) {
+    // rows past N read the last row; what they make is not stored
+    const int64_t first = static_cast<int64_t>(grp.expert) * a.N;
+    const int64_t size = F8 ? 1 : 2;
+    w_lo = reinterpret_cast<const char*>(a.w) + (first + min(n0 + band * 16 + g, a.N - 1)) * a.ldw * size + q * 32;
+    w_hi = reinterpret_cast<const char*>(a.w) + (first + min(n0 + band * 16 + g + 8, a.N - 1)) * a.ldw * size + q * 32;
+    if constexpr (F8)
+      sw = a.w_scales + (static_cast<int64_t>(grp.expert) * ((a.N + kFp8Block - 1) / kFp8Block) +
+                         min(n0 + band * 16, a.N - 1) / kFp8Block) * KB;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (wb0 + i < wb1) {
+        ld_global_cg_v8(w_lo + static_cast<int64_t>(wb0 + i) * 128, w[i][0], w[i][1]);
+        ld_global_cg_v8(w_hi + static_cast<int64_t>(wb0 + i) * 128, w[i][2], w[i][3]);
+      }
+    }
+  }
+  if (a.offsets == nullptr) pdl_wait();
+
+  if (blockIdx.y == 0 && rank == 0) {
+    // rows of no expert are zeros
+    for (int64_t r = past + warp; r < a.rows; r += kWarps)
+      for (int i = lane; i < ROWS; i += 32)
+        if (n0 + i < a.N) {
+          if (a.y_f32) reinterpret_cast<float*>(a.y)[r * a.ldy + n0 + i] = 0.0f;
+          else reinterpret_cast<uint16_t*>(a.y)[r * a.ldy + n0 + i] = 0;
+        }
+  }
+
+  for (int begin = grp.begin; begin < grp.end; begin += kPassRows) {
+    const int n = min(kPassRows, grp.end - begin), tiles = (n + 7) >> 3;
+    __syncthreads();
+    stage_x<F8, DT, SRC>(a, begin, n, kb0, kb1, xs, pitch, sx);
+    __syncthreads();
+    float acc[4][4] = {};
+    for (int b0 = wb0; b0 < wb1; b0 += kAhead) {
+      if (b0 != wb0 || begin != grp.begin) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (b0 + i < wb1) {
+            ld_global_cg_v8(w_lo + static_cast<int64_t>(b0 + i) * 128, w[i][0], w[i][1]);
+            ld_global_cg_v8(w_hi + static_cast<int64_t>(b0 + i) * 128, w[i][2], w[i][3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (b0 + i >= wb1) break;
+        const uint32_t lo[8] = {w[i][0].x, w[i][0].y, w[i][0].z, w[i][0].w, w[i][1].x, w[i][1].y, w[i][1].z, w[i][1].w};
+        const uint32_t hi[8] = {w[i][2].x, w[i][2].y, w[i][2].z, w[i][2].w, w[i][3].x, w[i][3].y, w[i][3].z, w[i][3].w};
+        const int b = b0 + i - kb0;
+        float scale = 0.0f;
+        if constexpr (F8) scale = __ldg(sw + b0 + i);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if (t < tiles) {
+            const uint4* xp = reinterpret_cast<const uint4*>(xs + (t * 8 + g) * pitch + b * 128 + q * 32);
+            const uint4 x0 = xp[0], x1 = xp[1];
+            const uint32_t x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+            if constexpr (F8) {
+              float p[4] = {};
+#pragma unroll
+              for (int s = 0; s < 4; ++s) mma_e4m3(p, lo[2 * s], hi[2 * s], lo[2 * s + 1], hi[2 * s + 1], x[2 * s], x[2 * s + 1]);
+              const float2 f = *reinterpret_cast<const float2*>(sx + b * kPassRows + t * 8 + q * 2);
+              const float f0 = f.x * scale, f1 = f.y * scale;
+              acc[t][0] = fmaf(p[0], f0, acc[t][0]);
+              acc[t][1] = fmaf(p[1], f1, acc[t][1]);
+              acc[t][2] = fmaf(p[2], f0, acc[t][2]);
+              acc[t][3] = fmaf(p[3], f1, acc[t][3]);
+            } else {
+#pragma unroll
+              for (int s = 0; s < 4; ++s)
+                mma_16816<DT>(acc[t], lo[2 * s], hi[2 * s], lo[2 * s + 1], hi[2 * s + 1], x[2 * s], x[2 * s + 1]);
+            }
+          }
+        }
+      }
+    }
+    // the slices' sums, row by row of the tile
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (t < tiles) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          red[(slice * kPassRows + t * 8 + q * 2 + (i & 1)) * (ROWS + 1) + band * 16 + g + (i >> 1) * 8] = acc[t][i];
+      }
+    }
+    __syncthreads();
+    if (splits > 1 && begin == grp.begin) cluster_wait();
+    for (int i = threadIdx.x; i < n * ROWS; i += kThreads) {
+      const int r = i / ROWS, c = i % ROWS;
+      float v = 0.0f;
+#pragma unroll
+      for (int s = 0; s < SLICES; ++s) v += red[(s * kPassRows + r) * (ROWS + 1) + c];
+      if (splits > 1) {
+        st_dsmem_f32(mapa_shared(smem_u32(clus + (rank * kPassRows + r) * ROWS + c), 0), v);
+      } else if (n0 + c < a.N) {
+        if (a.bias != nullptr) v += ld_t<DT>(a.bias, static_cast<int64_t>(grp.expert) * a.N + n0 + c);
+        v = activate(v, a.act);
+        const int64_t at = (static_cast<int64_t>(begin) + r) * a.ldy + n0 + c;
+        if (a.y_f32) st_t<kF32>(a.y, at, v);
+        else st_t<DT>(a.y, at, v);
+      }
+    }
+    if (splits > 1) {
+      cluster_sync_all();
+      if (rank == 0) {
+        for (int i = threadIdx.x; i < n * ROWS; i += kThreads) {
+          const int r = i / ROWS, c = i % ROWS;
+          if (n0 + c >= a.N) continue;
+          float v = 0.0f;
+          for (int s = 0; s < splits; ++s) v += clus[(s * kPassRows + r) * ROWS + c];
+          if (a.bias != nullptr) v += ld_t<DT>(a.bias, static_cast<int64_t>(grp.expert) * a.N + n0 + c);
+          v = activate(v, a.act);
+          const int64_t at = (static_cast<int64_t>(begin) + r) * a.ldy + n0 + c;
+          if (a.y_f32) st_t<kF32>(a.y, at, v);
+          else st_t<DT>(a.y, at, v);
+        }
+      }
+      if (begin + kPassRows < grp.end) cluster_sync_all();  // the first CTA has read them
+    }
+  }
+  if (splits > 1 && grp.begin >= grp.end) cluster_wait();
+}
+
+struct GemvPlan {
+  int bands, splits, smem;
+};
+
+int smem_of(bool e4m3, int rows, int KB, int bands, int splits) {
+  const int per = (KB + splits - 1) / splits;
+  const int staged = (std::min(rows, kPassRows) + 7) & ~7;
+  int bytes = staged * x_pitch(per) + (e4m3 ? per * kPassRows * 4 : 0);
+  bytes += kWarps / bands * kPassRows * (16 * bands + 1) * 4;
+  if (splits > 1) bytes += splits * kPassRows * 16 * bands * 4;
+  return bytes;
+}
+
+GemvPlan plan(bool e4m3, int rows, int groups, int N, int K, int num_sms) {
+  const int KB = (K + (e4m3 ? 127 : 63)) / (e4m3 ? 128 : 64);
+  GemvPlan p{2, 1, 0};
+  if (static_cast<int64_t>((N + 31) / 32) * groups < num_sms) p.bands = 1;
+  const int64_t ctas = static_cast<int64_t>((N + 16 * p.bands - 1) / (16 * p.bands)) * groups;
+  const int slices = kWarps / p.bands;
+  // split k while a warp still has a block of its own and the GPU has room, or
+  // while the rows of x do not fit
+  for (int s : {2, 4, 8}) {
+    const int per = (KB + s - 1) / s;
+    if ((s - 1) * per >= KB) break;
+    const bool room = ctas * s <= 2 * num_sms && per >= slices;
+    if (room || smem_of(e4m3, rows, KB, p.bands, p.splits) > 56 * 1024) p.splits = s;
+  }
+  p.smem = smem_of(e4m3, rows, KB, p.bands, p.splits);
+  return p;
+}
+
+template <bool F8, int DT, int SRC, int BANDS>
+cudaError_t launch_typed(const GemvPlan& p, const ExpertGemvArgs& a, int groups, cudaStream_t stream, bool pdl) {
+  static SharedMemoryOptIn opt_in;
+  auto kernel = expert_gemv_kernel<F8, DT, SRC, BANDS>;
+  const cudaError_t e = opt_in.ensure(reinterpret_cast<const void*>(kernel), kSmemMax);
+  if (e != cudaSuccess) return e;
+  const int tiles = (a.N + 16 * BANDS - 1) / (16 * BANDS);
+  return launch_clustered(kernel, dim3(tiles * p.splits, groups), dim3(kThreads), p.smem, stream, pdl, p.splits, a, p.splits);
+}
+
+template <bool F8, int DT, int SRC>
+cudaError_t launch_source(const ExpertGemvArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
+  const int groups = a.offsets == nullptr ? 1 : std::min(a.experts, a.rows);
+  const GemvPlan p = plan(F8, a.rows, groups, a.N, a.K, num_sms);
+  return p.bands == 1 ? launch_typed<F8, DT, SRC, 1>(p, a, groups, stream, pdl)
+                      : launch_typed<F8, DT, SRC, 2>(p, a, groups, stream, pdl);
+}
+
+template <int DT>
+cudaError_t launch_dtype(bool e4m3, int source, const ExpertGemvArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
+  if (!e4m3) return source == kSourceT ? launch_source<false, DT, kSourceT>(a, num_sms, stream, pdl) : cudaErrorInvalidValue;
+  if (source == kSourceT) return launch_source<true, DT, kSourceT>(a, num_sms, stream, pdl);
+  if (source == kSourceF32) return launch_source<true, DT, kSourceF32>(a, num_sms, stream, pdl);
+  return launch_source<true, DT, kSourceCodes>(a, num_sms, stream, pdl);
+}
+
+}  // namespace
+
+bool expert_gemv_fits(bool e4m3, int rows, int K) {
+  const int KB = (K + (e4m3 ? 127 : 63)) / (e4m3 ? 128 : 64);
+  int splits = 1;
+  for (int s : {2, 4, 8})
+    if ((s - 1) * ((KB + s - 1) / s) < KB) splits = s;
+    else break;
+  return smem_of(e4m3, rows, KB, 2, splits) <= kSmemMax && smem_of(e4m3, rows, KB, 1, splits) <= kSmemMax;
+}
+
+cudaError_t launch_expert_gemv(int dtype, bool e4m3, int source, const ExpertGemvArgs& a, int num_sms,
+                               cudaStream_t stream, bool pdl) {
+  if (!expert_gemv_fits(e4m3, a.rows, a.K)) return cudaErrorInvalidValue;
+  return dtype == kF16 ? launch_dtype<kF16>(e4m3, source, a, num_sms, stream, pdl)
+                       : launch_dtype<kBF16>(e4m3, source, a, num_sms, stream, pdl);
+}
+
+}  // namespace cq

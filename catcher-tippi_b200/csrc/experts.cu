@@ -1,9 +1,11 @@
 // Host layer of the fp8 linear and the linears of experts; see experts.hpp.
 #include "experts.hpp"
 
+#include <algorithm>
 #include <string>
 
 #include "expert_gemm.hpp"
+#include "expert_gemv.hpp"
 #include "expert_ops.hpp"
 #include "qlinear.hpp"
 
@@ -68,39 +70,6 @@ int device_of(const void* p, const char* what) {
   if (attr.type != cudaMemoryTypeDevice && attr.type != cudaMemoryTypeManaged)
     throw_invalid(std::string(what) + " must be device memory");
   return attr.device;
-}
-
-// Rows in a workspace, as the product takes them: codes and scales, or T.
-struct StagedRows {
-  void* x;
-  float* scales;
-  int64_t ld;
-};
-StagedRows take_rows(Arena& arena, int64_t rows, int cols, bool e4m3) {
-  StagedRows s{};
-  if (e4m3) {
-    s.ld = round_up(cols, kBlock);
-    s.x = arena.take<uint8_t>(rows * s.ld);
-    s.scales = arena.take<float>(rows * (s.ld / kBlock));
-  } else {
-    s.ld = round_up(cols, 8);
-    s.x = arena.take<uint16_t>(rows * s.ld);
-  }
-  return s;
-}
-
-// Brings rows of T (in the order of row_index where given) to the form that
-// the product takes.
-ExpertLinear::Rows stage_rows(const StagedRows& s, const void* x, int64_t ldx, const int32_t* row_index, int x_rows,
-                              int rows, int cols, cq_dtype dtype, bool e4m3, cudaStream_t stream) {
-  if (e4m3) {
-    const cq::QuantizeRowsArgs q{x, ldx, row_index, x_rows, rows, cols, static_cast<uint8_t*>(s.x), s.ld, s.scales};
-    check_cuda(cq::launch_quantize_rows(dtype, q, stream, pdl_enabled()), "quantize rows");
-  } else {
-    const cq::GatherRowsArgs g{x, ldx, row_index, x_rows, rows, cols, s.x, s.ld};
-    check_cuda(cq::launch_gather_rows(g, stream, pdl_enabled()), "gather rows");
-  }
-  return {s.x, s.ld, s.scales};
 }
 
 }  // namespace
@@ -173,11 +142,17 @@ std::unique_ptr<ExpertLinear> ExpertLinear::from_f32(const float* weight, const 
                                         CQ_WEIGHT_E4M3, dtype, device);
 }
 
-size_t ExpertLinear::workspace(int rows) const {
-  if (rows == 0) return 0;
-  Arena arena(nullptr);
-  take_rows(arena, rows, K_, e4m3());
-  return arena.used();
+size_t ExpertLinear::staging_bytes(int64_t rows) const {
+  if (!e4m3()) return rows * round_up(K_, 8) * 2;
+  const int64_t ld = round_up(K_, kBlock);
+  return round_up(rows * ld, 256) + rows * (ld / kBlock) * sizeof(float);
+}
+
+size_t ExpertLinear::workspace(int rows) const { return round_up(staging_bytes(rows), 256); }
+
+bool ExpertLinear::few_rows(int rows, bool grouped) const {
+  const int groups = grouped ? std::min(experts_, rows) : 1;
+  return rows <= 16 * groups && rows <= 64 && cq::expert_gemv_fits(e4m3(), rows, K_);
 }
 
 void ExpertLinear::check_rows(const void* x, int64_t ldx, int rows, const void* y, int64_t ldy, int act) const {
@@ -190,10 +165,36 @@ void ExpertLinear::check_rows(const void* x, int64_t ldx, int rows, const void* 
 }
 
 void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, int out, void* y, int64_t ldy, int act,
-                           cudaStream_t stream) const {
+                           void* staging, cudaStream_t stream) const {
   DeviceContext& ctx = device_context(device_);
+  const bool pdl = pdl_enabled();
+  if (out != cq::kOutCodes && few_rows(rows, offsets != nullptr)) {
+    const cq::ExpertGemvArgs a{x.x,           x.ld,  x.row_index,        x.x_rows,     x.scales, rows,
+                               weight_.get(), ldw_,  scales_.as<float>(), bias_.get(), offsets,  experts_,
+                               N_,            K_,    act,                out == cq::kOutF32, y,  ldy};
+    check_cuda(cq::launch_expert_gemv(dtype_, e4m3(), x.source, a, ctx.num_sms, stream, pdl), "expert product");
+    return;
+  }
+  // rows as the tile copies take them: codes, or 16-byte aligned rows of T
+  const void* from = x.x;
+  int64_t ld = x.ld;
+  const float* x_scales = x.scales;
+  if (e4m3() && x.source != cq::kSourceCodes) {
+    ld = round_up(K_, kBlock);
+    float* s = reinterpret_cast<float*>(static_cast<char*>(staging) + round_up(rows * ld, 256));
+    const cq::QuantizeRowsArgs q{x.x, x.ld, x.row_index, x.x_rows, rows, K_, static_cast<uint8_t*>(staging), ld, s};
+    check_cuda(cq::launch_quantize_rows(x.source == cq::kSourceF32 ? static_cast<int>(CQ_F32) : dtype_, q, stream, pdl),
+               "quantize rows");
+    from = staging;
+    x_scales = s;
+  } else if (!e4m3() && (x.row_index != nullptr || x.ld % 8 != 0 || (reinterpret_cast<uintptr_t>(x.x) & 15) != 0)) {
+    ld = round_up(K_, 8);
+    const cq::GatherRowsArgs g{x.x, x.ld, x.row_index, x.x_rows, rows, K_, staging, ld};
+    check_cuda(cq::launch_gather_rows(g, stream, pdl), "gather rows");
+    from = staging;
+  }
   cq::ExpertGemmArgs a{};
-  a.x_scales = x.scales;
+  a.x_scales = x_scales;
   a.w_scales = scales_.as<float>();
   a.bias = bias_.get();
   a.offsets = offsets;
@@ -206,13 +207,13 @@ void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, int 
   a.y = y;
   a.ldy = ldy;
   a.status = ctx.status;
-  const cq::ExpertGemmConfig cfg = cq::plan_expert_gemm(e4m3(), rows, experts_, N_, K_, false, ctx.num_sms);
+  const cq::ExpertGemmConfig cfg =
+      cq::plan_expert_gemm(e4m3(), rows, experts_, N_, K_, out == cq::kOutCodes, ctx.num_sms);
   const int size = e4m3() ? 1 : 2, k = 128 / size;
-  const CUtensorMap xmap = make_map_2d(x.x, size, rows, K_, x.ld, cq::kGemmRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
+  const CUtensorMap xmap = make_map_2d(from, size, rows, K_, ld, cq::kGemmRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
   const CUtensorMap wmap =
       make_map_2d(weight_.get(), size, experts_ * N_, K_, ldw_, cfg.bn / cfg.pair, k, CU_TENSOR_MAP_SWIZZLE_128B);
-  check_cuda(cq::launch_expert_gemm(dtype_, e4m3(), xmap, wmap, cfg, a, ctx.num_sms, stream, pdl_enabled()),
-             "expert product");
+  check_cuda(cq::launch_expert_gemm(dtype_, e4m3(), xmap, wmap, cfg, a, ctx.num_sms, stream, pdl), "expert product");
 }
 
 void ExpertLinear::forward(const void* x, int64_t ldx, int rows, const int32_t* offsets, void* y, int64_t ldy, int act,
@@ -222,12 +223,7 @@ void ExpertLinear::forward(const void* x, int64_t ldx, int rows, const int32_t* 
   if (rows == 0) return;
   check_workspace(workspace, workspace_bytes, this->workspace(rows));
   DeviceGuard guard(device_);
-  Rows r{x, ldx, nullptr};
-  if (e4m3() || ldx % 8 != 0 || (reinterpret_cast<uintptr_t>(x) & 15) != 0) {
-    Arena arena(workspace);
-    r = stage_rows(take_rows(arena, rows, K_, e4m3()), x, ldx, nullptr, rows, rows, K_, dtype_, e4m3(), stream);
-  }
-  product(r, rows, offsets, cq::kOutT, y, ldy, act, stream);
+  product({cq::kSourceT, x, ldx, nullptr, nullptr, rows}, rows, offsets, cq::kOutT, y, ldy, act, workspace, stream);
 }
 
 void ExpertLinear::forward_codes(const uint8_t* codes, int64_t ld, const float* scales, int rows, void* y, int64_t ldy,
@@ -239,7 +235,7 @@ void ExpertLinear::forward_codes(const uint8_t* codes, int64_t ld, const float* 
   if (scales == nullptr) throw_invalid("scales must not be null");
   check_aligned(scales, 4, "scales");
   DeviceGuard guard(device_);
-  product({codes, ld, scales}, rows, nullptr, cq::kOutT, y, ldy, act, stream);
+  product({cq::kSourceCodes, codes, ld, scales, nullptr, rows}, rows, nullptr, cq::kOutT, y, ldy, act, nullptr, stream);
 }
 
 void quantize_rows(const void* x, int64_t ldx, const int32_t* row_index, int x_rows, int rows, int cols,
@@ -339,9 +335,10 @@ struct FfnScratch {
   float* weight;
   void* route;
   size_t route_bytes;
-  StagedRows x, h;
-  float* h_f32;  // e4m3: up's result, before it goes to codes
-  float* z;      // f32: the sum over a token's experts is rounded once
+  void *x, *h_staged;  // the products' staging
+  void* h;             // up's result: T, or f32 on its way to e4m3
+  int64_t ld_h;
+  float* z;  // f32: the sum over a token's experts is rounded once
 };
 
 FfnScratch take_ffn(Arena& arena, const ExpertLinear& up, const ExpertLinear& down, int tokens, int top) {
@@ -354,9 +351,10 @@ FfnScratch take_ffn(Arena& arena, const ExpertLinear& up, const ExpertLinear& do
   s.position = arena.take<int32_t>(pairs);
   s.route_bytes = route_workspace_bytes(tokens, up.experts(), top);
   s.route = arena.take<uint8_t>(s.route_bytes);
-  s.x = take_rows(arena, pairs, up.input_dims(), up.e4m3());
-  s.h = take_rows(arena, pairs, up.output_dims(), up.e4m3());
-  if (up.e4m3()) s.h_f32 = arena.take<float>(pairs * up.output_dims());
+  s.x = arena.take<uint8_t>(up.staging_bytes(pairs));
+  s.h_staged = up.e4m3() ? arena.take<uint8_t>(down.staging_bytes(pairs)) : nullptr;
+  s.ld_h = round_up(up.output_dims(), 8);
+  s.h = arena.take<uint8_t>(pairs * s.ld_h * (up.e4m3() ? 4 : 2));
   s.z = arena.take<float>(pairs * down.output_dims());
   return s;
 }
@@ -386,7 +384,7 @@ void expert_ffn(const ExpertLinear& up, const ExpertLinear& down, const void* x,
   const size_t need = expert_ffn_workspace(up, down, tokens, top);
   check_act(act);
   check_dtype(logits_dtype);
-  const int d = up.input_dims(), ff = up.output_dims(), out = down.output_dims();
+  const int d = up.input_dims(), out = down.output_dims();
   if (ldx < d) throw_invalid("input row stride " + std::to_string(ldx) + " is smaller than " + std::to_string(d));
   if (ldy < out) throw_invalid("output row stride " + std::to_string(ldy) + " is smaller than " + std::to_string(out));
   if (tokens == 0) return;
@@ -400,16 +398,10 @@ void expert_ffn(const ExpertLinear& up, const ExpertLinear& down, const void* x,
   DeviceGuard guard(up.device());
   route(logits, ld_logits, logits_dtype, tokens, up.experts(), top, renormalize, s.expert, s.weight, s.offsets,
         s.token, s.position, s.route, s.route_bytes, stream);
-  const ExpertLinear::Rows rows =
-      stage_rows(s.x, x, ldx, s.token, tokens, pairs, d, up.dtype(), up.e4m3(), stream);
-  ExpertLinear::Rows h{s.h.x, s.h.ld, s.h.scales};
-  if (up.e4m3()) {
-    up.product(rows, pairs, s.offsets, cq::kOutF32, s.h_f32, ff, act, stream);
-    h = stage_rows(s.h, s.h_f32, ff, nullptr, pairs, pairs, ff, CQ_F32, true, stream);
-  } else {
-    up.product(rows, pairs, s.offsets, cq::kOutT, s.h.x, s.h.ld, act, stream);
-  }
-  down.product(h, pairs, s.offsets, cq::kOutF32, s.z, out, CQ_ACT_NONE, stream);
+  up.product({cq::kSourceT, x, ldx, nullptr, s.token, tokens}, pairs, s.offsets,
+             up.e4m3() ? cq::kOutF32 : cq::kOutT, s.h, s.ld_h, act, s.x, stream);
+  down.product({up.e4m3() ? cq::kSourceF32 : cq::kSourceT, s.h, s.ld_h, nullptr, nullptr, pairs}, pairs, s.offsets,
+               cq::kOutF32, s.z, out, CQ_ACT_NONE, s.h_staged, stream);
   const cq::CombineArgs c{s.z, out, s.position, s.weight, pairs, tokens, top, out, y, ldy, 1};
   check_cuda(cq::launch_combine(up.dtype(), c, stream, pdl_enabled()), "combine");
 }

@@ -37,16 +37,26 @@ class ExpertLinear {
   cq_dtype dtype() const { return dtype_; }
   int device() const { return device_; }
 
-  // Rows as the product's tile copies take them: 16-byte aligned rows of T, or
-  // of codes with their scales [k blocks][rows].
+  // Rows of a product: T, f32 (e4m3 weights only) or e4m3 codes with their
+  // scales [k blocks][rows], as cq::ExpertSource says; row r is x row
+  // row_index[r] where that is given (T only).
   struct Rows {
+    int source;
     const void* x;
     int64_t ld;
     const float* scales;
+    const int32_t* row_index;
+    int x_rows;
   };
+  // Bytes in which product() brings rows to the form that the tensor cores'
+  // tile copies take.
+  size_t staging_bytes(int64_t rows) const;
   // The product alone, arguments checked; out: a cq::ExpertOut.
   void product(const Rows& x, int rows, const int32_t* offsets, int out, void* y, int64_t ldy, int act,
-               cudaStream_t stream) const;
+               void* staging, cudaStream_t stream) const;
+  // True when calls on `rows` rows stream the weights (expert_gemv.cu) instead
+  // of running tiles on the tensor cores (expert_gemm.cu).
+  bool few_rows(int rows, bool grouped) const;
 
  private:
   ExpertLinear(int experts, int output_dims, int input_dims, cq_weight_format format, cq_dtype dtype, int device);
