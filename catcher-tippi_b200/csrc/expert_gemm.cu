@@ -126,7 +126,17 @@ __device__ __forceinline__ void fma2(float& a, float& b, uint32_t x, uint32_t y,
       "fma.rn.f32x2 t, p, q, t;\n\tmov.b64 {%0, %1}, t;\n\t}"
       : "+f"(a), "+f"(b) : "r"(x), "r"(y), "f"(s));
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for the warp's tensor-memory loads.  The loaded registers pass through
+// it, so that no use of them can be scheduled before it.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+               "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+               "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+               "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
 
 // Shared-memory matrix descriptor, K-major, 128-byte swizzle: 8-row atoms of
 // 128-byte rows, 1024 bytes apart.
@@ -194,6 +204,13 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, int* 
   }
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+  return ok != 0;
+}
+
 // --------------------------------------------------------------- tile list
 
 // Tiles of all experts in order: start[e] is the first row of expert e, tile[e]
@@ -248,6 +265,18 @@ __device__ __forceinline__ void build_list(const ExpertGemmArgs& a, TileList l, 
 
 struct Tile {
   int expert, m0, end, n0;
+};
+
+// A place in a ring of barriers and the parity of its next phase.
+struct Ring {
+  int at = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int size) {
+    if (++at == size) {
+      at = 0;
+      phase ^= 1u;
+    }
+  }
 };
 
 // The t-th tile; `e` only moves forward.
@@ -327,7 +356,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(part_empty + 1);
   __shared__ __align__(16) float bias_s[256];
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the same in all lanes, and known to be
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = CG == 2 || S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int worker = blockIdx.x / (CG * S), workers = gridDim.x / (CG * S);
   const int tile_rows = kGemmRows * CG, tiles_n = (a.N + BN - 1) / BN;
@@ -366,57 +396,67 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
       // ---------------------------------------------------------- copies
       const uint64_t keep = l2_policy_evict_normal();
       const uint32_t bytes = static_cast<uint32_t>(L.stage_bytes) * CG;
-      int e = 0, it = 0;
+      int e = 0, issued = 0;
+      Ring ring;
       for (int t = worker; t < total && ok; t += workers) {
         const Tile tile = find_tile(list, t, tile_rows, tiles_n, BN, e);
         const int m = tile.m0 + (CG == 2 ? rank * kGemmRows : 0);
         const int w = tile.expert * a.N + tile.n0 + (CG == 2 ? rank * (BN / 2) : 0);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % stages;
-          if (!wait_phase<false>(&empty[s], ((it / stages) & 1) ^ 1, a.status)) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!wait_phase<false>(&empty[ring.at], ring.phase ^ 1u, a.status)) {
             ok = false;
             break;
           }
-          uint8_t* st = smem + s * L.stage_bytes;
-          uint32_t bar = smem_u32(&full[s]);
+          uint8_t* st = smem + ring.at * L.stage_bytes;
+          uint32_t bar = smem_u32(&full[ring.at]);
           if (CG == 2) bar = mapa_shared(bar, 0);
-          if (rank == 0 || CG == 1) mbar_arrive_expect_tx(&full[s], bytes);
-          load_tile<CG>(st, &xmap, kb * kElems, m, bar, keep);
-          load_tile<CG>(st + kXBytes, &wmap, kb * kElems, w, bar, keep);
+          if (elect_one()) {
+            if (rank == 0 || CG == 1) mbar_arrive_expect_tx(&full[ring.at], bytes);
+            load_tile<CG>(st, &xmap, kb * kElems, m, bar, keep);
+            load_tile<CG>(st + kXBytes, &wmap, kb * kElems, w, bar, keep);
+          }
+          __syncwarp();
+          ring.next(stages);
+          ++issued;
         }
       }
       if (!ok && (rank == 0 || CG == 1))  // a wait ran out: let the copies in flight land before the CTA ends
-        for (int i = max(0, it - stages); i < it; ++i) wait_phase<false>(&full[i % stages], (i / stages) & 1, a.status);
-    } else if (warp == 1 && lane == 0 && (CG == 1 || rank == 0)) {
+        for (int i = max(0, issued - stages); i < issued; ++i) wait_phase<false>(&full[i % stages], (i / stages) & 1, a.status);
+    } else if (warp == 1 && (CG == 1 || rank == 0)) {
       // ---------------------------------------------------------- products
       const uint32_t idesc = mma_idesc<FMT, CG>(BN);
+      // The tensor pipe queues few products, so this loop's scalar work has to
+      // fit under four of them: the whole warp runs it, with values that are
+      // the same in all lanes, and one lane issues; ring places by counters,
+      // descriptors by adds (every address field stays below 2^14).
       const uint64_t base = sw128_desc(smem_u32(smem));
-      int it = 0, use = 0;
+      const uint32_t stage_units = static_cast<uint32_t>(L.stage_bytes) >> 4;
+      Ring ring, acc;
       for (int t = worker; t < total && ok; t += workers) {
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int b = use % buffers;
+        for (int kb = kb0; kb < kb1; ++kb) {
           const bool first = FMT == kFmtE4M3 || kb == kb0, last = FMT == kFmtE4M3 || kb == kb1 - 1;
-          if (first) ok = ok && wait_phase<false>(&acc_empty[b], ((use / buffers) & 1) ^ 1, a.status);
-          const int s = it % stages;
-          ok = ok && wait_phase<false>(&full[s], (it / stages) & 1, a.status);
+          if (first) ok = wait_phase<false>(&acc_empty[acc.at], acc.phase ^ 1u, a.status);
+          ok = ok && wait_phase<false>(&full[ring.at], ring.phase, a.status);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t da = base + static_cast<uint64_t>((s * L.stage_bytes) >> 4);
+          const uint64_t da = base + ring.at * stage_units;
           const uint64_t db = da + (kXBytes >> 4);
-          const uint32_t d = tmem + static_cast<uint32_t>(b * BN);
-          tc_mma<FMT, CG>(d, da, db, idesc, !first);
-          tc_mma<FMT, CG>(d, da + 2, db + 2, idesc, 1);
-          tc_mma<FMT, CG>(d, da + 4, db + 4, idesc, 1);
-          tc_mma<FMT, CG>(d, da + 6, db + 6, idesc, 1);
-          tc_commit<CG>(&empty[s]);
-          if (last) {
-            tc_commit<CG>(&acc_full[b]);
-            ++use;
+          const uint32_t d = tmem + static_cast<uint32_t>(acc.at * BN);
+          if (elect_one()) {
+            tc_mma<FMT, CG>(d, da, db, idesc, !first);
+            tc_mma<FMT, CG>(d, da + 2, db + 2, idesc, 1);
+            tc_mma<FMT, CG>(d, da + 4, db + 4, idesc, 1);
+            tc_mma<FMT, CG>(d, da + 6, db + 6, idesc, 1);
+            tc_commit<CG>(&empty[ring.at]);
+            if (last) tc_commit<CG>(&acc_full[acc.at]);
           }
+          __syncwarp();
+          ring.next(stages);
+          if (last) acc.next(buffers);
         }
       }
     }
@@ -442,7 +482,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
 
-    int e = 0, use = 0, turn = 0;
+    int e = 0, turn = 0;
+    Ring ring;
     for (int t = worker; t < total && ok; t += workers, ++turn) {
       const Tile tile = find_tile(list, t, tile_rows, tiles_n, BN, e);
       const int64_t row = tile.m0 + (CG == 2 ? rank * kGemmRows : 0) + local;
@@ -485,44 +526,48 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (kb + i < kb1) {
-              const int b = use % buffers;
-              ok = ok && wait_phase<false>(&acc_full[b], (use / buffers) & 1, a.status);
-              ++use;
+              ok = ok && wait_phase<false>(&acc_full[ring.at], ring.phase, a.status);
               tc_fence_after();
-              const uint32_t src = lane_base + static_cast<uint32_t>(b * BN);
+              const uint32_t src = lane_base + static_cast<uint32_t>(ring.at * BN);
+              // the next columns are on their way while these are added
+              uint32_t r[2][32];
+              tmem_ld32(src, r[0]);
 #pragma unroll
               for (int c = 0; c < W; c += 32) {
-                uint32_t r[32];
-                tmem_ld32(src + c, r);
-                tmem_wait_ld();
+                tmem_wait_ld(r[(c / 32) & 1]);
+                if (c + 32 < W) {
+                  tmem_ld32(src + c + 32, r[(c / 32 + 1) & 1]);
+                } else {
+                  // all read: the buffer goes back before the last sums
+                  tc_fence_before();
+                  if (lane == 0) mbar_arrive_remote(acc_empty0 + ring.at * 8);
+                }
+                const uint32_t(&v)[32] = r[(c / 32) & 1];
 #pragma unroll
-                for (int j = 0; j < 32; j += 2) fma2(acc[c + j], acc[c + j + 1], r[j], r[j + 1], now[i]);
+                for (int j = 0; j < 32; j += 2) fma2(acc[c + j], acc[c + j + 1], v[j], v[j + 1], now[i]);
               }
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_remote(acc_empty0 + b * 8);
+              ring.next(buffers);
             }
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) next[i] = fx[i] * fw[i];
         }
       } else {
-        const int b = use % buffers;
-        ok = ok && wait_phase<false>(&acc_full[b], (use / buffers) & 1, a.status);
-        ++use;
+        ok = ok && wait_phase<false>(&acc_full[ring.at], ring.phase, a.status);
         tc_fence_after();
-        const uint32_t src = lane_base + static_cast<uint32_t>(b * BN);
+        const uint32_t src = lane_base + static_cast<uint32_t>(ring.at * BN);
 #pragma unroll
         for (int c = 0; c < W; c += 32) {
           uint32_t r[32];
           tmem_ld32(src + c, r);
-          tmem_wait_ld();
+          tmem_wait_ld(r);
 #pragma unroll
           for (int j = 0; j < 32; ++j) acc[c + j] = __uint_as_float(r[j]);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_remote(acc_empty0 + b * 8);
+        if (lane == 0) mbar_arrive_remote(acc_empty0 + ring.at * 8);
+        ring.next(buffers);
       }
       if (!ok) break;
 

@@ -15,7 +15,8 @@ namespace {
 // One block of 128 values per half warp, eight values a lane: the largest
 // magnitude by shuffles, then the codes, eight bytes a lane.  Bound by memory:
 // (2 + 1) bytes a value for 16-bit rows.
-constexpr int kQuantThreads = 256;
+constexpr int kQuantThreads = 256, kQuantHalves = kQuantThreads / 16;
+constexpr int kQuantItems = 4;  // blocks a half warp has in flight
 
 template <int DT>
 __device__ __forceinline__ void load8(const void* row, int k, int cols, bool aligned, float (&v)[8]) {
@@ -53,42 +54,48 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const Quan
   pdl_launch_dependents();
   pdl_wait();
   constexpr int kSize = DT == kF32 ? 4 : 2;
-  const int blocks = (a.cols + kFp8Block - 1) / kFp8Block;
-  const int64_t items = static_cast<int64_t>(a.rows) * blocks;
+  const uint32_t blocks = (a.cols + kFp8Block - 1) / kFp8Block;
+  const uint32_t items = static_cast<uint32_t>(a.rows) * blocks;  // below 2^32: x fits the device's memory
   const bool aligned = ((a.ldx * kSize) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
-  const int half = threadIdx.x >> 4, lane = threadIdx.x & 15;
-  constexpr int kHalves = kQuantThreads / 16;
-  // every lane of a warp makes the same number of turns: the shuffles below
-  // are the warp's
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kHalves; base < items;
-       base += static_cast<int64_t>(gridDim.x) * kHalves) {
-    const int64_t item = base + half;
-    bool live = item < items;
-    const int64_t row = live ? item / blocks : 0;
-    const int block = live ? static_cast<int>(item - row * blocks) : 0;
-    int64_t src = row;
-    if (live && a.row_index != nullptr) {
-      src = a.row_index[row];
-      live = src >= 0 && src < a.x_rows;
-    }
-    const int k = block * kFp8Block + lane * 8;
-    float v[8];
+  const uint32_t half = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  const uint32_t first = blockIdx.x * (kQuantHalves * kQuantItems) + half;
+  // all loads before the first use
+  float v[kQuantItems][8];
+  uint32_t row[kQuantItems], block[kQuantItems];
+  bool live[kQuantItems];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    if (live) load8<DT>(reinterpret_cast<const char*>(a.x) + src * a.ldx * kSize, k, a.cols, aligned, v);
+  for (int u = 0; u < kQuantItems; ++u) {
+    const uint32_t item = first + u * kQuantHalves;
+    live[u] = item < items;
+    row[u] = live[u] ? item / blocks : 0;
+    block[u] = item - row[u] * blocks;
+    int64_t src = row[u];
+    if (live[u] && a.row_index != nullptr) {
+      src = a.row_index[row[u]];
+      live[u] = src >= 0 && src < a.x_rows;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
+    if (live[u])
+      load8<DT>(reinterpret_cast<const char*>(a.x) + src * a.ldx * kSize, block[u] * kFp8Block + lane * 8, a.cols,
+                aligned, v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kQuantItems; ++u) {
     uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, finite_magnitude(v[j]));
+    for (int j = 0; j < 8; ++j) top = max(top, finite_magnitude(v[u][j]));
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    if (!live) continue;
+    if (!live[u]) continue;
     const int e = fp8_scale_exponent(top);
     const float inv = pow2f(-e);
     uint2 out;
-    out.x = e4m3x2(v[0] * inv, v[1] * inv) | (e4m3x2(v[2] * inv, v[3] * inv) << 16);
-    out.y = e4m3x2(v[4] * inv, v[5] * inv) | (e4m3x2(v[6] * inv, v[7] * inv) << 16);
-    if (k < a.ld) *reinterpret_cast<uint2*>(a.codes + row * a.ld + k) = out;
-    if (lane == 0) a.scales[static_cast<int64_t>(block) * a.rows + row] = pow2f(e);
+    out.x = e4m3x2(v[u][0] * inv, v[u][1] * inv) | (e4m3x2(v[u][2] * inv, v[u][3] * inv) << 16);
+    out.y = e4m3x2(v[u][4] * inv, v[u][5] * inv) | (e4m3x2(v[u][6] * inv, v[u][7] * inv) << 16);
+    const uint32_t k = block[u] * kFp8Block + lane * 8;
+    if (k < a.ld) *reinterpret_cast<uint2*>(a.codes + row[u] * a.ld + k) = out;
+    if (lane == 0) a.scales[static_cast<int64_t>(block[u]) * a.rows + row[u]] = pow2f(e);
   }
 }
 
@@ -398,41 +405,95 @@ cudaError_t route_dtype(const RouteArgs& a, cudaStream_t stream, bool pdl) {
 // ------------------------------------------------------------------ combine
 
 // A thread sums eight columns of one token.  Bound by memory: the rows of z
-// once, y once.
-template <int DT, int ZT>
+// once, y once.  Four experts' rows are on their way before the first is
+// added.  `VEC`: every row is 16-byte aligned and dims a multiple of 8.
+template <int T>
+struct Raw8 {
+  uint4 u[T == kF32 ? 2 : 1];
+};
+template <int T>
+__device__ __forceinline__ void add_raw8(const Raw8<T>& r, float w, float (&acc)[8]) {
+  if constexpr (T == kF32) {
+    const uint32_t b[8] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w, r.u[1].x, r.u[1].y, r.u[1].z, r.u[1].w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, __uint_as_float(b[j]), acc[j]);
+  } else {
+    const uint32_t b[4] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float lo, hi;
+      if constexpr (T == kBF16) {
+        lo = __uint_as_float(b[j] << 16), hi = __uint_as_float(b[j] & 0xFFFF0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[j]));
+        lo = f.x, hi = f.y;
+      }
+      acc[2 * j] = fmaf(w, lo, acc[2 * j]);
+      acc[2 * j + 1] = fmaf(w, hi, acc[2 * j + 1]);
+    }
+  }
+}
+
+template <int DT, int ZT, bool VEC>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  const int chunks = (a.dims + 7) / 8;
   constexpr int kSize = ZT == kF32 ? 4 : 2;
-  const bool zv = (a.ldz & 7) == 0 && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0;
-  const bool yv = (a.ldy & 7) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
-  const int64_t items = static_cast<int64_t>(a.tokens) * chunks;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < items;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t t = i / chunks;
-    const int d = static_cast<int>(i - t * chunks) * 8;
-    float acc[8] = {};
-    for (int j = 0; j < a.top; ++j) {
-      const int p = __ldg(a.position + t * a.top + j);
-      if (p < 0 || p >= a.rows) continue;
-      const float w = __ldg(a.weight + t * a.top + j);
-      float v[8];
-      load8<ZT>(reinterpret_cast<const char*>(a.z) + p * a.ldz * kSize, d, a.dims, zv, v);
+  const uint32_t chunks = (a.dims + 7) / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= static_cast<int64_t>(a.tokens) * chunks) return;
+  const int64_t t = i / chunks;
+  const int d = static_cast<int>(i - t * chunks) * 8;
+  const int32_t* position = a.position + t * a.top;
+  const float* weight = a.weight + t * a.top;
+  float acc[8] = {};
+  for (int j0 = 0; j0 < a.top; j0 += 4) {
+    if constexpr (VEC) {
+      Raw8<ZT> raw[4];
+      float w[4];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) acc[c] = fmaf(w, v[c], acc[c]);
-    }
-    uint16_t* out = reinterpret_cast<uint16_t*>(a.y) + t * a.ldy + d;
-    if (yv && d + 8 <= a.dims) {
-      uint32_t u[4];
+      for (int u = 0; u < 4; ++u) {
+        const int p = j0 + u < a.top ? __ldg(position + j0 + u) : -1;
+        const bool ok = p >= 0 && p < a.rows;
+        w[u] = ok ? __ldg(weight + j0 + u) : 0.0f;
+        const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(a.z) + (p * a.ldz + d) * kSize);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) u[c] = pack_t<DT>(acc[2 * c], acc[2 * c + 1]);
-      *reinterpret_cast<uint4*>(out) = make_uint4(u[0], u[1], u[2], u[3]);
+        for (int h = 0; h < (ZT == kF32 ? 2 : 1); ++h) raw[u].u[h] = ok ? from[h] : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) add_raw8<ZT>(raw[u], w[u], acc);
     } else {
-      for (int c = 0; c < 8; ++c)
-        if (d + c < a.dims) st_t<DT>(out, c, acc[c]);
+      for (int j = j0; j < min(j0 + 4, a.top); ++j) {
+        const int p = __ldg(position + j);
+        if (p < 0 || p >= a.rows) continue;
+        const float w = __ldg(weight + j);
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (d + c < a.dims) acc[c] = fmaf(w, ld_t<ZT>(reinterpret_cast<const char*>(a.z) + p * a.ldz * kSize, d + c), acc[c]);
+      }
     }
   }
+  uint16_t* out = reinterpret_cast<uint16_t*>(a.y) + t * a.ldy + d;
+  if constexpr (VEC) {
+    uint32_t u[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) u[c] = pack_t<DT>(acc[2 * c], acc[2 * c + 1]);
+    *reinterpret_cast<uint4*>(out) = make_uint4(u[0], u[1], u[2], u[3]);
+  } else {
+    for (int c = 0; c < 8; ++c)
+      if (d + c < a.dims) st_t<DT>(out, c, acc[c]);
+  }
+}
+
+template <int DT, int ZT>
+cudaError_t combine_typed(const CombineArgs& a, cudaStream_t stream, bool pdl) {
+  const int64_t items = static_cast<int64_t>(a.tokens) * ((a.dims + 7) / 8);
+  const dim3 grid(static_cast<unsigned>((items + 255) / 256));
+  const int64_t bytes = ZT == kF32 ? 4 : 2;
+  const bool vec = a.dims % 8 == 0 && (a.ldz * bytes) % 16 == 0 && a.ldy % 8 == 0 &&
+                   (reinterpret_cast<uintptr_t>(a.z) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
+  return vec ? launch(combine_kernel<DT, ZT, true>, grid, dim3(256), 0, stream, pdl, a)
+             : launch(combine_kernel<DT, ZT, false>, grid, dim3(256), 0, stream, pdl, a);
 }
 
 }  // namespace
@@ -440,7 +501,8 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
 cudaError_t launch_quantize_rows(int dtype, const QuantizeRowsArgs& a, cudaStream_t stream, bool pdl) {
   const int64_t items = static_cast<int64_t>(a.rows) * ((a.cols + kFp8Block - 1) / kFp8Block);
   if (items == 0) return cudaSuccess;
-  const int grid = static_cast<int>(std::min<int64_t>((items + 15) / 16, 148 * 8 * 4));
+  constexpr int kPer = kQuantHalves * kQuantItems;
+  const int grid = static_cast<int>((items + kPer - 1) / kPer);
   switch (dtype) {
     case kF16: return launch(quantize_rows_kernel<kF16>, dim3(grid), dim3(kQuantThreads), 0, stream, pdl, a);
     case kBF16: return launch(quantize_rows_kernel<kBF16>, dim3(grid), dim3(kQuantThreads), 0, stream, pdl, a);
@@ -483,14 +545,9 @@ cudaError_t launch_route(int dtype, const RouteArgs& a, cudaStream_t stream, boo
 }
 
 cudaError_t launch_combine(int dtype, const CombineArgs& a, cudaStream_t stream, bool pdl) {
-  const int64_t items = static_cast<int64_t>(a.tokens) * ((a.dims + 7) / 8);
-  if (items == 0) return cudaSuccess;
-  const int grid = static_cast<int>(std::min<int64_t>((items + 255) / 256, 1 << 20));
-  if (a.z_f32)
-    return dtype == kF16 ? launch(combine_kernel<kF16, kF32>, dim3(grid), dim3(256), 0, stream, pdl, a)
-                         : launch(combine_kernel<kBF16, kF32>, dim3(grid), dim3(256), 0, stream, pdl, a);
-  return dtype == kF16 ? launch(combine_kernel<kF16, kF16>, dim3(grid), dim3(256), 0, stream, pdl, a)
-                       : launch(combine_kernel<kBF16, kBF16>, dim3(grid), dim3(256), 0, stream, pdl, a);
+  if (a.tokens == 0) return cudaSuccess;
+  if (a.z_f32) return dtype == kF16 ? combine_typed<kF16, kF32>(a, stream, pdl) : combine_typed<kBF16, kF32>(a, stream, pdl);
+  return dtype == kF16 ? combine_typed<kF16, kF16>(a, stream, pdl) : combine_typed<kBF16, kBF16>(a, stream, pdl);
 }
 
 }  // namespace cq
