@@ -20,6 +20,7 @@
 //   warp 0      copies tiles of x and W (TMA, 128-byte swizzle) into a ring
 //   warp 1      issues tcgen05.mma
 //   warp 2      owns the tensor memory
+//   warp 3      e4m3: fetches the scales, eight k blocks ahead
 //   warps 4-11  epilogue: two groups of four warps, each half of the columns
 #include "expert_gemm.hpp"
 
@@ -43,20 +44,29 @@ constexpr int kMaxBuffers = 4;  // tensor-memory accumulators
 
 enum Format : int { kFmtE4M3 = 0, kFmtF16 = 1, kFmtBF16 = 2 };
 
+constexpr int kScaleBlocks = 8;  // k blocks of scales fetched at a time
+constexpr int kScaleSlots = 2;
+constexpr int kScaleBytes = kScaleBlocks * (kGemmRows + 2) * 4;
+constexpr int kStageOut = kStoreRows * kStoreBytes;  // one of a warp's two tile stores
+
 struct SmemPlan {
-  int stage_bytes, stages, part_off, list_off, bar_off, bytes;
+  int stage_bytes, stages, out_off, part_off, scale_off, list_off, bar_off, bytes;
 };
 
-__host__ __device__ inline SmemPlan plan_smem(int bn, int pair, int splits, int experts) {
+__host__ __device__ inline SmemPlan plan_smem(bool e4m3, int bn, int pair, int splits, int experts) {
   SmemPlan p{};
   p.stage_bytes = kXBytes + bn / pair * kRowBytes;
   const int part = splits > 1 ? bn * kGemmRows * 4 : 0;
   const int list = (2 * (experts + 2) * 4 + 15) / 16 * 16;
-  const int bars = (2 * kMaxStages + 2 * kMaxBuffers + 2) * 8 + 16;
-  p.stages = (kSmemLimit - 2048 - part - list - bars)  /* alignment, the bias */ / p.stage_bytes;
+  const int bars = (2 * kMaxStages + 2 * kMaxBuffers + 2 * kScaleSlots + 2) * 8 + 16;
+  const int scales = e4m3 ? kScaleSlots * kScaleBytes : 0;
+  const int rest = kEpiWarps * 2 * kStageOut + part + scales + list + bars;
+  p.stages = (kSmemLimit - 2048 - rest) / p.stage_bytes;  // 2048: alignment, and the bias
   if (p.stages > kMaxStages) p.stages = kMaxStages;
-  p.part_off = p.stages * p.stage_bytes;
-  p.list_off = p.part_off + part;
+  p.out_off = p.stages * p.stage_bytes;
+  p.part_off = p.out_off + kEpiWarps * 2 * kStageOut;
+  p.scale_off = p.part_off + part;
+  p.list_off = p.scale_off + scales;
   p.bar_off = p.list_off + list;
   p.bytes = p.bar_off + bars + 1024;  // + alignment
   return p;
@@ -327,6 +337,30 @@ __device__ __forceinline__ void store_values(const ExpertGemmArgs& a, int64_t ro
   }
 }
 
+// 64 bytes of each of a warp's 32 rows: through the warp's shared memory
+// (16-byte pieces in the 64-byte swizzle, free of bank conflicts) to one tile
+// store.  Whole sectors leave the SM in few requests; a store by each lane to
+// its own row touches 32 lines an instruction.  Two buffers take turns, so that
+// a piece waits for the one before the last.
+__device__ __forceinline__ void store_piece(uint8_t* out_s, int& turn, int lane, const uint32_t* w,
+                                            const CUtensorMap* ymap, int n, int row) {
+  uint8_t* buf = out_s + turn * kStageOut;
+  turn ^= 1;
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+  __syncwarp();
+#pragma unroll
+  for (int p = 0; p < 4; ++p)
+    *reinterpret_cast<uint4*>(buf + lane * kStoreBytes + ((p ^ ((lane >> 1) & 3)) << 4)) =
+        make_uint4(w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
+  fence_proxy_async_shared();
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(ymap)), "r"(n), "r"(row), "r"(smem_u32(buf)) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
+
 // The four warps of an epilogue group.
 __device__ __forceinline__ void group_sync(int half) {
   if (half == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -338,11 +372,11 @@ __device__ __forceinline__ void group_sync(int half) {
 template <int FMT, int DT, int CG, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
     expert_gemm_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
-                       const ExpertGemmArgs a) {
+                       const __grid_constant__ CUtensorMap ymap, const ExpertGemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int S = CG == 2 || BN == 256 ? 1 : a.splits;
-  const SmemPlan L = plan_smem(BN, CG, S, a.experts);
+  const SmemPlan L = plan_smem(FMT == kFmtE4M3, BN, CG, S, a.experts);
   const int stages = L.stages;
   constexpr int buffers = static_cast<int>(kTmemCols) / BN < kMaxBuffers ? static_cast<int>(kTmemCols) / BN : kMaxBuffers;
   float* part = reinterpret_cast<float*>(smem + L.part_off);
@@ -353,7 +387,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* acc_empty = acc_full + kMaxBuffers;
   uint64_t* part_full = acc_empty + kMaxBuffers;
   uint64_t* part_empty = part_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(part_empty + 1);
+  uint64_t* scale_full = part_empty + 1;
+  uint64_t* scale_empty = scale_full + kScaleSlots;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scale_empty + kScaleSlots);
+  // [slot][k block][row], then [slot][k block][column half]
+  float* scale_x = reinterpret_cast<float*>(smem + L.scale_off);
+  float* scale_w = scale_x + kScaleSlots * kScaleBlocks * kGemmRows;
   __shared__ __align__(16) float bias_s[256];
 
   // the same in all lanes, and known to be
@@ -369,6 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     prefetch_tensormap(&xmap);
     prefetch_tensormap(&wmap);
+    prefetch_tensormap(&ymap);
     for (int s = 0; s < kMaxStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -379,6 +419,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(part_full, S * kEpiWarps);
     mbar_init(part_empty, S * kEpiWarps);
+    for (int b = 0; b < kScaleSlots; ++b) {
+      mbar_init(&scale_full[b], 32);
+      mbar_init(&scale_empty[b], kEpiWarps);
+    }
     fence_mbar_init();
   }
   if (warp == 2) tmem_alloc<CG>(tmem_slot, kTmemCols);
@@ -459,6 +503,39 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (last) acc.next(buffers);
         }
       }
+    } else if (FMT == kFmtE4M3 && warp == 3) {
+      // ---------------------------------------------------------- scales
+      const int NBLK = (a.N + kFp8Block - 1) / kFp8Block;
+      int e = 0;
+      Ring ring;
+      for (int t = worker; t < total && ok; t += workers) {
+        const Tile tile = find_tile(list, t, tile_rows, tiles_n, BN, e);
+        const int row0 = tile.m0 + (CG == 2 ? rank * kGemmRows : 0) + lane;
+        const float* sw = a.w_scales + static_cast<int64_t>(tile.expert) * NBLK * KB;
+        const int blk0 = min(tile.n0 / kFp8Block, NBLK - 1), blk1 = min((tile.n0 + BN / 2) / kFp8Block, NBLK - 1);
+        for (int kb = kb0; kb < kb1; kb += kScaleBlocks) {
+          ok = wait_phase<false>(&scale_empty[ring.at], ring.phase ^ 1u, a.status);
+          if (!ok) break;
+          float v[kScaleBlocks][4];
+#pragma unroll
+          for (int i = 0; i < kScaleBlocks; ++i) {
+            const int k = min(kb + i, kb1 - 1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              v[i][j] = __ldg(a.x_scales + static_cast<int64_t>(k) * a.rows + min(row0 + 32 * j, a.rows - 1));
+          }
+          float* sx = scale_x + ring.at * kScaleBlocks * kGemmRows + lane;
+          if (lane < 2 * kScaleBlocks)
+            scale_w[ring.at * 2 * kScaleBlocks + lane] =
+                __ldg(sw + static_cast<int64_t>(lane & 1 ? blk1 : blk0) * KB + min(kb + (lane >> 1), kb1 - 1));
+#pragma unroll
+          for (int i = 0; i < kScaleBlocks; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sx[i * kGemmRows + 32 * j] = v[i][j];
+          mbar_arrive(&scale_full[ring.at]);
+          ring.next(kScaleSlots);
+        }
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -467,8 +544,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int W = BN / 2;  // columns of this warp group
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(half * W);
     const uint32_t acc_empty0 = CG == 2 ? mapa_shared(smem_u32(acc_empty), 0) : smem_u32(acc_empty);
-    const int NBLK = (a.N + kFp8Block - 1) / kFp8Block;
     const int local = quarter * 32 + lane;  // row of the tile's 128
+    uint8_t* out_s = smem + L.out_off + (warp - kEpiWarp0) * 2 * kStageOut;
+    int turn_out = 0;
 
     // rows of no expert are zeros
     if (a.out != kOutCodes) {
@@ -483,11 +561,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 
     int e = 0, turn = 0;
-    Ring ring;
+    Ring ring, scales;
     for (int t = worker; t < total && ok; t += workers, ++turn) {
       const Tile tile = find_tile(list, t, tile_rows, tiles_n, BN, e);
       const int64_t row = tile.m0 + (CG == 2 ? rank * kGemmRows : 0) + local;
       const bool live = row < tile.end;
+      const int row_w = tile.m0 + (CG == 2 ? rank * kGemmRows : 0) + quarter * 32;  // the warp's first row
+      const bool idle = row_w >= tile.end;  // a warp without rows only hands buffers back
       const int n0 = tile.n0 + half * W;
       float acc[W];
 #pragma unroll
@@ -503,54 +583,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
 
       if constexpr (FMT == kFmtE4M3) {
-        // four k blocks' scales are fetched while the four before are used
-        const float* sx = a.x_scales + min(row, static_cast<int64_t>(a.rows) - 1);
-        const float* sw = a.w_scales + (static_cast<int64_t>(tile.expert) * NBLK + min(n0 / kFp8Block, NBLK - 1)) * KB;
-        float next[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int kb = min(kb0 + i, kb1 - 1);
-          next[i] = __ldg(sx + static_cast<int64_t>(kb) * a.rows) * __ldg(sw + kb);
-        }
-        for (int kb = kb0; kb < kb1; kb += 4) {
-          float now[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) now[i] = next[i];
-          float fx[4], fw[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = min(kb + 4 + i, kb1 - 1);
-            fx[i] = __ldg(sx + static_cast<int64_t>(k) * a.rows);
-            fw[i] = __ldg(sw + k);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (kb + i < kb1) {
-              ok = ok && wait_phase<false>(&acc_full[ring.at], ring.phase, a.status);
-              tc_fence_after();
-              const uint32_t src = lane_base + static_cast<uint32_t>(ring.at * BN);
-              // the next columns are on their way while these are added
-              uint32_t r[2][32];
-              tmem_ld32(src, r[0]);
-#pragma unroll
-              for (int c = 0; c < W; c += 32) {
-                tmem_wait_ld(r[(c / 32) & 1]);
-                if (c + 32 < W) {
-                  tmem_ld32(src + c + 32, r[(c / 32 + 1) & 1]);
-                } else {
-                  // all read: the buffer goes back before the last sums
-                  tc_fence_before();
-                  if (lane == 0) mbar_arrive_remote(acc_empty0 + ring.at * 8);
-                }
-                const uint32_t(&v)[32] = r[(c / 32) & 1];
-#pragma unroll
-                for (int j = 0; j < 32; j += 2) fma2(acc[c + j], acc[c + j + 1], v[j], v[j + 1], now[i]);
-              }
+        for (int kb = kb0; kb < kb1; kb += kScaleBlocks) {
+          ok = ok && wait_phase<false>(&scale_full[scales.at], scales.phase, a.status);
+          const float* sx = scale_x + scales.at * kScaleBlocks * kGemmRows + local;
+          const float* sw = scale_w + scales.at * 2 * kScaleBlocks + half;
+          const int blocks = min(kScaleBlocks, kb1 - kb);
+#pragma unroll 1
+          for (int i = 0; i < blocks; ++i) {
+            ok = ok && wait_phase<false>(&acc_full[ring.at], ring.phase, a.status);
+            tc_fence_after();
+            const uint32_t src = lane_base + static_cast<uint32_t>(ring.at * BN);
+            if (idle) {
+              if (lane == 0) mbar_arrive_remote(acc_empty0 + ring.at * 8);
               ring.next(buffers);
+              continue;
             }
-          }
+            // the next columns are on their way while these are added
+            uint32_t r[2][32];
+            tmem_ld32(src, r[0]);
+            const float scale = sx[i * kGemmRows] * sw[2 * i];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) next[i] = fx[i] * fw[i];
+            for (int c = 0; c < W; c += 32) {
+              tmem_wait_ld(r[(c / 32) & 1]);
+              if (c + 32 < W) {
+                tmem_ld32(src + c + 32, r[(c / 32 + 1) & 1]);
+              } else {
+                // all read: the buffer goes back before the last sums
+                tc_fence_before();
+                if (lane == 0) mbar_arrive_remote(acc_empty0 + ring.at * 8);
+              }
+              const uint32_t(&v)[32] = r[(c / 32) & 1];
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) fma2(acc[c + j], acc[c + j + 1], v[j], v[j + 1], scale);
+            }
+            ring.next(buffers);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&scale_empty[scales.at]);
+          scales.next(kScaleSlots);
         }
       } else {
         ok = ok && wait_phase<false>(&acc_full[ring.at], ring.phase, a.status);
@@ -558,6 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t src = lane_base + static_cast<uint32_t>(ring.at * BN);
 #pragma unroll
         for (int c = 0; c < W; c += 32) {
+          if (idle) break;
           uint32_t r[32];
           tmem_ld32(src + c, r);
           tmem_wait_ld(r);
@@ -606,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane < S) mbar_arrive_cluster(mapa_shared(smem_u32(part_empty), lane));
         continue;
       }
-      if (!live) continue;
+      if (idle) continue;
 #pragma unroll
       for (int c = 0; c < W; c += 32) {
         if (a.bias != nullptr) {
@@ -619,11 +690,82 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (a.act != kActNone) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) acc[c + j] = activate(acc[c + j], a.act);
+          for (int j = 0; j < 32; j += 2) activate2(acc[c + j], acc[c + j + 1], a.act);
         }
-        if (n0 + c < a.N) store_values<DT, 32>(a, row, n0 + c, acc + c);
+      }
+      const bool whole = a.tile_store && row_w + 32 <= tile.end;
+      if constexpr (BN == 256 && FMT == kFmtE4M3) {
+        if (a.out == kOutCodes) {
+          // the thread's 128 columns are one block of its row
+          if (n0 >= a.N) continue;
+          if (n0 + W > a.N) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) acc[i] = n0 + i < a.N ? acc[i] : 0.0f;
+          }
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < W; ++i) top = max(top, __float_as_uint(acc[i]) & 0x7FFFFFFFu);
+          int ex = fp8_scale_exponent(top);
+          if (top >= 0x7F800000u) {
+            // not all finite: the scale comes from those that are, the others become NaN
+            top = 0;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+              const uint32_t m = finite_magnitude(acc[i]);
+              top = max(top, m);
+              if (m == 0 && acc[i] != 0.0f) acc[i] = __uint_as_float(0x7FC00000u);
+            }
+            ex = fp8_scale_exponent(top);
+          }
+          const float inv = pow2f(-ex);
+          if (live) a.y_scales[static_cast<int64_t>(n0 / kFp8Block) * a.rows + row] = pow2f(ex);
+          // rows of codes are padded to whole blocks
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float* v = acc + 64 * h + 4 * i;
+              w[i] = e4m3x2_finite(v[0] * inv, v[1] * inv) | (e4m3x2_finite(v[2] * inv, v[3] * inv) << 16);
+            }
+            if (whole) {
+              store_piece(out_s, turn_out, lane, w, &ymap, n0 + 64 * h, row_w);
+            } else if (live) {
+              uint8_t* p = reinterpret_cast<uint8_t*>(a.y) + row * a.ldy + n0 + 64 * h;
+              store32(p, w);
+              store32(p + 32, w + 8);
+            }
+          }
+          continue;
+        }
+      }
+      if (whole) {
+#pragma unroll
+        for (int c = 0; c < W; c += 32) {
+          if (n0 + c >= a.N) break;
+          uint32_t w[16];
+          if (a.out == kOutF32) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(acc[c + i]);
+            store_piece(out_s, turn_out, lane, w, &ymap, n0 + c, row_w);
+            if (n0 + c + 16 >= a.N) break;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(acc[c + 16 + i]);
+            store_piece(out_s, turn_out, lane, w, &ymap, n0 + c + 16, row_w);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = pack_t<DT>(acc[c + 2 * i], acc[c + 2 * i + 1]);
+            store_piece(out_s, turn_out, lane, w, &ymap, n0 + c, row_w);
+          }
+        }
+      } else if (live) {
+#pragma unroll
+        for (int c = 0; c < W; c += 32)
+          if (n0 + c < a.N) store_values<DT, 32>(a, row, n0 + c, acc + c);
       }
     }
+    // the tile stores have read their shared memory
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   }
 
   __syncwarp();
@@ -637,35 +779,35 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int FMT, int DT, int CG, int BN>
-cudaError_t launch_typed(const CUtensorMap& xmap, const CUtensorMap& wmap, const ExpertGemmArgs& a, int num_sms,
+cudaError_t launch_typed(const CUtensorMap& xmap, const CUtensorMap& wmap, const CUtensorMap& ymap, const ExpertGemmArgs& a, int num_sms,
                          cudaStream_t stream, bool pdl) {
   auto kernel = expert_gemm_kernel<FMT, DT, CG, BN>;
   static SharedMemoryOptIn opt_in;
   const cudaError_t configured = opt_in.ensure(reinterpret_cast<const void*>(kernel), kSmemLimit - 1024);
   if (configured != cudaSuccess) return configured;
-  const SmemPlan p = plan_smem(BN, CG, a.splits, a.experts);
+  const SmemPlan p = plan_smem(FMT == kFmtE4M3, BN, CG, a.splits, a.experts);
   const int cluster = CG * a.splits;
   // at most one tile list per cluster; no more clusters than tiles there can be
   const int64_t tile_rows = kGemmRows * CG;
   const int64_t groups = a.offsets == nullptr ? 1 : std::min(a.experts, a.rows);
   const int64_t tiles = ((a.rows + tile_rows - 1) / tile_rows + groups) * ((a.N + BN - 1) / BN);
   const int clusters = static_cast<int>(std::min<int64_t>(tiles, num_sms / cluster));
-  return launch_clustered(kernel, dim3(clusters * cluster), dim3(kThreads), p.bytes, stream, pdl, cluster, xmap, wmap, a);
+  return launch_clustered(kernel, dim3(clusters * cluster), dim3(kThreads), p.bytes, stream, pdl, cluster, xmap, wmap, ymap, a);
 }
 
 template <int FMT, int DT>
 cudaError_t launch_config(const ExpertGemmConfig& cfg, const CUtensorMap& xmap, const CUtensorMap& wmap,
-                          const ExpertGemmArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
-  if (cfg.pair == 2) return launch_typed<FMT, DT, 2, 256>(xmap, wmap, a, num_sms, stream, pdl);
-  if (cfg.bn == 256) return launch_typed<FMT, DT, 1, 256>(xmap, wmap, a, num_sms, stream, pdl);
-  if (cfg.bn == 128) return launch_typed<FMT, DT, 1, 128>(xmap, wmap, a, num_sms, stream, pdl);
-  return launch_typed<FMT, DT, 1, 64>(xmap, wmap, a, num_sms, stream, pdl);
+                          const CUtensorMap& ymap, const ExpertGemmArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
+  if (cfg.pair == 2) return launch_typed<FMT, DT, 2, 256>(xmap, wmap, ymap, a, num_sms, stream, pdl);
+  if (cfg.bn == 256) return launch_typed<FMT, DT, 1, 256>(xmap, wmap, ymap, a, num_sms, stream, pdl);
+  if (cfg.bn == 128) return launch_typed<FMT, DT, 1, 128>(xmap, wmap, ymap, a, num_sms, stream, pdl);
+  return launch_typed<FMT, DT, 1, 64>(xmap, wmap, ymap, a, num_sms, stream, pdl);
 }
 
 }  // namespace
 
 cudaError_t launch_expert_gemm(int dtype, bool e4m3, const CUtensorMap& xmap, const CUtensorMap& wmap,
-                               const ExpertGemmConfig& cfg, ExpertGemmArgs a, int num_sms, cudaStream_t stream,
+                               const CUtensorMap& ymap, const ExpertGemmConfig& cfg, ExpertGemmArgs a, int num_sms, cudaStream_t stream,
                                bool pdl) {
   a.splits = cfg.splits;
   const int KB = (a.K + (e4m3 ? 127 : 63)) / (e4m3 ? 128 : 64);
@@ -676,10 +818,10 @@ cudaError_t launch_expert_gemm(int dtype, bool e4m3, const CUtensorMap& xmap, co
   if ((cfg.splits - 1) * ((KB + cfg.splits - 1) / cfg.splits) >= KB) return cudaErrorInvalidValue;
   if (pair && cfg.bn != 256) return cudaErrorInvalidValue;
   if (e4m3)
-    return dtype == kF16 ? launch_config<kFmtE4M3, kF16>(cfg, xmap, wmap, a, num_sms, stream, pdl)
-                         : launch_config<kFmtE4M3, kBF16>(cfg, xmap, wmap, a, num_sms, stream, pdl);
-  return dtype == kF16 ? launch_config<kFmtF16, kF16>(cfg, xmap, wmap, a, num_sms, stream, pdl)
-                       : launch_config<kFmtBF16, kBF16>(cfg, xmap, wmap, a, num_sms, stream, pdl);
+    return dtype == kF16 ? launch_config<kFmtE4M3, kF16>(cfg, xmap, wmap, ymap, a, num_sms, stream, pdl)
+                         : launch_config<kFmtE4M3, kBF16>(cfg, xmap, wmap, ymap, a, num_sms, stream, pdl);
+  return dtype == kF16 ? launch_config<kFmtF16, kF16>(cfg, xmap, wmap, ymap, a, num_sms, stream, pdl)
+                       : launch_config<kFmtBF16, kBF16>(cfg, xmap, wmap, ymap, a, num_sms, stream, pdl);
 }
 
 ExpertGemmConfig plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, bool codes_out, int num_sms) {
@@ -695,7 +837,7 @@ ExpertGemmConfig plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K
   const int bn = tiles(128, 128) >= num_sms ? 128 : 64;
   int splits = 1;
   for (int s : {2, 4, 8})
-    if (tiles(128, bn) * s <= num_sms && (KB + s - 1) / s >= 2 && (s - 1) * ((KB + s - 1) / s) < KB) splits = s;
+    if (tiles(128, bn) * s <= num_sms && (KB + s - 1) / s >= 8 && (s - 1) * ((KB + s - 1) / s) < KB) splits = s;
   return {1, bn, splits};
 }
 

@@ -33,12 +33,18 @@ struct ExpertGemmArgs {
   float* y_scales;  // kOutCodes: [ceil(N / 128)][rows]
   int* status;
   int splits;
+  int tile_store;
 };
 
-// xmap: [rows, K] of x, box 128 bytes x 128 rows; wmap: [experts * N, K], box
+// The box of a tile store: 64 bytes of 32 rows.
+constexpr int kStoreRows = 32, kStoreBytes = 64;
+
+// ymap: [rows, N] of y in its own type, box 64 bytes x 32 rows, 64-byte
+// swizzle; used where a.tile_store says that y's rows allow it (16-byte
+// aligned).  xmap: [rows, K] of x, box 128 bytes x 128 rows; wmap: [experts * N, K], box
 // 128 bytes x bn / pair rows; both with the 128-byte swizzle.
 cudaError_t launch_expert_gemm(int dtype, bool e4m3, const CUtensorMap& xmap, const CUtensorMap& wmap,
-                               const ExpertGemmConfig& cfg, ExpertGemmArgs a, int num_sms, cudaStream_t stream,
+                               const CUtensorMap& ymap, const ExpertGemmConfig& cfg, ExpertGemmArgs a, int num_sms, cudaStream_t stream,
                                bool pdl);
 
 ExpertGemmConfig plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, bool codes_out, int num_sms);

@@ -86,39 +86,6 @@ __device__ __forceinline__ Group find_group(const ExpertGemvArgs& a, int slot, i
   return g;
 }
 
-template <int DT, int SRC>
-__device__ __forceinline__ void load_x8(const ExpertGemvArgs& a, int64_t src, int k, bool aligned, float (&v)[8]) {
-  constexpr int T = SRC == kSourceF32 ? static_cast<int>(kF32) : DT;
-  const char* row = reinterpret_cast<const char*>(a.x) + src * a.ldx * (SRC == kSourceF32 ? 4 : 2);
-  if (aligned && k + 8 <= a.K) {
-    if constexpr (T == kF32) {
-      const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + k);
-      const float4 lo = p[0], hi = p[1];
-      v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w;
-      v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + k);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (T == kBF16) {
-          v[2 * j] = __uint_as_float(w[j] << 16);
-          v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-          v[2 * j] = f.x, v[2 * j + 1] = f.y;
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = 0.0f;
-      if (k + j < a.K) v[j] = ld_t<T>(row, k + j);
-    }
-  }
-}
-
 // Rows [begin, begin + n) of x, blocks [kb0, kb1), into shared memory: codes
 // (or T), `pitch` bytes a row, and for codes their scales [block][kPassRows].
 template <bool F8, int DT, int SRC>
@@ -135,19 +102,13 @@ __device__ __forceinline__ void stage_x(const ExpertGemvArgs& a, int begin, int 
       const bool live = item < items;
       const int r = live ? item / blocks : 0, b = live ? item - r * blocks : 0;
       const int64_t src = !live ? -1 : a.row_index != nullptr ? a.row_index[begin + r] : begin + r;
-      float v[8] = {};
-      if (src >= 0 && src < a.x_rows) load_x8<DT, SRC>(a, src, (kb0 + b) * kFp8Block + lane * 8, aligned, v);
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, finite_magnitude(v[j]));
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      constexpr int T = SRC == kSourceF32 ? static_cast<int>(kF32) : DT;
+      Raw8<T> raw{};
+      if (src >= 0 && src < a.x_rows)
+        raw = load_row8<T>(reinterpret_cast<const char*>(a.x) + src * a.ldx * kSize, (kb0 + b) * kFp8Block + lane * 8, a.K, aligned);
+      int e;
+      const uint2 out = quantize8<T>(raw, e);
       if (!live) continue;
-      const int e = fp8_scale_exponent(top);
-      const float inv = pow2f(-e);
-      uint2 out;
-      out.x = e4m3x2(v[0] * inv, v[1] * inv) | (e4m3x2(v[2] * inv, v[3] * inv) << 16);
-      out.y = e4m3x2(v[4] * inv, v[5] * inv) | (e4m3x2(v[6] * inv, v[7] * inv) << 16);
       *reinterpret_cast<uint2*>(xs + r * pitch + b * 128 + lane * 8) = out;
       if (lane == 0) sx[b * kPassRows + r] = pow2f(e);
     }

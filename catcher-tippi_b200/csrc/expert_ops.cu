@@ -12,91 +12,49 @@ namespace {
 
 // ------------------------------------------------------------------ rows to e4m3
 
-// One block of 128 values per half warp, eight values a lane: the largest
-// magnitude by shuffles, then the codes, eight bytes a lane.  Bound by memory:
-// (2 + 1) bytes a value for 16-bit rows.
-constexpr int kQuantThreads = 256, kQuantHalves = kQuantThreads / 16;
-constexpr int kQuantItems = 4;  // blocks a half warp has in flight
-
-template <int DT>
-__device__ __forceinline__ void load8(const void* row, int k, int cols, bool aligned, float (&v)[8]) {
-  if (aligned && k + 8 <= cols) {
-    if constexpr (DT == kF32) {
-      const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + k);
-      const float4 a = p[0], b = p[1];
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-      v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + k);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (DT == kBF16) {
-          v[2 * j] = __uint_as_float(w[j] << 16);
-          v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-          v[2 * j] = f.x, v[2 * j + 1] = f.y;
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = 0.0f;
-      if (k + j < cols) v[j] = ld_t<DT>(row, k + j);
-    }
-  }
-}
+// A CTA takes 16 rows times four blocks of 128 values, a half warp one row:
+// its four blocks are loaded (a kilobyte next to each other for 16-bit rows)
+// before the first is looked at, eight values a lane; the largest magnitude by
+// shuffles, then the codes, eight bytes a lane.  The scales leave as runs of 16
+// rows: written one by one they were scattered over as many sectors and cost as
+// much as the codes.  Bound by memory: (2 + 1) bytes a value for 16-bit rows.
+constexpr int kQuantThreads = 256, kQuantRows = kQuantThreads / 16;
+constexpr int kQuantBlocks = 4;
 
 template <int DT>
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const QuantizeRowsArgs a) {
+  __shared__ float scale_s[kQuantBlocks][kQuantRows];
   pdl_launch_dependents();
   pdl_wait();
   constexpr int kSize = DT == kF32 ? 4 : 2;
-  const uint32_t blocks = (a.cols + kFp8Block - 1) / kFp8Block;
-  const uint32_t items = static_cast<uint32_t>(a.rows) * blocks;  // below 2^32: x fits the device's memory
+  const int blocks = (a.cols + kFp8Block - 1) / kFp8Block;
   const bool aligned = ((a.ldx * kSize) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
-  const uint32_t half = threadIdx.x >> 4, lane = threadIdx.x & 15;
-  const uint32_t first = blockIdx.x * (kQuantHalves * kQuantItems) + half;
-  // all loads before the first use
-  float v[kQuantItems][8];
-  uint32_t row[kQuantItems], block[kQuantItems];
-  bool live[kQuantItems];
+  const int half = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  const int groups = (blocks + kQuantBlocks - 1) / kQuantBlocks;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x / groups) * kQuantRows, row = row0 + half;
+  const int b0 = static_cast<int>(blockIdx.x % groups) * kQuantBlocks;
+  int64_t src = row < a.rows ? row : -1;
+  if (src >= 0 && a.row_index != nullptr) src = a.row_index[row];
+  const bool live = src >= 0 && src < a.x_rows;
+  const char* from = reinterpret_cast<const char*>(a.x) + src * a.ldx * kSize;
+  Raw8<DT> raw[kQuantBlocks];
 #pragma unroll
-  for (int u = 0; u < kQuantItems; ++u) {
-    const uint32_t item = first + u * kQuantHalves;
-    live[u] = item < items;
-    row[u] = live[u] ? item / blocks : 0;
-    block[u] = item - row[u] * blocks;
-    int64_t src = row[u];
-    if (live[u] && a.row_index != nullptr) {
-      src = a.row_index[row[u]];
-      live[u] = src >= 0 && src < a.x_rows;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
-    if (live[u])
-      load8<DT>(reinterpret_cast<const char*>(a.x) + src * a.ldx * kSize, block[u] * kFp8Block + lane * 8, a.cols,
-                aligned, v[u]);
+  for (int u = 0; u < kQuantBlocks; ++u) {
+    raw[u] = Raw8<DT>{};
+    if (live && b0 + u < blocks) raw[u] = load_row8<DT>(from, (b0 + u) * kFp8Block + lane * 8, a.cols, aligned);
   }
 #pragma unroll
-  for (int u = 0; u < kQuantItems; ++u) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, finite_magnitude(v[u][j]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    if (!live[u]) continue;
-    const int e = fp8_scale_exponent(top);
-    const float inv = pow2f(-e);
-    uint2 out;
-    out.x = e4m3x2(v[u][0] * inv, v[u][1] * inv) | (e4m3x2(v[u][2] * inv, v[u][3] * inv) << 16);
-    out.y = e4m3x2(v[u][4] * inv, v[u][5] * inv) | (e4m3x2(v[u][6] * inv, v[u][7] * inv) << 16);
-    const uint32_t k = block[u] * kFp8Block + lane * 8;
-    if (k < a.ld) *reinterpret_cast<uint2*>(a.codes + row[u] * a.ld + k) = out;
-    if (lane == 0) a.scales[static_cast<int64_t>(block[u]) * a.rows + row[u]] = pow2f(e);
+  for (int u = 0; u < kQuantBlocks; ++u) {
+    int e;
+    const uint2 out = quantize8<DT>(raw[u], e);
+    const int k = (b0 + u) * kFp8Block + lane * 8;
+    if (live && b0 + u < blocks && k < a.ld) *reinterpret_cast<uint2*>(a.codes + row * a.ld + k) = out;
+    if (lane == 0) scale_s[u][half] = pow2f(e);
   }
+  __syncthreads();
+  const int u = threadIdx.x / kQuantRows, r = threadIdx.x % kQuantRows;
+  if (u < kQuantBlocks && b0 + u < blocks && row0 + r < a.rows)
+    a.scales[static_cast<int64_t>(b0 + u) * a.rows + row0 + r] = scale_s[u][r];
 }
 
 // One CTA per 128 x 128 block of a weight; used when a layer is made.
@@ -408,30 +366,11 @@ cudaError_t route_dtype(const RouteArgs& a, cudaStream_t stream, bool pdl) {
 // once, y once.  Four experts' rows are on their way before the first is
 // added.  `VEC`: every row is 16-byte aligned and dims a multiple of 8.
 template <int T>
-struct Raw8 {
-  uint4 u[T == kF32 ? 2 : 1];
-};
-template <int T>
 __device__ __forceinline__ void add_raw8(const Raw8<T>& r, float w, float (&acc)[8]) {
-  if constexpr (T == kF32) {
-    const uint32_t b[8] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w, r.u[1].x, r.u[1].y, r.u[1].z, r.u[1].w};
+  float v[8];
+  widen8<T>(r, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, __uint_as_float(b[j]), acc[j]);
-  } else {
-    const uint32_t b[4] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float lo, hi;
-      if constexpr (T == kBF16) {
-        lo = __uint_as_float(b[j] << 16), hi = __uint_as_float(b[j] & 0xFFFF0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[j]));
-        lo = f.x, hi = f.y;
-      }
-      acc[2 * j] = fmaf(w, lo, acc[2 * j]);
-      acc[2 * j + 1] = fmaf(w, hi, acc[2 * j + 1]);
-    }
-  }
+  for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, v[j], acc[j]);
 }
 
 template <int DT, int ZT, bool VEC>
@@ -499,14 +438,14 @@ cudaError_t combine_typed(const CombineArgs& a, cudaStream_t stream, bool pdl) {
 }  // namespace
 
 cudaError_t launch_quantize_rows(int dtype, const QuantizeRowsArgs& a, cudaStream_t stream, bool pdl) {
-  const int64_t items = static_cast<int64_t>(a.rows) * ((a.cols + kFp8Block - 1) / kFp8Block);
-  if (items == 0) return cudaSuccess;
-  constexpr int kPer = kQuantHalves * kQuantItems;
-  const int grid = static_cast<int>((items + kPer - 1) / kPer);
+  if (a.rows == 0) return cudaSuccess;
+  const int blocks = (a.cols + kFp8Block - 1) / kFp8Block;
+  const int64_t grid = static_cast<int64_t>((a.rows + kQuantRows - 1) / kQuantRows) * ((blocks + kQuantBlocks - 1) / kQuantBlocks);
+  if (grid > INT32_MAX) return cudaErrorInvalidValue;  // rows of 256 GB
   switch (dtype) {
-    case kF16: return launch(quantize_rows_kernel<kF16>, dim3(grid), dim3(kQuantThreads), 0, stream, pdl, a);
-    case kBF16: return launch(quantize_rows_kernel<kBF16>, dim3(grid), dim3(kQuantThreads), 0, stream, pdl, a);
-    case kF32: return launch(quantize_rows_kernel<kF32>, dim3(grid), dim3(kQuantThreads), 0, stream, pdl, a);
+    case kF16: return launch(quantize_rows_kernel<kF16>, dim3(static_cast<unsigned>(grid)), dim3(kQuantThreads), 0, stream, pdl, a);
+    case kBF16: return launch(quantize_rows_kernel<kBF16>, dim3(static_cast<unsigned>(grid)), dim3(kQuantThreads), 0, stream, pdl, a);
+    case kF32: return launch(quantize_rows_kernel<kF32>, dim3(static_cast<unsigned>(grid)), dim3(kQuantThreads), 0, stream, pdl, a);
     default: return cudaErrorInvalidValue;
   }
 }

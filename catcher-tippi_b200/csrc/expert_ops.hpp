@@ -12,8 +12,8 @@ constexpr int kMaxTop = 32;
 
 // x rows -> e4m3 codes [rows][ld] (ld a multiple of 16; zero from cols to the
 // next multiple of 128 or ld) and scales [ceil(cols / 128)][rows].  With
-// row_index, row r is x row row_index[r]; rows whose index is outside
-// [0, x_rows) are left as they are.
+// row_index, row r is x row row_index[r]; where that is outside [0, x_rows) the
+// codes are left as they are and the scales are 1.
 struct QuantizeRowsArgs {
   const void* x;
   int64_t ldx;

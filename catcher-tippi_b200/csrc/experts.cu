@@ -164,14 +164,14 @@ void ExpertLinear::check_rows(const void* x, int64_t ldx, int rows, const void* 
   check_act(act);
 }
 
-void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, int out, void* y, int64_t ldy, int act,
-                           void* staging, cudaStream_t stream) const {
+void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, const Out& out, int act, void* staging,
+                           cudaStream_t stream) const {
   DeviceContext& ctx = device_context(device_);
   const bool pdl = pdl_enabled();
-  if (out != cq::kOutCodes && few_rows(rows, offsets != nullptr)) {
+  if (out.kind != cq::kOutCodes && few_rows(rows, offsets != nullptr)) {
     const cq::ExpertGemvArgs a{x.x,           x.ld,  x.row_index,        x.x_rows,     x.scales, rows,
                                weight_.get(), ldw_,  scales_.as<float>(), bias_.get(), offsets,  experts_,
-                               N_,            K_,    act,                out == cq::kOutF32, y,  ldy};
+                               N_,            K_,    act,                out.kind == cq::kOutF32, out.y,  out.ld};
     check_cuda(cq::launch_expert_gemv(dtype_, e4m3(), x.source, a, ctx.num_sms, stream, pdl), "expert product");
     return;
   }
@@ -203,17 +203,24 @@ void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, int 
   a.N = N_;
   a.K = K_;
   a.act = act;
-  a.out = out;
-  a.y = y;
-  a.ldy = ldy;
+  a.out = out.kind;
+  a.y = out.y;
+  a.ldy = out.ld;
+  a.y_scales = out.scales;
   a.status = ctx.status;
-  const cq::ExpertGemmConfig cfg =
-      cq::plan_expert_gemm(e4m3(), rows, experts_, N_, K_, out == cq::kOutCodes, ctx.num_sms);
+  const bool codes = out.kind == cq::kOutCodes;
+  const cq::ExpertGemmConfig cfg = cq::plan_expert_gemm(e4m3(), rows, experts_, N_, K_, codes, ctx.num_sms);
   const int size = e4m3() ? 1 : 2, k = 128 / size;
   const CUtensorMap xmap = make_map_2d(from, size, rows, K_, ld, cq::kGemmRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
   const CUtensorMap wmap =
       make_map_2d(weight_.get(), size, experts_ * N_, K_, ldw_, cfg.bn / cfg.pair, k, CU_TENSOR_MAP_SWIZZLE_128B);
-  check_cuda(cq::launch_expert_gemm(dtype_, e4m3(), xmap, wmap, cfg, a, ctx.num_sms, stream, pdl), "expert product");
+  CUtensorMap ymap = xmap;
+  const int ysize = codes ? 1 : out.kind == cq::kOutF32 ? 4 : 2;
+  a.tile_store = out.ld * ysize % 16 == 0 && (reinterpret_cast<uintptr_t>(out.y) & 15) == 0;
+  if (a.tile_store)
+    ymap = make_map_2d(out.y, ysize, rows, codes ? static_cast<int>(out.ld) : N_, out.ld, cq::kStoreRows,
+                       cq::kStoreBytes / ysize, CU_TENSOR_MAP_SWIZZLE_64B);
+  check_cuda(cq::launch_expert_gemm(dtype_, e4m3(), xmap, wmap, ymap, cfg, a, ctx.num_sms, stream, pdl), "expert product");
 }
 
 void ExpertLinear::forward(const void* x, int64_t ldx, int rows, const int32_t* offsets, void* y, int64_t ldy, int act,
@@ -223,7 +230,8 @@ void ExpertLinear::forward(const void* x, int64_t ldx, int rows, const int32_t* 
   if (rows == 0) return;
   check_workspace(workspace, workspace_bytes, this->workspace(rows));
   DeviceGuard guard(device_);
-  product({cq::kSourceT, x, ldx, nullptr, nullptr, rows}, rows, offsets, cq::kOutT, y, ldy, act, workspace, stream);
+  product({cq::kSourceT, x, ldx, nullptr, nullptr, rows}, rows, offsets, {cq::kOutT, y, ldy, nullptr}, act,
+          workspace, stream);
 }
 
 void ExpertLinear::forward_codes(const uint8_t* codes, int64_t ld, const float* scales, int rows, void* y, int64_t ldy,
@@ -235,7 +243,8 @@ void ExpertLinear::forward_codes(const uint8_t* codes, int64_t ld, const float* 
   if (scales == nullptr) throw_invalid("scales must not be null");
   check_aligned(scales, 4, "scales");
   DeviceGuard guard(device_);
-  product({cq::kSourceCodes, codes, ld, scales, nullptr, rows}, rows, nullptr, cq::kOutT, y, ldy, act, nullptr, stream);
+  product({cq::kSourceCodes, codes, ld, scales, nullptr, rows}, rows, nullptr, {cq::kOutT, y, ldy, nullptr}, act,
+          nullptr, stream);
 }
 
 void quantize_rows(const void* x, int64_t ldx, const int32_t* row_index, int x_rows, int rows, int cols,
@@ -336,7 +345,7 @@ struct FfnScratch {
   void* route;
   size_t route_bytes;
   void *x, *h_staged;  // the products' staging
-  void* h;             // up's result: T, or f32 on its way to e4m3
+  void* h;             // up's result: T; f32 on its way to e4m3; or codes and scales
   int64_t ld_h;
   float* z;  // f32: the sum over a token's experts is rounded once
 };
@@ -352,9 +361,11 @@ FfnScratch take_ffn(Arena& arena, const ExpertLinear& up, const ExpertLinear& do
   s.route_bytes = route_workspace_bytes(tokens, up.experts(), top);
   s.route = arena.take<uint8_t>(s.route_bytes);
   s.x = arena.take<uint8_t>(up.staging_bytes(pairs));
-  s.h_staged = up.e4m3() ? arena.take<uint8_t>(down.staging_bytes(pairs)) : nullptr;
   s.ld_h = round_up(up.output_dims(), 8);
-  s.h = arena.take<uint8_t>(pairs * s.ld_h * (up.e4m3() ? 4 : 2));
+  const bool few = up.few_rows(static_cast<int>(pairs), true);
+  s.h_staged = up.e4m3() && few ? arena.take<uint8_t>(down.staging_bytes(pairs)) : nullptr;
+  s.h = up.e4m3() && !few ? arena.take<uint8_t>(down.staging_bytes(pairs))
+                          : arena.take<uint8_t>(pairs * s.ld_h * (up.e4m3() ? 4 : 2));
   s.z = arena.take<float>(pairs * down.output_dims());
   return s;
 }
@@ -398,10 +409,21 @@ void expert_ffn(const ExpertLinear& up, const ExpertLinear& down, const void* x,
   DeviceGuard guard(up.device());
   route(logits, ld_logits, logits_dtype, tokens, up.experts(), top, renormalize, s.expert, s.weight, s.offsets,
         s.token, s.position, s.route, s.route_bytes, stream);
-  up.product({cq::kSourceT, x, ldx, nullptr, s.token, tokens}, pairs, s.offsets,
-             up.e4m3() ? cq::kOutF32 : cq::kOutT, s.h, s.ld_h, act, s.x, stream);
-  down.product({up.e4m3() ? cq::kSourceF32 : cq::kSourceT, s.h, s.ld_h, nullptr, nullptr, pairs}, pairs, s.offsets,
-               cq::kOutF32, s.z, out, CQ_ACT_NONE, s.h_staged, stream);
+  const ExpertLinear::Rows rows{cq::kSourceT, x, ldx, nullptr, s.token, tokens};
+  ExpertLinear::Rows h{cq::kSourceT, s.h, s.ld_h, nullptr, nullptr, pairs};
+  if (!up.e4m3()) {
+    up.product(rows, pairs, s.offsets, {cq::kOutT, s.h, s.ld_h, nullptr}, act, s.x, stream);
+  } else if (up.few_rows(pairs, true)) {
+    up.product(rows, pairs, s.offsets, {cq::kOutF32, s.h, s.ld_h, nullptr}, act, s.x, stream);
+    h.source = cq::kSourceF32;
+  } else {
+    // from f32 sums to codes inside the first product
+    const int64_t ld = round_up(up.output_dims(), kBlock);
+    float* scales = reinterpret_cast<float*>(static_cast<char*>(s.h) + round_up(pairs * ld, 256));
+    up.product(rows, pairs, s.offsets, {cq::kOutCodes, s.h, ld, scales}, act, s.x, stream);
+    h = {cq::kSourceCodes, s.h, ld, scales, nullptr, pairs};
+  }
+  down.product(h, pairs, s.offsets, {cq::kOutF32, s.z, out, nullptr}, CQ_ACT_NONE, s.h_staged, stream);
   const cq::CombineArgs c{s.z, out, s.position, s.weight, pairs, tokens, top, out, y, ldy, 1};
   check_cuda(cq::launch_combine(up.dtype(), c, stream, pdl_enabled()), "combine");
 }

@@ -51,9 +51,17 @@ class ExpertLinear {
   // Bytes in which product() brings rows to the form that the tensor cores'
   // tile copies take.
   size_t staging_bytes(int64_t rows) const;
-  // The product alone, arguments checked; out: a cq::ExpertOut.
-  void product(const Rows& x, int rows, const int32_t* offsets, int out, void* y, int64_t ldy, int act,
-               void* staging, cudaStream_t stream) const;
+  // What a product makes: a cq::ExpertOut; codes need y_scales [n blocks][rows]
+  // and rows padded to whole blocks, and rows that few_rows() does not take.
+  struct Out {
+    int kind;
+    void* y;
+    int64_t ld;
+    float* scales;
+  };
+  // The product alone, arguments checked.
+  void product(const Rows& x, int rows, const int32_t* offsets, const Out& out, int act, void* staging,
+               cudaStream_t stream) const;
   // True when calls on `rows` rows stream the weights (expert_gemv.cu) instead
   // of running tiles on the tensor cores (expert_gemm.cu).
   bool few_rows(int rows, bool grouped) const;

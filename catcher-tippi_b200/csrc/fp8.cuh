@@ -43,6 +43,116 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return r;
 }
 
+// The same for finite values.
+__device__ __forceinline__ uint32_t e4m3x2_finite(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Eight values as they are in memory, 16 bytes (f32: 32).
+template <int T>
+struct Raw8 {
+  uint4 u[T == kF32 ? 2 : 1];
+};
+
+template <int T>
+__device__ __forceinline__ Raw8<T> load_raw8(const void* p) {
+  Raw8<T> r;
+  r.u[0] = reinterpret_cast<const uint4*>(p)[0];
+  if constexpr (T == kF32) r.u[1] = reinterpret_cast<const uint4*>(p)[1];
+  return r;
+}
+
+template <int T>
+__device__ __forceinline__ void widen8(const Raw8<T>& r, float (&v)[8]) {
+  if constexpr (T == kF32) {
+    const uint32_t b[8] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w, r.u[1].x, r.u[1].y, r.u[1].z, r.u[1].w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(b[j]);
+  } else {
+    const uint32_t b[4] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (T == kBF16) {
+        v[2 * j] = __uint_as_float(b[j] << 16);
+        v[2 * j + 1] = __uint_as_float(b[j] & 0xFFFF0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[j]));
+        v[2 * j] = f.x, v[2 * j + 1] = f.y;
+      }
+    }
+  }
+}
+
+// The largest magnitude of eight values, infinities and NaN among them, as the
+// bits of an f32.  16-bit magnitudes are compared two at a time as integers.
+template <int T>
+__device__ __forceinline__ uint32_t magnitude8(const Raw8<T>& r) {
+  if constexpr (T == kF32) {
+    const uint32_t b[8] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w, r.u[1].x, r.u[1].y, r.u[1].z, r.u[1].w};
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, b[j] & 0x7FFFFFFFu);
+    return m;
+  } else {
+    const uint32_t m = __vmaxu2(__vmaxu2(r.u[0].x & 0x7FFF7FFFu, r.u[0].y & 0x7FFF7FFFu),
+                                __vmaxu2(r.u[0].z & 0x7FFF7FFFu, r.u[0].w & 0x7FFF7FFFu));
+    const uint32_t top = max(m & 0xFFFFu, m >> 16);
+    if constexpr (T == kBF16) return top << 16;
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top))));
+  }
+}
+
+// Eight values of one lane of 16 that hold a block of 128: the block's scale
+// exponent and the lane's eight codes.  All lanes of the warp.
+template <int T>
+__device__ __forceinline__ uint2 quantize8(const Raw8<T>& r, int& exponent) {
+  uint32_t top = magnitude8<T>(r);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  float v[8];
+  widen8<T>(r, v);
+  uint2 out;
+  if (__any_sync(0xFFFFFFFFu, top >= 0x7F800000u)) {
+    // some value of the warp is not finite: the scale comes from those that are
+    top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, finite_magnitude(v[j]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    exponent = fp8_scale_exponent(top);
+    const float inv = pow2f(-exponent);
+    out.x = e4m3x2(v[0] * inv, v[1] * inv) | (e4m3x2(v[2] * inv, v[3] * inv) << 16);
+    out.y = e4m3x2(v[4] * inv, v[5] * inv) | (e4m3x2(v[6] * inv, v[7] * inv) << 16);
+  } else {
+    exponent = fp8_scale_exponent(top);
+    const float inv = pow2f(-exponent);
+    out.x = e4m3x2_finite(v[0] * inv, v[1] * inv) | (e4m3x2_finite(v[2] * inv, v[3] * inv) << 16);
+    out.y = e4m3x2_finite(v[4] * inv, v[5] * inv) | (e4m3x2_finite(v[6] * inv, v[7] * inv) << 16);
+  }
+  return out;
+}
+
+// Eight values of a row from element k on, zeros from `cols` on; aligned: the
+// row can be read 16 bytes at a time.
+template <int T>
+__device__ __forceinline__ Raw8<T> load_row8(const void* row, int k, int cols, bool aligned) {
+  constexpr int kSize = T == kF32 ? 4 : 2;
+  if (aligned && k + 8 <= cols) return load_raw8<T>(reinterpret_cast<const char*>(row) + static_cast<int64_t>(k) * kSize);
+  uint32_t b[8] = {};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (k + j >= cols) continue;
+    if constexpr (T == kF32) b[j] = reinterpret_cast<const uint32_t*>(row)[k + j];
+    else b[j / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[k + j]) << (16 * (j & 1));
+  }
+  Raw8<T> r;
+  r.u[0] = make_uint4(b[0], b[1], b[2], b[3]);
+  if constexpr (T == kF32) r.u[1] = make_uint4(b[4], b[5], b[6], b[7]);
+  return r;
+}
+
 __device__ __forceinline__ float e4m3_to_float(uint8_t code) {
   __nv_fp8_e4m3 v;
   v.__x = code;
@@ -55,6 +165,21 @@ __device__ __forceinline__ float activate(float v, int act) {
   if (act == kActSilu) return __fdividef(v, 1.0f + __expf(-v));
   if (act == kActRelu) return v < 0.0f ? 0.0f : v;
   return v;
+}
+
+// activate for two values: one reciprocal serves both SiLUs, 1 / a = b / (a b)
+// (an epilogue of SiLUs is bound by the special-function unit).  -v is cut at
+// 60, so that a b stays finite: below -60 SiLU is under 6e-25 either way.
+__device__ __forceinline__ void activate2(float& x, float& y, int act) {
+  if (act == kActSilu) {
+    const float a = 1.0f + __expf(fminf(-x, 60.0f)), b = 1.0f + __expf(fminf(-y, 60.0f));
+    const float r = __fdividef(1.0f, a * b);
+    x *= r * b;
+    y *= r * a;
+  } else if (act == kActRelu) {
+    x = x < 0.0f ? 0.0f : x;
+    y = y < 0.0f ? 0.0f : y;
+  }
 }
 
 // Two f32 values rounded to T, lo in the low half.

@@ -141,7 +141,9 @@ CUtensorMap make_map_2d(const void* base, int elem_bytes, int rows, int cols, in
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * elem_bytes};  // bytes per row
   const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
   const CUtensorMapDataType dt =
-      elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+      elem_bytes == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+      : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                        : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   return encode_map(dt, 2, base, dims, strides, box, swizzle);
 }
 

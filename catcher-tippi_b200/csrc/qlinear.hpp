@@ -54,8 +54,8 @@ class DeviceGuard {
   int prev_ = -1;
 };
 
-// 2-D tiled tensor map over a row-major [rows, cols] matrix of 1- or 2-byte
-// elements (row stride in elements), box [box_rows, box_cols].
+// 2-D tiled tensor map over a row-major [rows, cols] matrix of 1-, 2- or
+// 4-byte elements (row stride in elements), box [box_rows, box_cols].
 CUtensorMap make_map_2d(const void* base, int elem_bytes, int rows, int cols, int64_t ld,
                         int box_rows, int box_cols, CUtensorMapSwizzle swizzle);
 
