@@ -296,45 +296,17 @@ __device__ __forceinline__ Tile find_tile(const TileList& l, int t, int tile_row
   return Tile{e, l.start[e] + i / tiles_n * tile_rows, l.start[e + 1], i % tiles_n * bn};
 }
 
+constexpr int kBoxBytes = kGemmBoxRows * kRowBytes;
+__device__ __forceinline__ int row_boxes(int rows) {
+  return min(max(rows + kGemmBoxRows - 1, 0) / kGemmBoxRows, kGemmRows / kGemmBoxRows);
+}
+
 // --------------------------------------------------------------- epilogue
 
 // 32-byte store of eight words.
 __device__ __forceinline__ void store32(void* p, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
-}
-
-// `count` (a multiple of 16 at most 32) finished values of one row from column n on.
-template <int DT, int COUNT>
-__device__ __forceinline__ void store_values(const ExpertGemmArgs& a, int64_t row, int n, const float* v) {
-  if (a.out == kOutF32) {
-    float* p = reinterpret_cast<float*>(a.y) + row * a.ldy + n;
-    if ((reinterpret_cast<uintptr_t>(p) & 31) == 0 && n + COUNT <= a.N) {
-#pragma unroll
-      for (int i = 0; i < COUNT; i += 8) store32(p + i, reinterpret_cast<const uint32_t*>(v + i));
-    } else {
-#pragma unroll
-      for (int i = 0; i < COUNT; ++i)
-        if (n + i < a.N) p[i] = v[i];
-    }
-    return;
-  }
-  uint16_t* p = reinterpret_cast<uint16_t*>(a.y) + row * a.ldy + n;
-  uint32_t w[COUNT / 2];
-#pragma unroll
-  for (int i = 0; i < COUNT / 2; ++i) w[i] = pack_t<DT>(v[2 * i], v[2 * i + 1]);
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-  if ((at & 31) == 0 && n + COUNT <= a.N) {
-#pragma unroll
-    for (int i = 0; i < COUNT / 2; i += 8) store32(p + 2 * i, w + i);
-  } else if ((at & 15) == 0 && n + COUNT <= a.N) {
-#pragma unroll
-    for (int i = 0; i < COUNT / 2; i += 4) *reinterpret_cast<uint4*>(p + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i)
-      if (n + i < a.N) p[i] = static_cast<uint16_t>(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu);
-  }
 }
 
 // 64 bytes of each of a warp's 32 rows: through the warp's shared memory
@@ -361,6 +333,40 @@ __device__ __forceinline__ void store_piece(uint8_t* out_s, int& turn, int lane,
   }
 }
 
+// The same for rows that a tile store cannot take: the last rows of a group,
+// or rows of y that are not 16-byte aligned.  From shared memory the warp
+// writes row by row, so that its lanes' addresses are next to each other.
+// `size`: bytes of a value; `values`: how many of the piece are inside N.
+__device__ __forceinline__ void store_piece_by_rows(uint8_t* buf, int lane, const uint32_t* w, uint8_t* y, int64_t pitch,
+                                                    int size, int rows, int values, bool aligned) {
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  __syncwarp();
+#pragma unroll
+  for (int p = 0; p < 4; ++p)
+    *reinterpret_cast<uint4*>(buf + lane * kStoreBytes + ((p ^ ((lane >> 1) & 3)) << 4)) =
+        make_uint4(w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
+  __syncwarp();
+  if (aligned && values * size == kStoreBytes) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2), p = lane & 3;
+      if (r < rows)
+        *reinterpret_cast<uint4*>(y + r * pitch + p * 16) =
+            *reinterpret_cast<const uint4*>(buf + r * kStoreBytes + ((p ^ ((r >> 1) & 3)) << 4));
+    }
+  } else {
+    const int per_row = kStoreBytes / size, step = 32 / per_row;  // 32 T or 16 f32 values a row
+    const int c = lane % per_row, byte = c * size;
+    for (int r = lane / per_row; r < rows; r += step) {
+      const uint8_t* from = buf + r * kStoreBytes + ((((byte >> 4) ^ (r >> 1)) & 3) << 4) + (byte & 15);
+      if (c < values) {
+        if (size == 4) *reinterpret_cast<uint32_t*>(y + r * pitch + byte) = *reinterpret_cast<const uint32_t*>(from);
+        else *reinterpret_cast<uint16_t*>(y + r * pitch + byte) = *reinterpret_cast<const uint16_t*>(from);
+      }
+    }
+  }
+}
+
 // The four warps of an epilogue group.
 __device__ __forceinline__ void group_sync(int half) {
   if (half == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -371,7 +377,8 @@ __device__ __forceinline__ void group_sync(int half) {
 
 template <int FMT, int DT, int CG, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
-    expert_gemm_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
+    expert_gemm_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap xmap_part,
+                       const __grid_constant__ CUtensorMap wmap,
                        const __grid_constant__ CUtensorMap ymap, const ExpertGemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -407,6 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&xmap);
+    prefetch_tensormap(&xmap_part);
     prefetch_tensormap(&wmap);
     prefetch_tensormap(&ymap);
     for (int s = 0; s < kMaxStages; ++s) {
@@ -443,12 +451,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
       // ---------------------------------------------------------- copies
       const uint64_t keep = l2_policy_evict_normal();
-      const uint32_t bytes = static_cast<uint32_t>(L.stage_bytes) * CG;
       int e = 0, issued = 0;
       Ring ring;
       for (int t = worker; t < total && ok; t += workers) {
         const Tile tile = find_tile(list, t, tile_rows, tiles_n, BN, e);
+        // only the rows that there are, by 32: a small group's tile is mostly weights
         const int m = tile.m0 + (CG == 2 ? rank * kGemmRows : 0);
+        const int boxes = row_boxes(tile.end - m);
+        const int all_boxes = CG == 2 ? row_boxes(tile.end - tile.m0) + row_boxes(tile.end - tile.m0 - kGemmRows) : boxes;
+        const uint32_t bytes = static_cast<uint32_t>(all_boxes * kBoxBytes + BN * kRowBytes);
         const int w = tile.expert * a.N + tile.n0 + (CG == 2 ? rank * (BN / 2) : 0);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!wait_phase<false>(&empty[ring.at], ring.phase ^ 1u, a.status)) {
@@ -460,7 +471,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (CG == 2) bar = mapa_shared(bar, 0);
           if (elect_one()) {
             if (rank == 0 || CG == 1) mbar_arrive_expect_tx(&full[ring.at], bytes);
-            load_tile<CG>(st, &xmap, kb * kElems, m, bar, keep);
+            if (boxes == kGemmRows / kGemmBoxRows) {
+              load_tile<CG>(st, &xmap, kb * kElems, m, bar, keep);
+            } else {
+              for (int b = 0; b < boxes; ++b)
+                load_tile<CG>(st + b * kBoxBytes, &xmap_part, kb * kElems, m + b * kGemmBoxRows, bar, keep);
+            }
             load_tile<CG>(st + kXBytes, &wmap, kb * kElems, w, bar, keep);
           }
           __syncwarp();
@@ -739,29 +755,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           continue;
         }
       }
-      if (whole) {
+      const int rows_w = min(32, tile.end - row_w);
+      const int size = a.out == kOutF32 ? 4 : 2;
 #pragma unroll
-        for (int c = 0; c < W; c += 32) {
-          if (n0 + c >= a.N) break;
-          uint32_t w[16];
-          if (a.out == kOutF32) {
+      for (int c = 0; c < W; c += 16) {
+        // 64 bytes: 16 f32 values, or 32 of T
+        if (n0 + c >= a.N) break;
+        uint32_t w[16];
+        if (a.out == kOutF32) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(acc[c + i]);
-            store_piece(out_s, turn_out, lane, w, &ymap, n0 + c, row_w);
-            if (n0 + c + 16 >= a.N) break;
+          for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(acc[c + i]);
+        } else {
+          if (c % 32 != 0) continue;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(acc[c + 16 + i]);
-            store_piece(out_s, turn_out, lane, w, &ymap, n0 + c + 16, row_w);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = pack_t<DT>(acc[c + 2 * i], acc[c + 2 * i + 1]);
-            store_piece(out_s, turn_out, lane, w, &ymap, n0 + c, row_w);
-          }
+          for (int i = 0; i < 16; ++i) w[i] = pack_t<DT>(acc[(c + 2 * i) % W], acc[(c + 2 * i + 1) % W]);
         }
-      } else if (live) {
-#pragma unroll
-        for (int c = 0; c < W; c += 32)
-          if (n0 + c < a.N) store_values<DT, 32>(a, row, n0 + c, acc + c);
+        if (whole) {
+          store_piece(out_s, turn_out, lane, w, &ymap, n0 + c, row_w);
+        } else {
+          store_piece_by_rows(out_s, lane, w, reinterpret_cast<uint8_t*>(a.y) + (row_w * a.ldy + n0 + c) * size,
+                              a.ldy * size, size, rows_w, min(kStoreBytes / size, a.N - n0 - c), a.tile_store != 0);
+        }
       }
     }
     // the tile stores have read their shared memory
@@ -779,7 +793,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int FMT, int DT, int CG, int BN>
-cudaError_t launch_typed(const CUtensorMap& xmap, const CUtensorMap& wmap, const CUtensorMap& ymap, const ExpertGemmArgs& a, int num_sms,
+cudaError_t launch_typed(const CUtensorMap& xmap, const CUtensorMap& xmap_part, const CUtensorMap& wmap, const CUtensorMap& ymap, const ExpertGemmArgs& a, int num_sms,
                          cudaStream_t stream, bool pdl) {
   auto kernel = expert_gemm_kernel<FMT, DT, CG, BN>;
   static SharedMemoryOptIn opt_in;
@@ -792,22 +806,22 @@ cudaError_t launch_typed(const CUtensorMap& xmap, const CUtensorMap& wmap, const
   const int64_t groups = a.offsets == nullptr ? 1 : std::min(a.experts, a.rows);
   const int64_t tiles = ((a.rows + tile_rows - 1) / tile_rows + groups) * ((a.N + BN - 1) / BN);
   const int clusters = static_cast<int>(std::min<int64_t>(tiles, num_sms / cluster));
-  return launch_clustered(kernel, dim3(clusters * cluster), dim3(kThreads), p.bytes, stream, pdl, cluster, xmap, wmap, ymap, a);
+  return launch_clustered(kernel, dim3(clusters * cluster), dim3(kThreads), p.bytes, stream, pdl, cluster, xmap, xmap_part, wmap, ymap, a);
 }
 
 template <int FMT, int DT>
-cudaError_t launch_config(const ExpertGemmConfig& cfg, const CUtensorMap& xmap, const CUtensorMap& wmap,
-                          const CUtensorMap& ymap, const ExpertGemmArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
-  if (cfg.pair == 2) return launch_typed<FMT, DT, 2, 256>(xmap, wmap, ymap, a, num_sms, stream, pdl);
-  if (cfg.bn == 256) return launch_typed<FMT, DT, 1, 256>(xmap, wmap, ymap, a, num_sms, stream, pdl);
-  if (cfg.bn == 128) return launch_typed<FMT, DT, 1, 128>(xmap, wmap, ymap, a, num_sms, stream, pdl);
-  return launch_typed<FMT, DT, 1, 64>(xmap, wmap, ymap, a, num_sms, stream, pdl);
+cudaError_t launch_config(const ExpertGemmConfig& cfg, const CUtensorMap& xmap, const CUtensorMap& xmap_part,
+                          const CUtensorMap& wmap, const CUtensorMap& ymap, const ExpertGemmArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
+  if (cfg.pair == 2) return launch_typed<FMT, DT, 2, 256>(xmap, xmap_part, wmap, ymap, a, num_sms, stream, pdl);
+  if (cfg.bn == 256) return launch_typed<FMT, DT, 1, 256>(xmap, xmap_part, wmap, ymap, a, num_sms, stream, pdl);
+  if (cfg.bn == 128) return launch_typed<FMT, DT, 1, 128>(xmap, xmap_part, wmap, ymap, a, num_sms, stream, pdl);
+  return launch_typed<FMT, DT, 1, 64>(xmap, xmap_part, wmap, ymap, a, num_sms, stream, pdl);
 }
 
 }  // namespace
 
-cudaError_t launch_expert_gemm(int dtype, bool e4m3, const CUtensorMap& xmap, const CUtensorMap& wmap,
-                               const CUtensorMap& ymap, const ExpertGemmConfig& cfg, ExpertGemmArgs a, int num_sms, cudaStream_t stream,
+cudaError_t launch_expert_gemm(int dtype, bool e4m3, const CUtensorMap& xmap, const CUtensorMap& xmap_part,
+                               const CUtensorMap& wmap, const CUtensorMap& ymap, const ExpertGemmConfig& cfg, ExpertGemmArgs a, int num_sms, cudaStream_t stream,
                                bool pdl) {
   a.splits = cfg.splits;
   const int KB = (a.K + (e4m3 ? 127 : 63)) / (e4m3 ? 128 : 64);
@@ -818,10 +832,10 @@ cudaError_t launch_expert_gemm(int dtype, bool e4m3, const CUtensorMap& xmap, co
   if ((cfg.splits - 1) * ((KB + cfg.splits - 1) / cfg.splits) >= KB) return cudaErrorInvalidValue;
   if (pair && cfg.bn != 256) return cudaErrorInvalidValue;
   if (e4m3)
-    return dtype == kF16 ? launch_config<kFmtE4M3, kF16>(cfg, xmap, wmap, ymap, a, num_sms, stream, pdl)
-                         : launch_config<kFmtE4M3, kBF16>(cfg, xmap, wmap, ymap, a, num_sms, stream, pdl);
-  return dtype == kF16 ? launch_config<kFmtF16, kF16>(cfg, xmap, wmap, ymap, a, num_sms, stream, pdl)
-                       : launch_config<kFmtBF16, kBF16>(cfg, xmap, wmap, ymap, a, num_sms, stream, pdl);
+    return dtype == kF16 ? launch_config<kFmtE4M3, kF16>(cfg, xmap, xmap_part, wmap, ymap, a, num_sms, stream, pdl)
+                         : launch_config<kFmtE4M3, kBF16>(cfg, xmap, xmap_part, wmap, ymap, a, num_sms, stream, pdl);
+  return dtype == kF16 ? launch_config<kFmtF16, kF16>(cfg, xmap, xmap_part, wmap, ymap, a, num_sms, stream, pdl)
+                       : launch_config<kFmtBF16, kBF16>(cfg, xmap, xmap_part, wmap, ymap, a, num_sms, stream, pdl);
 }
 
 ExpertGemmConfig plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, bool codes_out, int num_sms) {

@@ -10,6 +10,7 @@
 namespace cq {
 
 constexpr int kGemmRows = 128;  // rows of x per CTA
+constexpr int kGemmBoxRows = 32;  // rows of one copy where a tile is not full
 
 // How one call is cut: CTAs per MMA (1, or 2 sharing one of 256 rows), weight
 // rows per tile (64, 128 or 256), and CTAs that share a tile's k (with pairs
@@ -41,10 +42,11 @@ constexpr int kStoreRows = 32, kStoreBytes = 64;
 
 // ymap: [rows, N] of y in its own type, box 64 bytes x 32 rows, 64-byte
 // swizzle; used where a.tile_store says that y's rows allow it (16-byte
-// aligned).  xmap: [rows, K] of x, box 128 bytes x 128 rows; wmap: [experts * N, K], box
-// 128 bytes x bn / pair rows; both with the 128-byte swizzle.
-cudaError_t launch_expert_gemm(int dtype, bool e4m3, const CUtensorMap& xmap, const CUtensorMap& wmap,
-                               const CUtensorMap& ymap, const ExpertGemmConfig& cfg, ExpertGemmArgs a, int num_sms, cudaStream_t stream,
+// aligned).  xmap, xmap_part: [rows, K] of x, box 128 bytes x 128 and x 32 rows;
+// wmap: [experts * N, K], box 128 bytes x bn / pair rows; all with the 128-byte
+// swizzle.
+cudaError_t launch_expert_gemm(int dtype, bool e4m3, const CUtensorMap& xmap, const CUtensorMap& xmap_part,
+                               const CUtensorMap& wmap, const CUtensorMap& ymap, const ExpertGemmConfig& cfg, ExpertGemmArgs a, int num_sms, cudaStream_t stream,
                                bool pdl);
 
 ExpertGemmConfig plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, bool codes_out, int num_sms);

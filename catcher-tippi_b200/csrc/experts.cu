@@ -212,6 +212,7 @@ void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, cons
   const cq::ExpertGemmConfig cfg = cq::plan_expert_gemm(e4m3(), rows, experts_, N_, K_, codes, ctx.num_sms);
   const int size = e4m3() ? 1 : 2, k = 128 / size;
   const CUtensorMap xmap = make_map_2d(from, size, rows, K_, ld, cq::kGemmRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
+  const CUtensorMap xpart = make_map_2d(from, size, rows, K_, ld, cq::kGemmBoxRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
   const CUtensorMap wmap =
       make_map_2d(weight_.get(), size, experts_ * N_, K_, ldw_, cfg.bn / cfg.pair, k, CU_TENSOR_MAP_SWIZZLE_128B);
   CUtensorMap ymap = xmap;
@@ -220,7 +221,7 @@ void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, cons
   if (a.tile_store)
     ymap = make_map_2d(out.y, ysize, rows, codes ? static_cast<int>(out.ld) : N_, out.ld, cq::kStoreRows,
                        cq::kStoreBytes / ysize, CU_TENSOR_MAP_SWIZZLE_64B);
-  check_cuda(cq::launch_expert_gemm(dtype_, e4m3(), xmap, wmap, ymap, cfg, a, ctx.num_sms, stream, pdl), "expert product");
+  check_cuda(cq::launch_expert_gemm(dtype_, e4m3(), xmap, xpart, wmap, ymap, cfg, a, ctx.num_sms, stream, pdl), "expert product");
 }
 
 void ExpertLinear::forward(const void* x, int64_t ldx, int rows, const int32_t* offsets, void* y, int64_t ldy, int act,

@@ -10,8 +10,10 @@ from __future__ import annotations
 import ctypes
 from typing import NamedTuple
 
+import torch
+
 from . import ACTS, DTYPES, _check, _ptr, lib
-from .fp8 import _allocating, _bytes, _Layer, _packed, _refuse, _rows_of, _stream_of, _torch, _types, blocks
+from .fp8 import CODES, SIZE_MAX, TYPES, _allocating, _bytes, _Layer, _packed, _refuse, _rows_of, _stream_of, blocks
 
 FORMATS = {"16bit": 0, "e4m3": 1}
 
@@ -27,58 +29,52 @@ class Route(NamedTuple):
 
 def route(logits, top: int, renormalize: bool = True, stream=None) -> Route:
     """Router logits torch [tokens, experts] (f32, f16 or bf16) -> each token's `top` best experts and the order of pairs."""
-    torch = _torch()
     if logits.dim() != 2:
         _refuse(f"logits must be [tokens, experts], got shape {tuple(logits.shape)}")
     tokens, experts = logits.shape
     _rows_of(logits, experts, "logits")
-    kind = _types().get(logits.dtype)
+    kind = CODES.get(logits.dtype)
     if kind is None:
         _refuse(f"logits have type {logits.dtype}, expected f32, f16 or bf16")
-    L = lib()
+    L, device = lib(), logits.device
     n = L.cq_route_workspace(tokens, experts, top)
-    if n == ctypes.c_size_t(-1).value:
+    if n == SIZE_MAX:
         _check(-1)
-    # one allocation for the integers, each array on a 256-byte boundary, and the workspace behind them
-    pairs = tokens * top
-    step = -(-pairs // 64) * 64
-    with _allocating(stream, logits.device):
-        ints = torch.empty(3 * step + -(-(experts + 1) // 64) * 64 + n // 4, dtype=torch.int32, device=logits.device)
-        weight = torch.empty((tokens, top), dtype=torch.float32, device=logits.device)
-    expert, position, token = ints[:pairs].view(tokens, top), ints[step:step + pairs].view(tokens, top), \
-        ints[2 * step:2 * step + pairs]
-    offsets = ints[3 * step:3 * step + experts + 1]
-    at = ints.data_ptr()
-    _check(L.cq_route(logits.data_ptr(), logits.stride(0), DTYPES[kind], tokens, experts, top, int(renormalize), at,
-                      weight.data_ptr(), at + 12 * step, at + 8 * step, at + 4 * step,
-                      at + 4 * (ints.numel() - n // 4) if n else None, n,
-                      _stream_of(stream, logits.device)))
+    with _allocating(stream, device):
+        expert, position = both = torch.empty((2, tokens, top), dtype=torch.int32, device=device)
+        token = torch.empty(tokens * top, dtype=torch.int32, device=device)
+        offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
+        weight = torch.empty((tokens, top), dtype=torch.float32, device=device)
+        ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+        at = both.data_ptr()
+        _check(L.cq_route(logits.data_ptr(), logits.stride(0), kind, tokens, experts, top, int(renormalize), at,
+                          weight.data_ptr(), offsets.data_ptr(), token.data_ptr(), at + 4 * tokens * top,
+                          ws.data_ptr() if n else None, n, _stream_of(stream, device)))
     return Route(expert, weight, offsets, token, position)
 
 
 def combine(z, position, weight, y=None, stream=None):
     """y[t] = sum_j weight[t, j] z[position[t, j]]: z torch [rows, dims] f16 or bf16, position int32 and weight f32 [tokens, top]."""
-    torch = _torch()
     if z.dim() != 2 or position.dim() != 2 or tuple(weight.shape) != tuple(position.shape):
         _refuse(f"expected rows, and positions and weights [tokens, top]; got shapes {tuple(z.shape)}, "
                 f"{tuple(position.shape)} and {tuple(weight.shape)}")
     rows, dims = z.shape
     tokens, top = position.shape
     _rows_of(z, dims, "rows")
-    kind = _types().get(z.dtype)
-    if kind not in ("f16", "bf16"):
+    kind = CODES.get(z.dtype)
+    if kind is None or z.dtype is torch.float32:
         _refuse(f"rows have type {z.dtype}, expected f16 or bf16")
     if position.dtype != torch.int32 or weight.dtype != torch.float32 or not position.is_contiguous() or \
             not weight.is_contiguous() or position.device != z.device or weight.device != z.device:
         _refuse("positions must be int32 and weights f32, without gaps, on the device of the rows")
     if y is None:
         with _allocating(stream, z.device):
-            y = torch.empty((tokens, dims), dtype=z.dtype, device=z.device)
+            y = z.new_empty((tokens, dims))
     elif y.dtype != z.dtype or y.shape[0] != tokens:
         _refuse(f"output must be {z.dtype} with {tokens} rows")
     _rows_of(y, dims, "output")
     _check(lib().cq_expert_combine(z.data_ptr(), z.stride(0), rows, position.data_ptr(), weight.data_ptr(), tokens,
-                                   top, dims, DTYPES[kind], y.data_ptr(), y.stride(0), _stream_of(stream, z.device)))
+                                   top, dims, kind, y.data_ptr(), y.stride(0), _stream_of(stream, z.device)))
     return y
 
 
@@ -106,7 +102,7 @@ class ExpertLinear(_Layer):
     @classmethod
     def from_weight(cls, weight, bias=None, device: int = 0) -> "ExpertLinear":
         """torch f16 or bf16 weights [experts, N, K] and bias [experts, N] or None, host or device."""
-        kind = _types().get(weight.dtype)
+        kind = TYPES.get(weight.dtype)
         if kind not in ("f16", "bf16"):
             _refuse(f"weight has type {weight.dtype}, expected f16 or bf16")
         return cls._create(weight, None, bias, "16bit", kind, device)
@@ -121,9 +117,9 @@ class ExpertLinear(_Layer):
     def forward(self, x, offsets, y=None, act: str = "none", stream=None):
         """x torch [rows, K] of T, offsets int32 [experts + 1] on the device -> y [rows, N], zeros from offsets[-1] on."""
         _rows_of(x, self.input_dims)
-        if offsets.dtype != _torch().int32 or tuple(offsets.shape) != (self.experts + 1,) or \
-                not offsets.is_contiguous() or offsets.device != self._torch_device:
-            _refuse(f"offsets must be int32 [{self.experts + 1}] on {self._torch_device}, got {offsets.dtype} "
+        if offsets.dtype != torch.int32 or tuple(offsets.shape) != (self.experts + 1,) or \
+                not offsets.is_contiguous() or offsets.device != self._device:
+            _refuse(f"offsets must be int32 [{self.experts + 1}] on {self._device}, got {offsets.dtype} "
                     f"{tuple(offsets.shape)} on {offsets.device}")
         L = lib()
         with _allocating(stream, x.device):
@@ -147,7 +143,7 @@ class ExpertFeedForward:
         n = self._sizes.get(tokens)
         if n is None:
             n = lib().cq_expert_ffn_workspace(self.up._h, self.down._h, tokens, self.top)
-            if n == ctypes.c_size_t(-1).value:
+            if n == SIZE_MAX:
                 _check(-1)
             if len(self._sizes) > 256:
                 self._sizes.clear()
@@ -156,12 +152,11 @@ class ExpertFeedForward:
 
     def forward(self, x, logits, y=None, stream=None):
         """x torch [tokens, K] of T, logits [tokens, experts] (f32, f16 or bf16) -> y [tokens, N]."""
-        torch = _torch()
         up, down = self.up, self.down
         _rows_of(x, up.input_dims)
         _rows_of(logits, up.experts, "logits")
         tokens = x.shape[0]
-        kind = _types().get(logits.dtype)
+        kind = CODES.get(logits.dtype)
         if kind is None or logits.shape[0] != tokens:
             _refuse(f"logits must be f32, f16 or bf16 with {tokens} rows, got {logits.dtype} {tuple(logits.shape)}")
         if tokens > 0x7FFFFFFF // self.top:
@@ -173,7 +168,7 @@ class ExpertFeedForward:
             y = down._output(x, y)
             ws = torch.empty(n, dtype=torch.uint8, device=x.device)
             _check(lib().cq_expert_ffn_forward(up._h, down._h, x.data_ptr(), x.stride(0), tokens, logits.data_ptr(),
-                                               logits.stride(0), DTYPES[kind], self.top, int(self.renormalize),
+                                               logits.stride(0), kind, self.top, int(self.renormalize),
                                                ACTS[self.act], y.data_ptr(), y.stride(0), ws.data_ptr(), n,
                                                _stream_of(stream, x.device)))
         return y

@@ -10,20 +10,17 @@ import contextlib
 import ctypes
 
 import numpy as np
+import torch
 
 from . import ACTS, CQ_INVALID_ARGUMENT, DTYPES, CQError, _check, _ptr, lib
 
 BLOCK = 128
-
-
-def _torch():
-    import torch
-    return torch
-
-
-def _types():
-    torch = _torch()
-    return {torch.float16: "f16", torch.bfloat16: "bf16", torch.float32: "f32"}
+TYPES = {torch.float16: "f16", torch.bfloat16: "bf16", torch.float32: "f32"}
+# dtype -> the library's code, for the calls
+CODES = {t: DTYPES[name] for t, name in TYPES.items()}
+SIZE_MAX = ctypes.c_size_t(-1).value
+# the stream as a number, without building torch's Stream object (2 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _refuse(message: str):
@@ -32,16 +29,18 @@ def _refuse(message: str):
 
 def _stream_of(stream, device) -> int:
     if stream is None:
-        return _torch().cuda.current_stream(device).cuda_stream
+        return _raw_stream(device.index)
     return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _allocating(stream, device):
     """The context in which a call's tensors are allocated: torch's memory pool goes by the stream that uses it."""
     if stream is None:
-        return contextlib.nullcontext()
-    cuda = _torch().cuda
-    return cuda.stream(cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream)
+        return _HERE
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream)
 
 
 def _contiguous(a):
@@ -82,19 +81,17 @@ class _Layer:
         self._h = handle
         self.experts, self.output_dims, self.input_dims = experts, output_dims, input_dims
         self.dtype, self.device = dtype, device
-        torch = _torch()
         self._type = {"f16": torch.float16, "bf16": torch.bfloat16}[dtype]
-        self._torch_device = torch.device("cuda", device)
+        self._device = torch.device("cuda", device)
         self._sizes: dict[int, int] = {}
 
     def _output(self, x, y):
-        torch = _torch()
-        if x.device != self._torch_device:
-            _refuse(f"input is on {x.device}, the layer on {self._torch_device}")
+        if x.device != self._device:
+            _refuse(f"input is on {x.device}, the layer on {self._device}")
         if x.dtype != self._type:
             _refuse(f"input has type {x.dtype}, expected {self._type}")
         if y is None:
-            return torch.empty((x.shape[0], self.output_dims), dtype=self._type, device=x.device)
+            return x.new_empty((x.shape[0], self.output_dims))
         if y.dtype != self._type or y.shape[0] != x.shape[0]:
             _refuse(f"output must be {self._type} with {x.shape[0]} rows")
         _rows_of(y, self.output_dims, "output")
@@ -109,7 +106,7 @@ class _Layer:
             n = self._sizes[rows] = entry(self._h, rows)
         if n == 0:
             return None, None, 0
-        w = _torch().empty(n, dtype=_torch().uint8, device=self._torch_device)
+        w = torch.empty(n, dtype=torch.uint8, device=self._device)
         return w, w.data_ptr(), n
 
     def close(self) -> None:
@@ -168,9 +165,8 @@ class Fp8Linear(_Layer):
 
     def forward_codes(self, codes, scales, y=None, act: str = "none", stream=None):
         """forward on rows that quantize_rows made: codes [rows, >= K], scales [ceil(K / 128), rows]."""
-        torch = _torch()
-        if codes.device != self._torch_device or scales.device != self._torch_device:
-            _refuse(f"codes and scales must be on {self._torch_device}")
+        if codes.device != self._device or scales.device != self._device:
+            _refuse(f"codes and scales must be on {self._device}")
         rows = codes.shape[0]
         if codes.dim() != 2 or codes.shape[1] < self.input_dims or codes.stride(1) != 1 or _bytes(codes) != 1:
             _refuse(f"codes must be rows of at least {self.input_dims} bytes, got shape {tuple(codes.shape)}")
@@ -191,12 +187,11 @@ class Fp8Linear(_Layer):
 
 def quantize_rows(x, stream=None):
     """x torch [rows, K] (f16, bf16 or f32) -> (e4m3 codes [rows, 128 ceil(K / 128)], scales f32 [ceil(K / 128), rows])."""
-    torch = _torch()
     if x.dim() != 2:
         _refuse(f"input must be rows, got shape {tuple(x.shape)}")
     rows, k = x.shape
     _rows_of(x, k)
-    kind = _types().get(x.dtype)
+    kind = TYPES.get(x.dtype)
     if kind is None:
         _refuse(f"input has type {x.dtype}, expected f16, bf16 or f32")
     with _allocating(stream, x.device):
@@ -209,7 +204,6 @@ def quantize_rows(x, stream=None):
 
 def quantize_weight(w, stream=None):
     """w torch f32 [N, K] on the device -> (e4m3 codes [N, K], scales f32 [ceil(N / 128), ceil(K / 128)])."""
-    torch = _torch()
     if not w.is_cuda or w.dim() != 2 or w.dtype != torch.float32 or not w.is_contiguous():
         _refuse("weight must be f32 [N, K] without gaps on the device")
     n, k = w.shape
