@@ -12,13 +12,6 @@ namespace cq {
 constexpr int kGemmRows = 128;  // rows of x per CTA
 constexpr int kGemmBoxRows = 32;  // rows of one copy where a tile is not full
 
-// How one call is cut: CTAs per MMA (1, or 2 sharing one of 256 rows), weight
-// rows per tile (64, 128 or 256), and CTAs that share a tile's k (with pairs
-// and 256-wide tiles: 1).
-struct ExpertGemmConfig {
-  int pair, bn, splits;
-};
-
 // What a value of y becomes: T, f32, or e4m3 codes with their scales.
 enum ExpertOut : int { kOutT = 0, kOutF32 = 1, kOutCodes = 2 };
 
@@ -27,28 +20,30 @@ struct ExpertGemmArgs {
   const float* w_scales;  // e4m3: [experts][n blocks][k blocks]
   const void* bias;       // T [experts][N] or null
   const int32_t* offsets; // null: all rows meet expert 0
+  int offsets_ready;      // the kernel launched before this one began after what wrote the offsets was done
   int rows, experts, N, K, act;
   int out;
   void* y;  // T, f32 or codes, row stride ldy
   int64_t ldy;
   float* y_scales;  // kOutCodes: [ceil(N / 128)][rows]
   int* status;
-  int splits;
   int tile_store;
 };
 
 // The box of a tile store: 64 bytes of 32 rows.
 constexpr int kStoreRows = 32, kStoreBytes = 64;
 
-// ymap: [rows, N] of y in its own type, box 64 bytes x 32 rows, 64-byte
-// swizzle; used where a.tile_store says that y's rows allow it (16-byte
-// aligned).  xmap, xmap_part: [rows, K] of x, box 128 bytes x 128 and x 32 rows;
-// wmap: [experts * N, K], box 128 bytes x bn / pair rows; all with the 128-byte
-// swizzle.
-cudaError_t launch_expert_gemm(int dtype, bool e4m3, const CUtensorMap& xmap, const CUtensorMap& xmap_part,
-                               const CUtensorMap& wmap, const CUtensorMap& ymap, const ExpertGemmConfig& cfg, ExpertGemmArgs a, int num_sms, cudaStream_t stream,
-                               bool pdl);
+// Tensor maps of one call.  x, x_part: [rows, K], box 128 bytes x 128 and x 32
+// rows; w: [experts * N, K], box 128 bytes x bn rows; all with the 128-byte
+// swizzle.  y: [rows, N] in its own type, box 64 bytes x 32 rows, 64-byte
+// swizzle, used where tile_store says that y's rows allow it (16-byte aligned).
+struct ExpertGemmMaps {
+  CUtensorMap x, x_part, w, y;
+};
 
-ExpertGemmConfig plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, bool codes_out, int num_sms);
+// bn: weight rows of a tile, 64, 128 or 256 (codes: 256), as planned below.
+cudaError_t launch_expert_gemm(int dtype, bool e4m3, int bn, const ExpertGemmMaps& maps, const ExpertGemmArgs& a,
+                               int num_sms, cudaStream_t stream, bool pdl);
+int plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, int num_sms);
 
 }  // namespace cq

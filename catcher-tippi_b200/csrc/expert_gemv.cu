@@ -95,22 +95,39 @@ __device__ __forceinline__ void stage_x(const ExpertGemvArgs& a, int begin, int 
   if constexpr (F8 && SRC != kSourceCodes) {
     constexpr int kSize = SRC == kSourceF32 ? 4 : 2;
     const bool aligned = ((a.ldx * kSize) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+    // half warps share the rows out, a power of two of them to a row, each
+    // with up to four of its blocks on their way
     const int half = threadIdx.x >> 4, lane = threadIdx.x & 15;
-    const int items = n * blocks;
-    for (int base = 0; base < items; base += kThreads / 16) {
-      const int item = base + half;
-      const bool live = item < items;
-      const int r = live ? item / blocks : 0, b = live ? item - r * blocks : 0;
-      const int64_t src = !live ? -1 : a.row_index != nullptr ? a.row_index[begin + r] : begin + r;
-      constexpr int T = SRC == kSourceF32 ? static_cast<int>(kF32) : DT;
-      Raw8<T> raw{};
-      if (src >= 0 && src < a.x_rows)
-        raw = load_row8<T>(reinterpret_cast<const char*>(a.x) + src * a.ldx * kSize, (kb0 + b) * kFp8Block + lane * 8, a.K, aligned);
-      int e;
-      const uint2 out = quantize8<T>(raw, e);
-      if (!live) continue;
-      *reinterpret_cast<uint2*>(xs + r * pitch + b * 128 + lane * 8) = out;
-      if (lane == 0) sx[b * kPassRows + r] = pow2f(e);
+    constexpr int kHalves = kThreads / 16, kFlight = 4;
+    const int shift = n > 8 ? 0 : n > 4 ? 1 : n > 2 ? 2 : n > 1 ? 3 : 4;  // log2 of half warps to a row
+    constexpr int T = SRC == kSourceF32 ? static_cast<int>(kF32) : DT;
+    for (int r0 = 0; r0 < n; r0 += kHalves >> shift) {
+      const int r = r0 + (half >> shift);
+      int64_t src = -1;
+      if (r < n) src = a.row_index != nullptr ? a.row_index[begin + r] : begin + r;
+      const bool there = src >= 0 && src < a.x_rows;
+      const char* row = reinterpret_cast<const char*>(a.x) + src * a.ldx * kSize;
+      // the same turns in every half warp: the shuffles below are the warp's
+      for (int b0 = 0; b0 < blocks; b0 += kFlight << shift) {
+        Raw8<T> raw[kFlight];
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) {
+          const int b = b0 + (u << shift) + (half & ((1 << shift) - 1));
+          raw[u] = Raw8<T>{};
+          if (there && b < blocks) raw[u] = load_row8<T>(row, (kb0 + b) * kFp8Block + lane * 8, a.K, aligned);
+        }
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) {
+          const int b = b0 + (u << shift) + (half & ((1 << shift) - 1));
+          if (b0 + (u << shift) >= blocks) break;
+          int e;
+          const uint2 out = quantize8<T>(raw[u], e);
+          if (r < n && b < blocks) {
+            *reinterpret_cast<uint2*>(xs + r * pitch + b * 128 + lane * 8) = out;
+            if (lane == 0) sx[b * kPassRows + r] = pow2f(e);
+          }
+        }
+      }
     }
   } else {
     // 16 bytes a thread
@@ -327,7 +344,7 @@ int smem_of(bool e4m3, int rows, int KB, int bands, int splits) {
 GemvPlan plan(bool e4m3, int rows, int groups, int N, int K, int num_sms) {
   const int KB = (K + (e4m3 ? 127 : 63)) / (e4m3 ? 128 : 64);
   GemvPlan p{2, 1, 0};
-  if (static_cast<int64_t>((N + 31) / 32) * groups < num_sms) p.bands = 1;
+  if (static_cast<int64_t>((N + 31) / 32) * groups < num_sms / 2) p.bands = 1;
   const int64_t ctas = static_cast<int64_t>((N + 16 * p.bands - 1) / (16 * p.bands)) * groups;
   const int slices = kWarps / p.bands;
   // split k while a warp still has a block of its own and the GPU has room, or

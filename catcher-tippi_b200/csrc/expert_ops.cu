@@ -24,8 +24,8 @@ constexpr int kQuantBlocks = 4;
 template <int DT>
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const QuantizeRowsArgs a) {
   __shared__ float scale_s[kQuantBlocks][kQuantRows];
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();  // in this order: the product after it may rely on the offsets
   constexpr int kSize = DT == kF32 ? 4 : 2;
   const int blocks = (a.cols + kFp8Block - 1) / kFp8Block;
   const bool aligned = ((a.ldx * kSize) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
@@ -94,8 +94,8 @@ __global__ void __launch_bounds__(256) round_kernel(const float* v, int64_t n, v
 // 16-bit rows to 16-byte aligned rows, eight values a thread: the order of a
 // row list, or rows whose own alignment a tile copy cannot take.
 __global__ void __launch_bounds__(256) gather_rows_kernel(const GatherRowsArgs a) {
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();  // in this order: the product after it may rely on the offsets
   const int chunks = (a.cols + 7) / 8;
   const bool aligned = (a.ldx & 7) == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
   const int64_t items = static_cast<int64_t>(a.rows) * chunks;

@@ -151,8 +151,7 @@ size_t ExpertLinear::staging_bytes(int64_t rows) const {
 size_t ExpertLinear::workspace(int rows) const { return round_up(staging_bytes(rows), 256); }
 
 bool ExpertLinear::few_rows(int rows, bool grouped) const {
-  const int groups = grouped ? std::min(experts_, rows) : 1;
-  return rows <= 16 * groups && rows <= 64 && cq::expert_gemv_fits(e4m3(), rows, K_);
+  return !grouped && rows <= 32 && cq::expert_gemv_fits(e4m3(), rows, K_);
 }
 
 void ExpertLinear::check_rows(const void* x, int64_t ldx, int rows, const void* y, int64_t ldy, int act) const {
@@ -179,6 +178,7 @@ void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, cons
   const void* from = x.x;
   int64_t ld = x.ld;
   const float* x_scales = x.scales;
+  bool staged = false;
   if (e4m3() && x.source != cq::kSourceCodes) {
     ld = round_up(K_, kBlock);
     float* s = reinterpret_cast<float*>(static_cast<char*>(staging) + round_up(rows * ld, 256));
@@ -187,17 +187,20 @@ void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, cons
                "quantize rows");
     from = staging;
     x_scales = s;
+    staged = true;
   } else if (!e4m3() && (x.row_index != nullptr || x.ld % 8 != 0 || (reinterpret_cast<uintptr_t>(x.x) & 15) != 0)) {
     ld = round_up(K_, 8);
     const cq::GatherRowsArgs g{x.x, x.ld, x.row_index, x.x_rows, rows, K_, staging, ld};
     check_cuda(cq::launch_gather_rows(g, stream, pdl), "gather rows");
     from = staging;
+    staged = true;
   }
   cq::ExpertGemmArgs a{};
   a.x_scales = x_scales;
   a.w_scales = scales_.as<float>();
   a.bias = bias_.get();
   a.offsets = offsets;
+  a.offsets_ready = staged || x.offsets_ready;
   a.rows = rows;
   a.experts = experts_;
   a.N = N_;
@@ -209,19 +212,18 @@ void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, cons
   a.y_scales = out.scales;
   a.status = ctx.status;
   const bool codes = out.kind == cq::kOutCodes;
-  const cq::ExpertGemmConfig cfg = cq::plan_expert_gemm(e4m3(), rows, experts_, N_, K_, codes, ctx.num_sms);
+  const int bn = codes ? 256 : cq::plan_expert_gemm(e4m3(), rows, experts_, N_, K_, ctx.num_sms);
   const int size = e4m3() ? 1 : 2, k = 128 / size;
-  const CUtensorMap xmap = make_map_2d(from, size, rows, K_, ld, cq::kGemmRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
-  const CUtensorMap xpart = make_map_2d(from, size, rows, K_, ld, cq::kGemmBoxRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
-  const CUtensorMap wmap =
-      make_map_2d(weight_.get(), size, experts_ * N_, K_, ldw_, cfg.bn / cfg.pair, k, CU_TENSOR_MAP_SWIZZLE_128B);
-  CUtensorMap ymap = xmap;
   const int ysize = codes ? 1 : out.kind == cq::kOutF32 ? 4 : 2;
   a.tile_store = out.ld * ysize % 16 == 0 && (reinterpret_cast<uintptr_t>(out.y) & 15) == 0;
-  if (a.tile_store)
-    ymap = make_map_2d(out.y, ysize, rows, codes ? static_cast<int>(out.ld) : N_, out.ld, cq::kStoreRows,
-                       cq::kStoreBytes / ysize, CU_TENSOR_MAP_SWIZZLE_64B);
-  check_cuda(cq::launch_expert_gemm(dtype_, e4m3(), xmap, xpart, wmap, ymap, cfg, a, ctx.num_sms, stream, pdl), "expert product");
+  cq::ExpertGemmMaps maps;
+  maps.x = make_map_2d(from, size, rows, K_, ld, cq::kGemmRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
+  maps.x_part = make_map_2d(from, size, rows, K_, ld, cq::kGemmBoxRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
+  maps.w = make_map_2d(weight_.get(), size, experts_ * N_, K_, ldw_, bn, k, CU_TENSOR_MAP_SWIZZLE_128B);
+  maps.y = !a.tile_store ? maps.x
+                         : make_map_2d(out.y, ysize, rows, codes ? static_cast<int>(out.ld) : N_, out.ld,
+                                       cq::kStoreRows, cq::kStoreBytes / ysize, CU_TENSOR_MAP_SWIZZLE_64B);
+  check_cuda(cq::launch_expert_gemm(dtype_, e4m3(), bn, maps, a, ctx.num_sms, stream, pdl), "expert product");
 }
 
 void ExpertLinear::forward(const void* x, int64_t ldx, int rows, const int32_t* offsets, void* y, int64_t ldy, int act,
@@ -414,6 +416,7 @@ void expert_ffn(const ExpertLinear& up, const ExpertLinear& down, const void* x,
   ExpertLinear::Rows h{cq::kSourceT, s.h, s.ld_h, nullptr, nullptr, pairs};
   if (!up.e4m3()) {
     up.product(rows, pairs, s.offsets, {cq::kOutT, s.h, s.ld_h, nullptr}, act, s.x, stream);
+    h.offsets_ready = true;  // a gather and the first product ran since the route
   } else if (up.few_rows(pairs, true)) {
     up.product(rows, pairs, s.offsets, {cq::kOutF32, s.h, s.ld_h, nullptr}, act, s.x, stream);
     h.source = cq::kSourceF32;
@@ -423,6 +426,7 @@ void expert_ffn(const ExpertLinear& up, const ExpertLinear& down, const void* x,
     float* scales = reinterpret_cast<float*>(static_cast<char*>(s.h) + round_up(pairs * ld, 256));
     up.product(rows, pairs, s.offsets, {cq::kOutCodes, s.h, ld, scales}, act, s.x, stream);
     h = {cq::kSourceCodes, s.h, ld, scales, nullptr, pairs};
+    h.offsets_ready = true;  // the first product ran between the route and the second
   }
   down.product(h, pairs, s.offsets, {cq::kOutF32, s.z, out, nullptr}, CQ_ACT_NONE, s.h_staged, stream);
   const cq::CombineArgs c{s.z, out, s.position, s.weight, pairs, tokens, top, out, y, ldy, 1};

@@ -47,6 +47,9 @@ class ExpertLinear {
     const float* scales;
     const int32_t* row_index;
     int x_rows;
+    // the kernel that the product follows on the stream began after what wrote
+    // the offsets was done (and says so to its dependents only then)
+    bool offsets_ready = false;
   };
   // Bytes in which product() brings rows to the form that the tensor cores'
   // tile copies take.

@@ -159,27 +159,36 @@ __device__ __forceinline__ float e4m3_to_float(uint8_t code) {
   return static_cast<float>(v);
 }
 
-// act(v) in f32 for the fp8 and expert linears' epilogues.  SiLU by the fast
-// exponential and division: a few f32 ulps, far inside T's rounding step.
-__device__ __forceinline__ float activate(float v, int act) {
-  if (act == kActSilu) return __fdividef(v, 1.0f + __expf(-v));
-  if (act == kActRelu) return v < 0.0f ? 0.0f : v;
-  return v;
+__device__ __forceinline__ float fast_exp2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float fast_reciprocal(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+
+// SiLU of two values, v / (1 + 2^(-v log2 e)): one reciprocal serves both,
+// 1 / a = b / (a b), as an epilogue of SiLUs is bound by the special-function
+// unit and by its instruction count.  -v log2 e is cut at 62, so that a b stays
+// below the range of the reciprocal: past it SiLU is under 1e-17 either way.  The approximate functions
+// are off by a few f32 ulps, far inside T's rounding step; values that a flush
+// of subnormals touches are 2^-126 next to 1.
+__device__ __forceinline__ void silu2(float& x, float& y) {
+  const float a = 1.0f + fast_exp2(fminf(-kLog2E * x, 62.0f)), b = 1.0f + fast_exp2(fminf(-kLog2E * y, 62.0f));
+  const float r = fast_reciprocal(a * b);
+  x *= r * b;
+  y *= r * a;
 }
 
-// activate for two values: one reciprocal serves both SiLUs, 1 / a = b / (a b)
-// (an epilogue of SiLUs is bound by the special-function unit).  -v is cut at
-// 60, so that a b stays finite: below -60 SiLU is under 6e-25 either way.
-__device__ __forceinline__ void activate2(float& x, float& y, int act) {
-  if (act == kActSilu) {
-    const float a = 1.0f + __expf(fminf(-x, 60.0f)), b = 1.0f + __expf(fminf(-y, 60.0f));
-    const float r = __fdividef(1.0f, a * b);
-    x *= r * b;
-    y *= r * a;
-  } else if (act == kActRelu) {
-    x = x < 0.0f ? 0.0f : x;
-    y = y < 0.0f ? 0.0f : y;
-  }
+// act(v) in f32 for the fp8 and expert linears' epilogues.
+__device__ __forceinline__ float activate(float v, int act) {
+  if (act == kActSilu) return v * fast_reciprocal(1.0f + fast_exp2(fminf(-kLog2E * v, 126.0f)));
+  if (act == kActRelu) return v < 0.0f ? 0.0f : v;
+  return v;
 }
 
 // Two f32 values rounded to T, lo in the low half.
