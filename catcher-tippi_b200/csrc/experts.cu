@@ -148,7 +148,10 @@ size_t ExpertLinear::staging_bytes(int64_t rows) const {
   return round_up(rows * ld, 256) + rows * (ld / kBlock) * sizeof(float);
 }
 
-size_t ExpertLinear::workspace(int rows) const { return round_up(staging_bytes(rows), 256); }
+size_t ExpertLinear::workspace(int rows) const {
+  // the streaming kernel of a single expert needs none
+  return experts_ == 1 && few_rows(rows, false) ? 0 : round_up(staging_bytes(rows), 256);
+}
 
 bool ExpertLinear::few_rows(int rows, bool grouped) const {
   return !grouped && rows <= 32 && cq::expert_gemv_fits(e4m3(), rows, K_);

@@ -8,6 +8,7 @@ expert, ``combine`` sums what each token's experts made, and
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -27,6 +28,14 @@ class Route(NamedTuple):
     position: object  # int32 [tokens, top]
 
 
+@functools.lru_cache(maxsize=256)
+def _route_workspace(tokens: int, experts: int, top: int) -> int:
+    n = lib().cq_route_workspace(tokens, experts, top)
+    if n == SIZE_MAX:
+        _check(-1)
+    return n
+
+
 def route(logits, top: int, renormalize: bool = True, stream=None) -> Route:
     """Router logits torch [tokens, experts] (f32, f16 or bf16) -> each token's `top` best experts and the order of pairs."""
     if logits.dim() != 2:
@@ -37,19 +46,21 @@ def route(logits, top: int, renormalize: bool = True, stream=None) -> Route:
     if kind is None:
         _refuse(f"logits have type {logits.dtype}, expected f32, f16 or bf16")
     L, device = lib(), logits.device
-    n = L.cq_route_workspace(tokens, experts, top)
-    if n == SIZE_MAX:
-        _check(-1)
+    n = _route_workspace(tokens, experts, top)
+    # one allocation: expert, weight, position and token, each from a 256-byte
+    # boundary on, then the offsets and the call's workspace
+    step = (tokens * top + 63) & ~63
+    end = 4 * step + ((experts + 64) & ~63)
     with _allocating(stream, device):
-        expert, position = both = torch.empty((2, tokens, top), dtype=torch.int32, device=device)
-        token = torch.empty(tokens * top, dtype=torch.int32, device=device)
-        offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
-        weight = torch.empty((tokens, top), dtype=torch.float32, device=device)
-        ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-        at = both.data_ptr()
-        _check(L.cq_route(logits.data_ptr(), logits.stride(0), kind, tokens, experts, top, int(renormalize), at,
-                          weight.data_ptr(), offsets.data_ptr(), token.data_ptr(), at + 4 * tokens * top,
-                          ws.data_ptr() if n else None, n, _stream_of(stream, device)))
+        ints = logits.new_empty(end + n // 4, dtype=torch.int32)
+        at = ints.data_ptr()
+        _check(L.cq_route(logits.data_ptr(), logits.stride(0), kind, tokens, experts, top, int(renormalize), at, at + 4 * step,
+                          at + 16 * step, at + 12 * step, at + 8 * step, at + 4 * end if n else None, n,
+                          _stream_of(stream, device)))
+    pairs, across = (tokens, top), (top, 1)
+    expert, weight = ints.as_strided(pairs, across, 0), ints.as_strided(pairs, across, step).view(torch.float32)
+    position, token = ints.as_strided(pairs, across, 2 * step), ints.as_strided((tokens * top,), (1,), 3 * step)
+    offsets = ints.as_strided((experts + 1,), (1,), 4 * step)
     return Route(expert, weight, offsets, token, position)
 
 

@@ -297,12 +297,14 @@ def test_expert_linear_refusals(cq):
         with pytest.raises(cq.CQError, match=needle):
             bad()
     f = fp8.Fp8Linear.from_codes(torch.zeros(8, 16, dtype=torch.uint8, device="cuda"), torch.ones(1, 1, device="cuda"))
-    L, y = cq.lib(), torch.zeros(4, 8, dtype=torch.bfloat16, device="cuda")
-    need = L.cq_fp8_linear_workspace(f._h, 4)
+    x, y = torch.zeros(40, 16, dtype=torch.bfloat16, device="cuda"), torch.zeros(40, 8, dtype=torch.bfloat16, device="cuda")
+    L = cq.lib()
+    need = L.cq_fp8_linear_workspace(f._h, 40)
+    assert L.cq_fp8_linear_workspace(f._h, 0) == 0 and need > 0
     ws = torch.zeros(need + 512, dtype=torch.uint8, device="cuda")
 
     def call(ptr, n, act=0, ldx=16, ldy=8):
-        return L.cq_fp8_linear_forward(f._h, x.data_ptr(), ldx, 4, y.data_ptr(), ldy, act, ptr, n, None)
+        return L.cq_fp8_linear_forward(f._h, x.data_ptr(), ldx, 40, y.data_ptr(), ldy, act, ptr, n, None)
     for status, needle in ((call(None, need), "workspace has 0 bytes"), (call(ws.data_ptr(), need - 1), "expected"),
                            (call(ws.data_ptr() + 16, need), "256-byte aligned"), (call(ws.data_ptr(), need, act=3), "unknown activation"),
                            (call(ws.data_ptr(), need, ldx=15), "input row stride"), (call(ws.data_ptr(), need, ldy=7), "output row stride")):
