@@ -14,7 +14,13 @@
 // tensor-memory buffer.  16-bit: kind::f16 sums all of k in tensor memory, and
 // the epilogue of a tile overlaps the next tile's products.
 //
-// Persistent: a CTA takes every W-th tile of all experts' tiles; the tile list follows from the offsets, which only the device knows.
+// Wide tiles are bound by the copies from L2: a 128 x 256 tile takes 48 KB a k
+// block, 1100 cycles at the rate that all SMs have together.  So large groups
+// run on pairs of CTAs (cta_group::2): 256 rows, each CTA half of the weights'
+// tile in its shared memory, 32 KB a CTA.
+//
+// Persistent: a CTA or pair takes every W-th tile of all experts' tiles; the
+// tile list follows from the offsets, which only the device knows.
 //   warps 0, 2  copy tiles of x and of W (TMA, 128-byte swizzle) into a ring
 //   warp 1      issues tcgen05.mma
 //               (warp 2 also owns the tensor memory)
@@ -57,9 +63,9 @@ struct SmemPlan {
   int stage_bytes, stages, out_off, scale_off, list_off, bar_off, bytes;
 };
 
-__host__ __device__ inline SmemPlan plan_smem(bool e4m3, int bn, int experts) {
+__host__ __device__ inline SmemPlan plan_smem(bool e4m3, int bn, int pair, int experts) {
   SmemPlan p{};
-  p.stage_bytes = stage_blocks(bn) * (kXBytes + bn * kRowBytes);
+  p.stage_bytes = stage_blocks(bn) * (kXBytes + bn / pair * kRowBytes);
   const int list = (2 * (experts + 2) * 4 + 15) / 16 * 16;
   const int bars = (2 * kMaxStages + 2 * kGroups + 2 * kScaleSlots) * 8 + 16;
   const int scales = e4m3 ? kScaleSlots * kScaleBytes : 0;
@@ -76,28 +82,47 @@ __host__ __device__ inline SmemPlan plan_smem(bool e4m3, int bn, int experts) {
 
 // --------------------------------------------------------------- tcgen05
 
+template <int CG>
 __device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  if constexpr (CG == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
 }
+template <int CG>
 __device__ __forceinline__ void tmem_release(uint32_t taddr, uint32_t cols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
 }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-template <int FMT>
+template <int FMT, int CG>
 __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (FMT == kFmtE4M3)
+  if constexpr (FMT == kFmtE4M3 && CG == 2)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else if constexpr (FMT == kFmtE4M3)
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else if constexpr (CG == 2)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
   else
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// Arrives on the barrier at `bar` when the MMAs issued so far are done.
+// Arrives on the barrier at `bar` when the MMAs issued so far are done; with a
+// pair, on the barrier at that place in both CTAs.
+template <int CG>
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // 32 lanes x 32 columns: thread i of the warp gets its lane's 32 columns.
@@ -132,19 +157,27 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
 }
 
 // Instruction descriptor: f32 sums, both operands K-major.
-template <int FMT>
+template <int FMT, int CG>
 __device__ __forceinline__ uint32_t mma_idesc(int n) {
   constexpr uint32_t type = FMT == kFmtBF16 ? 1u : 0u;  // f16 kind: 0 f16, 1 bf16; f8f6f4 kind: 0 e4m3
   return (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
-         (static_cast<uint32_t>(kGemmRows >> 4) << 24);
+         (static_cast<uint32_t>(kGemmRows * CG >> 4) << 24);
 }
 
-// TMA load into shared memory, counted on the barrier at `bar`.
+// TMA load into this CTA's shared memory, counted on the barrier at `bar`: of a
+// pair, the first CTA's.
+template <int CG>
 __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
-      "[%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar),
-      "l"(policy) : "memory");
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint "
+        "[%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar),
+        "l"(policy) : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar),
+        "l"(policy) : "memory");
 }
 
 // --------------------------------------------------------------- barriers
@@ -153,6 +186,12 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
 // products have a few hundred cycles a turn, and address arithmetic counts.
 __device__ __forceinline__ void arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// The same on a barrier of the pair's first CTA.  It publishes no memory (a
+// tensor-memory buffer has been read, which tcgen05.fence orders): release at
+// cluster scope would cost a fence of all outstanding stores for every k block.
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -201,13 +240,13 @@ struct TileList {
 
 // One warp.  Offsets are cut to [0, rows] and made to rise, so that whatever
 // the array holds no tile reaches outside the rows.
-__device__ __forceinline__ void build_list(const ExpertGemmArgs& a, TileList l, int tiles_n, int lane) {
+__device__ __forceinline__ void build_list(const ExpertGemmArgs& a, TileList l, int tile_rows, int tiles_n, int lane) {
   if (a.offsets == nullptr) {
     if (lane == 0) {
       l.start[0] = 0;
       l.start[1] = a.rows;
       l.tile[0] = 0;
-      l.tile[1] = (a.rows + kGemmRows - 1) / kGemmRows * tiles_n;
+      l.tile[1] = (a.rows + tile_rows - 1) / tile_rows * tiles_n;
     }
     return;
   }
@@ -222,7 +261,7 @@ __device__ __forceinline__ void build_list(const ExpertGemmArgs& a, TileList l, 
     }
     int begin = __shfl_up_sync(0xFFFFFFFFu, end, 1);
     if (lane == 0) begin = row;
-    const int mine = (end - begin + kGemmRows - 1) / kGemmRows * tiles_n;
+    const int mine = (end - begin + tile_rows - 1) / tile_rows * tiles_n;
     int sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -259,10 +298,10 @@ struct Ring {
 };
 
 // The t-th tile; `e` only moves forward.
-__device__ __forceinline__ Tile find_tile(const TileList& l, int t, int tiles_n, int bn, int& e) {
+__device__ __forceinline__ Tile find_tile(const TileList& l, int t, int tile_rows, int tiles_n, int bn, int& e) {
   while (t >= l.tile[e + 1]) ++e;
   const int i = t - l.tile[e];
-  return Tile{e, l.start[e] + i / tiles_n * kGemmRows, l.start[e + 1], i % tiles_n * bn};
+  return Tile{e, l.start[e] + i / tiles_n * tile_rows, l.start[e + 1], i % tiles_n * bn};
 }
 
 constexpr int kBoxBytes = kGemmBoxRows * kRowBytes;
@@ -354,14 +393,14 @@ __device__ __forceinline__ void group_sync(int half) {
 
 // --------------------------------------------------------------- kernel
 
-template <int FMT, int DT, int BN>
+template <int FMT, int DT, int CG, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
     expert_gemm_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap xmap_part,
                        const __grid_constant__ CUtensorMap wmap,
                        const __grid_constant__ CUtensorMap ymap, const ExpertGemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  const SmemPlan L = plan_smem(FMT == kFmtE4M3, BN, a.experts);
+  const SmemPlan L = plan_smem(FMT == kFmtE4M3, BN, CG, a.experts);
   const int stages = L.stages;
   // Tensor memory is two groups of accumulators that go back and forth between
   // the products and the epilogue: of kPer k blocks' partial sums each (e4m3),
@@ -383,7 +422,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // the same in all lanes, and known to be
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int worker = blockIdx.x, workers = gridDim.x;
+  const int rank = CG == 2 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
   const int tiles_n = (a.N + BN - 1) / BN;
   constexpr int kElems = FMT == kFmtE4M3 ? 128 : 64;  // values of a k block
   const int KB = (a.K + kElems - 1) / kElems;
@@ -398,20 +438,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       // warps; scale_full: the lanes of the scale warp
       const bool is_full = i < kMaxStages, is_scale = i >= kBarriers - 2 * kScaleSlots;
       const bool by_epilogue = i >= kBarriers - kScaleSlots || (!is_scale && i >= 2 * kMaxStages + kGroups);
-      mbar_init(bars + i, is_full ? 2 : by_epilogue ? kEpiWarps : is_scale ? 32 : 1);
+      mbar_init(bars + i, is_full ? 2 : by_epilogue ? (is_scale ? kEpiWarps : CG * kEpiWarps) : is_scale ? 32 : 1);
     }
     fence_mbar_init();
   }
-  if (warp == 2) tmem_alloc(tmem_slot, kTmemCols);
+  if (warp == 2) tmem_alloc<CG>(tmem_slot, kTmemCols);
   // Weights are nobody's result, and the offsets may be known to be there: then
   // the weights' stream starts while the kernel before still runs.  What reads
   // rows or scales, or writes y, waits for it.
   if (warp == 3) {
     if (a.offsets != nullptr && !a.offsets_ready) pdl_wait();
-    build_list(a, list, tiles_n, lane);
+    build_list(a, list, kGemmRows * CG, tiles_n, lane);
   }
   tc_fence_before();
   __syncthreads();
+  if (CG == 2) cluster_sync_all();  // the other CTA's barriers are ready
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int groups = a.offsets == nullptr ? 1 : a.experts;
@@ -434,30 +475,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       int e = 0, issued = 0;
       Ring ring;
       for (int t = worker; t < total && ok; t += workers) {
-        const Tile tile = find_tile(list, t, tiles_n, BN, e);
-        const int boxes = row_boxes(tile.end - tile.m0);
-        const int bytes = warp == 0 ? boxes * kBoxBytes : BN * kRowBytes;
-        const int w = tile.expert * a.N + tile.n0;
+        const Tile tile = find_tile(list, t, kGemmRows * CG, tiles_n, BN, e);
+        const int m = tile.m0 + rank * kGemmRows, boxes = row_boxes(tile.end - m);
+        // both CTAs' bytes count on the first's barrier
+        const int all_boxes = CG == 2 ? row_boxes(tile.end - tile.m0) + row_boxes(tile.end - tile.m0 - kGemmRows) : boxes;
+        const int bytes = warp == 0 ? all_boxes * kBoxBytes : BN * kRowBytes;
+        const int w = tile.expert * a.N + tile.n0 + rank * (BN / CG);
         for (int kb = 0; kb < KB; kb += kStageBlocks, ++issued) {
           if (!wait_phase(empty + ring.at * 8, ring.phase ^ 1u, a.status)) {
             ok = false;
             break;
           }
-          const uint32_t bar = full + ring.at * 8, dst = dst0 + ring.at * L.stage_bytes;
+          uint32_t bar = full + ring.at * 8;
+          if (CG == 2) bar = mapa_shared(bar, 0);
+          const uint32_t dst = dst0 + ring.at * L.stage_bytes;
           const int blocks = min(kStageBlocks, KB - kb);
           if (elect_one()) {
-            arrive_expect(bar, blocks * bytes);
+            if (CG == 1 || rank == 0) arrive_expect(full + ring.at * 8, blocks * bytes);
 #pragma unroll
             for (int j = 0; j < kStageBlocks; ++j) {
               if (j >= blocks) break;
               const int k = (kb + j) * kElems;
               if (warp == 2) {
-                load_tile(dst + j * BN * kRowBytes, &wmap, k, w, bar, keep);
+                load_tile<CG>(dst + j * (BN / CG) * kRowBytes, &wmap, k, w, bar, keep);
               } else if (boxes == kGemmRows / kGemmBoxRows) {
-                load_tile(dst + j * kXBytes, &xmap, k, tile.m0, bar, keep);
+                load_tile<CG>(dst + j * kXBytes, &xmap, k, m, bar, keep);
               } else {
                 for (int b = 0; b < boxes; ++b)
-                  load_tile(dst + j * kXBytes + b * kBoxBytes, &xmap_part, k, tile.m0 + b * kGemmBoxRows, bar, keep);
+                  load_tile<CG>(dst + j * kXBytes + b * kBoxBytes, &xmap_part, k, m + b * kGemmBoxRows, bar, keep);
               }
             }
           }
@@ -465,11 +510,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           ring.next(stages);
         }
       }
-      if (!ok)  // a wait ran out: let the copies in flight land before the CTA ends
+      if (!ok && rank == 0)  // a wait ran out: let the copies in flight land before the CTA ends
         for (int i = max(0, issued - stages); i < issued; ++i) wait_phase(full + i % stages * 8, (i / stages) & 1, a.status);
-    } else if (warp == 1) {
+    } else if (warp == 1 && rank == 0) {
       // ---------------------------------------------------------- products
-      const uint32_t idesc = mma_idesc<FMT>(BN);
+      const uint32_t idesc = mma_idesc<FMT, CG>(BN);
       // The tensor pipe queues few products, so this loop's scalar work has to
       // fit under them: the whole warp runs it, with values that are the same
       // in all lanes, and one lane issues; ring places by counters,
@@ -494,15 +539,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < kStageBlocks; ++j) {
               if (j >= blocks) break;
               const uint64_t a0 = da + j * (kXBytes >> 4);
-              const uint64_t b0 = da + kStageBlocks * (kXBytes >> 4) + j * (BN * kRowBytes >> 4);
+              const uint64_t b0 = da + kStageBlocks * (kXBytes >> 4) + j * (BN / CG * kRowBytes >> 4);
               const uint32_t to = FMT == kFmtE4M3 ? d + j * BN : d;
-              tc_mma<FMT>(to, a0, b0, idesc, FMT != kFmtE4M3 && (kb != 0 || j != 0));
-              tc_mma<FMT>(to, a0 + 2, b0 + 2, idesc, 1);
-              tc_mma<FMT>(to, a0 + 4, b0 + 4, idesc, 1);
-              tc_mma<FMT>(to, a0 + 6, b0 + 6, idesc, 1);
+              tc_mma<FMT, CG>(to, a0, b0, idesc, FMT != kFmtE4M3 && (kb != 0 || j != 0));
+              tc_mma<FMT, CG>(to, a0 + 2, b0 + 2, idesc, 1);
+              tc_mma<FMT, CG>(to, a0 + 4, b0 + 4, idesc, 1);
+              tc_mma<FMT, CG>(to, a0 + 6, b0 + 6, idesc, 1);
             }
-            tc_commit(empty + ring.at * 8);
-            if (closes) tc_commit(acc_full + acc.at * 8);
+            tc_commit<CG>(empty + ring.at * 8);
+            if (closes) tc_commit<CG>(acc_full + acc.at * 8);
           }
           __syncwarp();
           ring.next(stages);
@@ -519,8 +564,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int e = 0;
       Ring ring;
       for (int t = worker; t < total && ok; t += workers) {
-        const Tile tile = find_tile(list, t, tiles_n, BN, e);
-        const int row0 = tile.m0 + lane;
+        const Tile tile = find_tile(list, t, kGemmRows * CG, tiles_n, BN, e);
+        const int row0 = tile.m0 + rank * kGemmRows + lane;
         const float* sw = a.w_scales + static_cast<int64_t>(tile.expert) * NBLK * KB;
         const int blk0 = min(tile.n0 / kFp8Block, NBLK - 1), blk1 = min((tile.n0 + BN / 2) / kFp8Block, NBLK - 1);
         for (int kb = 0; kb < KB; kb += kScaleBlocks) {
@@ -558,6 +603,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* out_s = smem + L.out_off + (warp - kEpiWarp0) * 2 * kStageOut;
     int turn_out = 0;
 
+    const uint32_t acc_empty0 = CG == 2 ? mapa_shared(acc_empty, 0) : acc_empty;
+    const auto hand_back = [&](int group) {
+      if (CG == 2) arrive_cluster(acc_empty0 + group * 8);
+      else arrive(acc_empty0 + group * 8);
+    };
+
     // rows of no expert are zeros
     if (a.out != kOutCodes) {
       const int size = a.out == kOutF32 ? 4 : 2;
@@ -573,10 +624,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     int e = 0;
     Ring ring, scales;
     for (int t = worker; t < total && ok; t += workers) {
-      const Tile tile = find_tile(list, t, tiles_n, BN, e);
-      const int64_t row = tile.m0 + local;
+      const Tile tile = find_tile(list, t, kGemmRows * CG, tiles_n, BN, e);
+      const int64_t row = tile.m0 + rank * kGemmRows + local;
       const bool live = row < tile.end;
-      const int row_w = tile.m0 + quarter * 32;  // the warp's first row
+      const int row_w = tile.m0 + rank * kGemmRows + quarter * 32;  // the warp's first row
       const bool idle = row_w >= tile.end;  // a warp without rows only hands buffers back
       const int n0 = tile.n0 + half * W;
       float acc[FMT == kFmtE4M3 ? W : 1];
@@ -604,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             const uint32_t src = lane_base + static_cast<uint32_t>(ring.at * kGroupCols);
             if (idle) {
-              if (lane == 0) arrive(acc_empty + ring.at * 8);
+              if (lane == 0) hand_back(ring.at);
               ring.next(kGroups);
               continue;
             }
@@ -627,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               } else {
                 // all read: the group goes back before the last sums
                 tc_fence_before();
-                if (lane == 0) arrive(acc_empty + ring.at * 8);
+                if (lane == 0) hand_back(ring.at);
               }
               if (g == 0 || i + g < blocks) {
                 const uint32_t(&v)[32] = r[t & 1];
@@ -668,7 +719,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (c + 32 >= W) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) arrive(acc_empty + ring.at * 8);
+            if (lane == 0) hand_back(ring.at);
           }
         }
       };
@@ -695,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
       if (idle || n0 >= a.N) {
         if constexpr (FMT != kFmtE4M3) {
-          if (lane == 0) arrive(acc_empty + ring.at * 8);
+          if (lane == 0) hand_back(ring.at);
           ring.next(kGroups);
         }
         continue;
@@ -790,75 +841,85 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (CG == 2) cluster_sync_all();  // neither CTA ends while the other signals its barriers
   if (warp == 2) {
     tc_fence_after();
-    tmem_release(tmem, kTmemCols);
+    tmem_release<CG>(tmem, kTmemCols);
   }
 }
 
-template <int FMT, int DT, int BN>
+template <int FMT, int DT, int CG, int BN>
 cudaError_t launch_typed(const ExpertGemmMaps& m, const ExpertGemmArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
-  auto kernel = expert_gemm_kernel<FMT, DT, BN>;
+  auto kernel = expert_gemm_kernel<FMT, DT, CG, BN>;
   static SharedMemoryOptIn opt_in;
   const cudaError_t configured = opt_in.ensure(reinterpret_cast<const void*>(kernel), kSmemLimit - 1024);
   if (configured != cudaSuccess) return configured;
-  const SmemPlan p = plan_smem(FMT == kFmtE4M3, BN, a.experts);
-  // no more CTAs than tiles there can be
+  const SmemPlan p = plan_smem(FMT == kFmtE4M3, BN, CG, a.experts);
+  // no more CTAs (or pairs) than tiles there can be
   const int64_t groups = a.offsets == nullptr ? 1 : std::min(a.experts, a.rows);
-  const int64_t tiles = ((a.rows + kGemmRows - 1) / kGemmRows + groups) * ((a.N + BN - 1) / BN);
-  const int ctas = static_cast<int>(std::min<int64_t>(tiles, num_sms));
-  return launch(kernel, dim3(ctas), dim3(kThreads), p.bytes, stream, pdl, m.x, m.x_part, m.w, m.y, a);
+  const int64_t tiles = ((a.rows + kGemmRows * CG - 1) / (kGemmRows * CG) + groups) * ((a.N + BN - 1) / BN);
+  const int ctas = static_cast<int>(std::min<int64_t>(tiles, num_sms / CG));
+  return launch_clustered(kernel, dim3(ctas * CG), dim3(kThreads), p.bytes, stream, pdl, CG, m.x, m.x_part, m.w, m.y, a);
 }
 
 template <int FMT, int DT>
-cudaError_t launch_width(int bn, const ExpertGemmMaps& m, const ExpertGemmArgs& a, int num_sms, cudaStream_t stream,
-                         bool pdl) {
-  if (bn == 256) return launch_typed<FMT, DT, 256>(m, a, num_sms, stream, pdl);
-  if (bn == 128) return launch_typed<FMT, DT, 128>(m, a, num_sms, stream, pdl);
-  return launch_typed<FMT, DT, 64>(m, a, num_sms, stream, pdl);
+cudaError_t launch_cut(const ExpertGemmCut& cut, const ExpertGemmMaps& m, const ExpertGemmArgs& a, int num_sms,
+                       cudaStream_t stream, bool pdl) {
+  if (cut.pair == 2) return launch_typed<FMT, DT, 2, 256>(m, a, num_sms, stream, pdl);
+  if (cut.bn == 256) return launch_typed<FMT, DT, 1, 256>(m, a, num_sms, stream, pdl);
+  if (cut.bn == 128) return launch_typed<FMT, DT, 1, 128>(m, a, num_sms, stream, pdl);
+  return launch_typed<FMT, DT, 1, 64>(m, a, num_sms, stream, pdl);
 }
 
 }  // namespace
 
-cudaError_t launch_expert_gemm(int dtype, bool e4m3, int bn, const ExpertGemmMaps& maps, const ExpertGemmArgs& a,
-                               int num_sms, cudaStream_t stream, bool pdl) {
-  if ((bn != 64 && bn != 128 && bn != 256) || (a.out == kOutCodes && bn != 256)) return cudaErrorInvalidValue;
+cudaError_t launch_expert_gemm(int dtype, bool e4m3, const ExpertGemmCut& cut, const ExpertGemmMaps& maps,
+                               const ExpertGemmArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
+  if (cut.bn != 64 && cut.bn != 128 && cut.bn != 256) return cudaErrorInvalidValue;
+  if ((cut.pair == 2 || a.out == kOutCodes) && cut.bn != 256) return cudaErrorInvalidValue;
   if (e4m3)
-    return dtype == kF16 ? launch_width<kFmtE4M3, kF16>(bn, maps, a, num_sms, stream, pdl)
-                         : launch_width<kFmtE4M3, kBF16>(bn, maps, a, num_sms, stream, pdl);
-  return dtype == kF16 ? launch_width<kFmtF16, kF16>(bn, maps, a, num_sms, stream, pdl)
-                       : launch_width<kFmtBF16, kBF16>(bn, maps, a, num_sms, stream, pdl);
+    return dtype == kF16 ? launch_cut<kFmtE4M3, kF16>(cut, maps, a, num_sms, stream, pdl)
+                         : launch_cut<kFmtE4M3, kBF16>(cut, maps, a, num_sms, stream, pdl);
+  return dtype == kF16 ? launch_cut<kFmtF16, kF16>(cut, maps, a, num_sms, stream, pdl)
+                       : launch_cut<kFmtBF16, kBF16>(cut, maps, a, num_sms, stream, pdl);
 }
 
-int plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, int num_sms) {
-  // The width with the least estimated time: waves of tiles, each of its k
-  // blocks' time and a tile's own.  A k block takes the longer of what the
-  // products and the epilogue need and of its weights' share of the memory's
-  // rate (which the tiles of one group share: the second finds them in L2).
-  // Cycles, fitted to measured calls: 8 to 16384 rows, 1 to 64 experts, n and k
-  // 512 to 4096.
+ExpertGemmCut plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, bool codes_out, int num_sms) {
+  // The cut with the least estimated time: waves of tiles, each of its k
+  // blocks' time and a tile's own.  A k block takes the longest of what the
+  // products and the epilogue need, its copies from L2 at the rate that all SMs
+  // have together, and its weights' share of the memory's rate (which the tiles
+  // of one group share: the second finds them in L2).  Cycles, fitted to
+  // measured calls: 8 to 16384 rows, 1 to 64 experts, n and k 512 to 4096.
   struct Cut {
-    int bn;
+    int pair, bn;
     double block_e4m3, block_16, tile_e4m3, tile_16;
   };
-  static constexpr Cut kCuts[] = {{64, 250, 200, 3500, 2500}, {128, 400, 350, 4500, 3000}, {256, 700, 650, 7000, 2500}};
-  constexpr double kBytesPerCycle = 24.0;  // one SM's share of the memory's rate
+  static constexpr Cut kCuts[] = {{1, 64, 250, 200, 3500, 2500},
+                                  {1, 128, 400, 350, 4500, 3000},
+                                  {1, 256, 800, 650, 6000, 2500},
+                                  {2, 256, 850, 650, 6000, 2500}};
+  constexpr double kMemoryBytes = 24.0, kL2Bytes = 43.0;  // a cycle and SM
   const int KB = (K + (e4m3 ? 127 : 63)) / (e4m3 ? 128 : 64);
   // experts that have rows, were the choice of expert even
   const double groups = experts * (1.0 - std::pow(1.0 - 1.0 / experts, rows)), mean = rows / groups;
-  // ragged groups have half a tile more than their mean size
-  double per_group = std::ceil(mean / kGemmRows);
-  if (experts > 1 && mean > kGemmRows / 2) per_group = mean / kGemmRows + 0.5;
-  int best = 0;
+  ExpertGemmCut best{1, 256};
   double least = 0.0;
   for (const Cut& c : kCuts) {
-    const double tiles = groups * per_group * ((N + c.bn - 1) / c.bn), busy = std::min(1.0, tiles / num_sms);
-    const double memory = c.bn * static_cast<double>(kRowBytes) / kBytesPerCycle * busy / per_group;
-    const double block = std::max(e4m3 ? c.block_e4m3 : c.block_16, memory);
-    const double time = std::ceil(tiles / num_sms) * (KB * block + (e4m3 ? c.tile_e4m3 : c.tile_16));
-    if (best == 0 || time < least) {
+    if (codes_out && c.bn != 256) continue;
+    const double tile_rows = kGemmRows * c.pair, workers = num_sms / c.pair;
+    // ragged groups have half a tile more than their mean size
+    double per_group = std::ceil(mean / tile_rows);
+    if (experts > 1 && mean > tile_rows / 2) per_group = mean / tile_rows + 0.5;
+    const double tiles = groups * per_group * ((N + c.bn - 1) / c.bn), busy = std::min(1.0, tiles / workers);
+    const double weights = static_cast<double>(c.bn / c.pair) * kRowBytes;
+    const double x = std::min(mean / c.pair, static_cast<double>(kGemmRows)) * kRowBytes;
+    const double block = std::max({e4m3 ? c.block_e4m3 : c.block_16, weights / kMemoryBytes * busy / per_group,
+                                   (weights + x) / kL2Bytes * busy});
+    const double time = std::ceil(tiles / workers) * (KB * block + (e4m3 ? c.tile_e4m3 : c.tile_16));
+    if (least == 0.0 || time < least) {
       least = time;
-      best = c.bn;
+      best = {c.pair, c.bn};
     }
   }
   return best;
