@@ -698,18 +698,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
 
-      // The rest of a tile runs once for thousands of cycles of products, so
-      // its loops over 32 columns are kept rolled: unrolled, their code alone
-      // overflowed the instruction caches (a tile of three rows took 11,000
-      // cycles).  Registers cannot be indexed, so e4m3 sums move down by 32
-      // after each turn; 16-bit sums are read from tensor memory turn by turn.
       const uint32_t src = lane_base + static_cast<uint32_t>(ring.at * kGroupCols);
       const auto take = [&](int c, float(&v)[32]) {
         if constexpr (FMT == kFmtE4M3) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = acc[j];
-#pragma unroll
-          for (int j = 0; j + 32 < W; ++j) acc[j] = acc[j + 32];
+          for (int j = 0; j < 32; ++j) v[j] = acc[c + j];
         } else {
           uint32_t r[32];
           tmem_ld32(src + c, r);
@@ -755,8 +748,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (a.out == kOutCodes) {
           // the thread's 128 columns are one block of its row: its largest
           // magnitude, then its codes; rows of codes are padded to whole blocks
-          uint32_t top = 0;
-#pragma unroll 1
+          float most = 0.0f;
+#pragma unroll
           for (int c = 0; c < W; c += 32) {
             float v[32];
             take(c, v);
@@ -767,12 +760,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-              top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-              acc[W - 32 + j] = v[j];
+              most = fmaxf(most, fabsf(v[j]));
+              acc[c + j] = v[j];
             }
           }
+          uint32_t top = __float_as_uint(most);
           if (top >= 0x7F800000u) {
-            // not all finite: the scale comes from those that are, the others become NaN
+            // infinities: the scale comes from the finite values, the others
+            // become NaN (a NaN is not in the maximum, and converts to one)
             top = 0;
 #pragma unroll
             for (int i = 0; i < W; ++i) {
@@ -784,15 +779,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int ex = fp8_scale_exponent(top);
           const float inv = pow2f(-ex);
           if (live) a.y_scales[static_cast<int64_t>(n0 / kFp8Block) * a.rows + row] = pow2f(ex);
-#pragma unroll 1
+#pragma unroll
           for (int h = 0; h < W; h += 64) {
             uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              w[i] = e4m3x2_finite(acc[4 * i] * inv, acc[4 * i + 1] * inv) |
-                     (e4m3x2_finite(acc[4 * i + 2] * inv, acc[4 * i + 3] * inv) << 16);
-#pragma unroll
-            for (int i = 0; i < W - 64; ++i) acc[i] = acc[i + 64];
+            for (int i = 0; i < 16; ++i) {
+              const float* v = acc + h + 4 * i;
+              w[i] = e4m3x2_finite(v[0] * inv, v[1] * inv) | (e4m3x2_finite(v[2] * inv, v[3] * inv) << 16);
+            }
             if (whole) {
               store_piece(out_s, turn_out, lane, w, &ymap, n0 + h, row_w);
             } else if (live) {
@@ -802,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           continue;
         }
       }
-#pragma unroll 1
+#pragma unroll
       for (int c = 0; c < W; c += 32) {
         float v[32];
         take(c, v);
