@@ -25,7 +25,8 @@
 //   warp 1      issues tcgen05.mma
 //               (warp 2 also owns the tensor memory)
 //   warp 3      e4m3: fetches the scales, eight k blocks ahead
-//   warps 4-11  epilogue: two groups of four warps, each half of the columns
+//   warps 4-    epilogue: one set of eight warps or two, in a set two groups of
+//               four warps, each half of the columns
 #include "expert_gemm.hpp"
 
 #include <algorithm>
@@ -38,8 +39,13 @@ namespace cq {
 
 namespace {
 
-constexpr int kThreads = 384;
-constexpr int kEpiWarp0 = 4, kEpiWarps = 8, kEpiThreads = kEpiWarps * 32;
+constexpr int kEpiWarp0 = 4, kSetWarps = 8;
+// Sets of eight epilogue warps.  Narrow tiles have two that take turns, so that
+// one set's last pass over a tile (activation, rounding or codes, stores) runs
+// beside the other's sums of the next tile: with one set that pass took as long
+// as the copies of a whole tile.
+__host__ __device__ constexpr int epi_sets(int bn) { return bn < 256 ? 2 : 1; }
+__host__ __device__ constexpr int gemm_threads(int bn) { return (kEpiWarp0 + kSetWarps * epi_sets(bn)) * 32; }
 constexpr int kRowBytes = 128;                       // a k block of one row
 constexpr int kXBytes = kGemmRows * kRowBytes;       // a stage's rows of x
 constexpr int kMaxStages = 8;
@@ -53,11 +59,14 @@ enum Format : int { kFmtE4M3 = 0, kFmtF16 = 1, kFmtBF16 = 2 };
 constexpr int kScaleBlocks = 8;  // k blocks of scales fetched at a time
 constexpr int kScaleSlots = 2;
 constexpr int kScaleBytes = kScaleBlocks * (kGemmRows + 2) * 4;
-constexpr int kStageOut = kStoreRows * kStoreBytes;  // one of a warp's two tile stores
+constexpr int kStageOut = kStoreRows * kStoreBytes;  // a warp's tile store
+constexpr int kStageOuts = 16;                        // two for each of one set's warps, one for each of two sets'
 
 // k blocks of one stage: two where a block's products are so short that the
 // waits and signals of a stage would outlast them.
 __host__ __device__ constexpr int stage_blocks(int bn) { return bn < 256 ? 2 : 1; }
+
+constexpr int kStaticBytes = 1024 + 4096;  // the bias, and the largest magnitudes of a block's halves
 
 struct SmemPlan {
   int stage_bytes, stages, out_off, scale_off, list_off, bar_off, bytes;
@@ -67,13 +76,13 @@ __host__ __device__ inline SmemPlan plan_smem(bool e4m3, int bn, int pair, int e
   SmemPlan p{};
   p.stage_bytes = stage_blocks(bn) * (kXBytes + bn / pair * kRowBytes);
   const int list = (2 * (experts + 2) * 4 + 15) / 16 * 16;
-  const int bars = (2 * kMaxStages + 2 * kGroups + 2 * kScaleSlots) * 8 + 16;
+  const int bars = (2 * kMaxStages + 2 * kGroups + 2 * kScaleSlots + 2) * 8 + 16;
   const int scales = e4m3 ? kScaleSlots * kScaleBytes : 0;
-  const int rest = kEpiWarps * 2 * kStageOut + scales + list + bars;
-  p.stages = (kSmemLimit - 2048 - rest) / p.stage_bytes;  // 2048: alignment, and the bias
+  const int rest = kStageOuts * kStageOut + scales + list + bars;
+  p.stages = (kSmemLimit - kStaticBytes - 1024 - rest) / p.stage_bytes;  // 1024: alignment
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   p.out_off = p.stages * p.stage_bytes;
-  p.scale_off = p.out_off + kEpiWarps * 2 * kStageOut;
+  p.scale_off = p.out_off + kStageOuts * kStageOut;
   p.list_off = p.scale_off + scales;
   p.bar_off = p.list_off + list;
   p.bytes = p.bar_off + bars + 1024;  // + alignment
@@ -125,8 +134,8 @@ __device__ __forceinline__ void tc_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// 32 lanes x 32 columns: thread i of the warp gets its lane's 32 columns.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+// 32 lanes x 32 (or 16) columns: thread i of the warp gets its lane's columns.
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
       "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -134,6 +143,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
 }
@@ -145,6 +162,14 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
                "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
                "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
                "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                :
                : "memory");
 }
@@ -289,6 +314,9 @@ struct Tile {
 struct Ring {
   int at = 0;
   uint32_t phase = 0;
+  Ring() = default;
+  // after `used` places
+  __device__ __forceinline__ Ring(int used, int size) : at(used % size), phase((used / size) & 1) {}
   __device__ __forceinline__ void next(int size) {
     if (++at == size) {
       at = 0;
@@ -320,13 +348,18 @@ __device__ __forceinline__ void store32(void* p, const uint32_t* w) {
 // 64 bytes of each of a warp's 32 rows: through the warp's shared memory
 // (16-byte pieces in the 64-byte swizzle, free of bank conflicts) to one tile
 // store.  Whole sectors leave the SM in few requests; a store by each lane to
-// its own row touches 32 lines an instruction.  Two buffers take turns, so that
-// a piece waits for the one before the last.
+// its own row touches 32 lines an instruction.  Where there are two buffers they
+// take turns, and a piece waits for the one before the last.
+template <int BUFFERS>
 __device__ __forceinline__ void store_piece(uint8_t* out_s, int& turn, int lane, const uint32_t* w,
                                             const CUtensorMap* ymap, int n, int row) {
   uint8_t* buf = out_s + turn * kStageOut;
-  turn ^= 1;
-  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+  if constexpr (BUFFERS == 2) {
+    turn ^= 1;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+  } else {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  }
   __syncwarp();
 #pragma unroll
   for (int p = 0; p < 4; ++p)
@@ -385,16 +418,22 @@ __device__ __forceinline__ void store_piece_by_rows(uint8_t* buf, int lane, cons
   __syncwarp();
 }
 
-// The four warps of an epilogue group.
-__device__ __forceinline__ void group_sync(int half) {
-  if (half == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
-  else asm volatile("bar.sync 2, 128;" ::: "memory");
+// The four warps of an epilogue group, and the eight of a set.
+__device__ __forceinline__ void group_sync(int group) {
+  if (group == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+  else if (group == 1) asm volatile("bar.sync 2, 128;" ::: "memory");
+  else if (group == 2) asm volatile("bar.sync 3, 128;" ::: "memory");
+  else asm volatile("bar.sync 4, 128;" ::: "memory");
+}
+__device__ __forceinline__ void set_sync(int set) {
+  if (set == 0) asm volatile("bar.sync 5, 256;" ::: "memory");
+  else asm volatile("bar.sync 6, 256;" ::: "memory");
 }
 
 // --------------------------------------------------------------- kernel
 
 template <int FMT, int DT, int CG, int BN>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(gemm_threads(BN), 1)
     expert_gemm_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap xmap_part,
                        const __grid_constant__ CUtensorMap wmap,
                        const __grid_constant__ CUtensorMap ymap, const ExpertGemmArgs a) {
@@ -405,6 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Tensor memory is two groups of accumulators that go back and forth between
   // the products and the epilogue: of kPer k blocks' partial sums each (e4m3),
   // or of one tile's sums.
+  constexpr int kSets = epi_sets(BN), kEpiThreads = kSets * kSetWarps * 32;
   constexpr int kStageBlocks = stage_blocks(BN);
   constexpr int kPer = FMT == kFmtE4M3 ? static_cast<int>(kTmemCols) / kGroups / BN : 1;
   static_assert(FMT != kFmtE4M3 || kPer % kStageBlocks == 0, "a stage's blocks are of one group");
@@ -413,12 +453,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t full = smem_u32(bars), empty = full + kMaxStages * 8;
   const uint32_t acc_full = empty + kMaxStages * 8, acc_empty = acc_full + kGroups * 8;
   const uint32_t scale_full = acc_empty + kGroups * 8, scale_empty = scale_full + kScaleSlots * 8;
-  constexpr int kBarriers = 2 * kMaxStages + 2 * kGroups + 2 * kScaleSlots;
+  const uint32_t token = scale_empty + kScaleSlots * 8;
+  constexpr int kBarriers = 2 * kMaxStages + 2 * kGroups + 2 * kScaleSlots + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBarriers);
   // [slot][k block][row], then [slot][k block][column half]
   float* scale_x = reinterpret_cast<float*>(smem + L.scale_off);
   float* scale_w = scale_x + kScaleSlots * kScaleBlocks * kGemmRows;
-  __shared__ __align__(16) float bias_s[256];
+  __shared__ __align__(16) float bias_s[256];  // [set][column]
+  __shared__ uint32_t top_s[2][4][kSets == 2 && BN >= kFp8Block && FMT == kFmtE4M3 ? kGemmRows : 1];  // [tile's parity][group][row]
 
   // the same in all lanes, and known to be
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -433,13 +475,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tensormap(&xmap_part);
     prefetch_tensormap(&wmap);
     prefetch_tensormap(&ymap);
-    for (int i = 0; i < kBarriers; ++i) {
-      // full: the two copying warps; acc_empty, scale_empty: the epilogue's
-      // warps; scale_full: the lanes of the scale warp
-      const bool is_full = i < kMaxStages, is_scale = i >= kBarriers - 2 * kScaleSlots;
-      const bool by_epilogue = i >= kBarriers - kScaleSlots || (!is_scale && i >= 2 * kMaxStages + kGroups);
-      mbar_init(bars + i, is_full ? 2 : by_epilogue ? (is_scale ? kEpiWarps : CG * kEpiWarps) : is_scale ? 32 : 1);
-    }
+    // arrivals: full by the two copying warps, acc_empty, scale_empty and token
+    // by a set's warps, scale_full by the lanes of the scale warp
+    uint64_t* b = bars;
+    const auto init = [&](int count, int arrivals) {
+      for (int i = 0; i < count; ++i) mbar_init(b++, arrivals);
+    };
+    init(kMaxStages, 2);
+    init(kMaxStages, 1);
+    init(kGroups, 1);
+    init(kGroups, CG * kSetWarps);
+    init(kScaleSlots, 32);
+    init(kScaleSlots, kSetWarps);
+    init(2, kSetWarps);
     fence_mbar_init();
   }
   if (warp == 2) tmem_alloc<CG>(tmem_slot, kTmemCols);
@@ -460,7 +508,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool ok = true;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if constexpr (kSets == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");  // of 640 threads of 96
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");                       // of 384 threads of 168
     if (warp == 0 || warp == 2) {
       // ---------------------------------------------------------- copies
       // warp 0: rows of x, only those that there are, by 32 (a small group's
@@ -593,15 +642,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if constexpr (kSets == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ------------------------------------------------------------ epilogue
     pdl_wait();
-    const int quarter = warp & 3, half = (warp - kEpiWarp0) >> 2;
+    const int quarter = warp & 3, half = ((warp - kEpiWarp0) >> 2) & 1, set = (warp - kEpiWarp0) / kSetWarps;
     constexpr int W = BN / 2;  // columns of this warp group
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(half * W);
     const int local = quarter * 32 + lane;  // row of the tile's 128
-    uint8_t* out_s = smem + L.out_off + (warp - kEpiWarp0) * 2 * kStageOut;
-    int turn_out = 0;
+    constexpr int kOuts = kStageOuts / (kSets * kSetWarps);
+    uint8_t* out_s = smem + L.out_off + (warp - kEpiWarp0) * kOuts * kStageOut;
+    int turn_out = 0, turn = 0;
+    const int tile_groups = FMT == kFmtE4M3 ? (KB + kPer - 1) / kPer : 1;  // of accumulators, per tile
+    const int tile_slots = (KB + kScaleBlocks - 1) / kScaleBlocks;         // of scales, per tile
 
     const uint32_t acc_empty0 = CG == 2 ? mapa_shared(acc_empty, 0) : acc_empty;
     const auto hand_back = [&](int group) {
@@ -622,9 +675,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 
     int e = 0;
-    Ring ring, scales;
-    for (int t = worker; t < total && ok; t += workers) {
+    for (int t = worker + set * workers, seq = set; t < total && ok; t += kSets * workers, seq += kSets) {
       const Tile tile = find_tile(list, t, kGemmRows * CG, tiles_n, BN, e);
+      Ring ring(seq * tile_groups, kGroups), scales(seq * tile_slots, kScaleSlots);
+      // The sets' sums follow one another: a set that waited for its accumulators
+      // while the other's are still to come would take a phase of theirs, of the
+      // same parity, for its own.
+      if (kSets == 2 && seq > 0) ok = wait_phase(token + set * 8, ((seq - 1) / 2) & 1, a.status);
       const int64_t row = tile.m0 + rank * kGemmRows + local;
       const bool live = row < tile.end;
       const int row_w = tile.m0 + rank * kGemmRows + quarter * 32;  // the warp's first row
@@ -635,12 +692,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < (FMT == kFmtE4M3 ? W : 1); ++i) acc[i] = 0.0f;
       if (a.bias != nullptr) {
         // the group's columns of the bias, one a thread
-        group_sync(half);  // the tile before has been read
+        group_sync(set * 2 + half);  // the tile before has been read
         if (local < W) {
           const int n = n0 + local;
-          bias_s[half * 128 + local] = n < a.N ? ld_t<DT>(a.bias, static_cast<int64_t>(tile.expert) * a.N + n) : 0.0f;
+          bias_s[set * BN + half * W + local] = n < a.N ? ld_t<DT>(a.bias, static_cast<int64_t>(tile.expert) * a.N + n) : 0.0f;
         }
-        group_sync(half);
+        group_sync(set * 2 + half);
       }
 
       if constexpr (FMT == kFmtE4M3) {
@@ -659,31 +716,33 @@ __global__ void __launch_bounds__(kThreads, 1)
               ring.next(kGroups);
               continue;
             }
-            // 32 columns at a time over the group's blocks, the next on their
+            // some columns at a time over the group's blocks, the next on their
             // way while these are added; a block past the end of k holds an
             // old group's sums and is left out
             float scale[kPer];
 #pragma unroll
             for (int g = 0; g < kPer; ++g) scale[g] = i + g < blocks ? sx[(i + g) * kGemmRows] * sw[2 * (i + g)] : 0.0f;
-            constexpr int kSteps = kPer * W / 32;
-            uint32_t r[2][32];
-            tmem_ld32(src, r[0]);
+            constexpr int kCols = kSets == 2 ? 16 : 32;  // what the registers hold of it
+            constexpr int kRun = W / kCols, kSteps = kPer * kRun;
+            constexpr int kDeep = kSets == 2 ? 1 : 2;   // loads in flight (two sets' warps hide each other's)
+            uint32_t r[kDeep][kCols];
+            if (kDeep == 2) tmem_ld(src, r[0]);
 #pragma unroll
             for (int t = 0; t < kSteps; ++t) {
-              constexpr int kRun = W / 32;
-              const int g = t / kRun, c = t % kRun * 32;
-              tmem_wait_ld(r[t & 1]);
-              if (t + 1 < kSteps) {
-                tmem_ld32(src + (t + 1) / kRun * BN + (t + 1) % kRun * 32, r[(t + 1) & 1]);
-              } else {
+              const int g = t / kRun, c = t % kRun * kCols;
+              if (kDeep == 1) tmem_ld(src + g * BN + c, r[0]);
+              tmem_wait_ld(r[t % kDeep]);
+              if (t + 1 == kSteps) {
                 // all read: the group goes back before the last sums
                 tc_fence_before();
                 if (lane == 0) hand_back(ring.at);
+              } else if (kDeep == 2) {
+                tmem_ld(src + (t + 1) / kRun * BN + (t + 1) % kRun * kCols, r[(t + 1) % kDeep]);
               }
               if (g == 0 || i + g < blocks) {
-                const uint32_t(&v)[32] = r[t & 1];
+                const uint32_t(&v)[kCols] = r[t % kDeep];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) acc[c + j] = fmaf(__uint_as_float(v[j]), scale[g], acc[c + j]);
+                for (int j = 0; j < kCols; ++j) acc[c + j] = fmaf(__uint_as_float(v[j]), scale[g], acc[c + j]);
               }
             }
             ring.next(kGroups);
@@ -697,6 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
       }
       if (!ok) break;
+      if (kSets == 2 && lane == 0) arrive(token + (set ^ 1) * 8);
 
       const uint32_t src = lane_base + static_cast<uint32_t>(ring.at * kGroupCols);
       const auto take = [&](int c, float(&v)[32]) {
@@ -705,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 32; ++j) v[j] = acc[c + j];
         } else {
           uint32_t r[32];
-          tmem_ld32(src + c, r);
+          tmem_ld(src + c, r);
           tmem_wait_ld(r);
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
@@ -718,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       const auto finish = [&](int c, float(&v)[32]) {
         if (a.bias != nullptr) {
-          const float4* b4 = reinterpret_cast<const float4*>(bias_s + half * 128 + c);
+          const float4* b4 = reinterpret_cast<const float4*>(bias_s + set * BN + half * W + c);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float4 b = b4[j];
@@ -737,48 +797,50 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int rows_w = min(32, tile.end - row_w);
       const bool whole = a.tile_store && rows_w == 32;
 
-      if (idle || n0 >= a.N) {
-        if constexpr (FMT != kFmtE4M3) {
-          if (lane == 0) hand_back(ring.at);
-          ring.next(kGroups);
-        }
-        continue;
-      }
-      if constexpr (BN == 256 && FMT == kFmtE4M3) {
+      if constexpr (BN >= kFp8Block && FMT == kFmtE4M3) {
         if (a.out == kOutCodes) {
-          // the thread's 128 columns are one block of its row: its largest
-          // magnitude, then its codes; rows of codes are padded to whole blocks
-          float most = 0.0f;
+          // a row's block of 128 columns is one thread's, or two threads' halves:
+          // its largest finite magnitude, then the codes (infinities made NaN)
+          uint32_t top = 0;
+          if (!idle && n0 < a.N) {
+            float most = 0.0f;
 #pragma unroll
-          for (int c = 0; c < W; c += 32) {
-            float v[32];
-            take(c, v);
-            finish(c, v);
-            if (n0 + c + 32 > a.N) {
+            for (int c = 0; c < W; c += 32) {
+              float v[32];
+              take(c, v);
+              finish(c, v);
+              if (n0 + c + 32 > a.N) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = n0 + c + j < a.N ? v[j] : 0.0f;
+                for (int j = 0; j < 32; ++j) v[j] = n0 + c + j < a.N ? v[j] : 0.0f;
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                most = fmaxf(most, fabsf(v[j]));
+                acc[c + j] = v[j];
+              }
             }
+            top = __float_as_uint(most);
+            if (top >= 0x7F800000u) {
+              // (a NaN is not in the maximum, and converts to one)
+              top = 0;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              most = fmaxf(most, fabsf(v[j]));
-              acc[c + j] = v[j];
+              for (int i = 0; i < W; ++i) {
+                const uint32_t m = finite_magnitude(acc[i]);
+                top = max(top, m);
+                if (m == 0 && acc[i] != 0.0f) acc[i] = __uint_as_float(0x7FC00000u);
+              }
             }
           }
-          uint32_t top = __float_as_uint(most);
-          if (top >= 0x7F800000u) {
-            // infinities: the scale comes from the finite values, the others
-            // become NaN (a NaN is not in the maximum, and converts to one)
-            top = 0;
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-              const uint32_t m = finite_magnitude(acc[i]);
-              top = max(top, m);
-              if (m == 0 && acc[i] != 0.0f) acc[i] = __uint_as_float(0x7FC00000u);
-            }
+          if constexpr (W < kFp8Block) {
+            top_s[turn][set * 2 + half][local] = top;
+            set_sync(set);
+            top = max(top, top_s[turn][set * 2 + (half ^ 1)][local]);
+            turn ^= 1;
           }
+          if (idle || n0 >= a.N) continue;
           const int ex = fp8_scale_exponent(top);
           const float inv = pow2f(-ex);
-          if (live) a.y_scales[static_cast<int64_t>(n0 / kFp8Block) * a.rows + row] = pow2f(ex);
+          if (live && n0 % kFp8Block == 0) a.y_scales[static_cast<int64_t>(n0 / kFp8Block) * a.rows + row] = pow2f(ex);
 #pragma unroll
           for (int h = 0; h < W; h += 64) {
             uint32_t w[16];
@@ -788,13 +850,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               w[i] = e4m3x2_finite(v[0] * inv, v[1] * inv) | (e4m3x2_finite(v[2] * inv, v[3] * inv) << 16);
             }
             if (whole) {
-              store_piece(out_s, turn_out, lane, w, &ymap, n0 + h, row_w);
+              store_piece<kOuts>(out_s, turn_out, lane, w, &ymap, n0 + h, row_w);
             } else if (live) {
               store_piece_by_lanes(w, reinterpret_cast<uint8_t*>(a.y) + row * a.ldy + n0 + h);
             }
           }
           continue;
         }
+      }
+      if (idle || n0 >= a.N) {
+        if constexpr (FMT != kFmtE4M3) {
+          if (lane == 0) hand_back(ring.at);
+        }
+        continue;
       }
 #pragma unroll
       for (int c = 0; c < W; c += 32) {
@@ -817,7 +885,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 16; ++i) w[i] = pack_t<DT>(v[2 * i], v[2 * i + 1]);
           }
           if (whole) {
-            store_piece(out_s, turn_out, lane, w, &ymap, n, row_w);
+            store_piece<kOuts>(out_s, turn_out, lane, w, &ymap, n, row_w);
           } else if (a.tile_store && n + kStoreBytes / size <= a.N) {
             if (live) store_piece_by_lanes(w, reinterpret_cast<uint8_t*>(a.y) + (row * a.ldy + n) * size);
           } else {
@@ -826,7 +894,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (FMT != kFmtE4M3) ring.next(kGroups);
     }
     // the tile stores have read their shared memory
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -846,14 +913,14 @@ template <int FMT, int DT, int CG, int BN>
 cudaError_t launch_typed(const ExpertGemmMaps& m, const ExpertGemmArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
   auto kernel = expert_gemm_kernel<FMT, DT, CG, BN>;
   static SharedMemoryOptIn opt_in;
-  const cudaError_t configured = opt_in.ensure(reinterpret_cast<const void*>(kernel), kSmemLimit - 1024);
+  const cudaError_t configured = opt_in.ensure(reinterpret_cast<const void*>(kernel), kSmemLimit - kStaticBytes);
   if (configured != cudaSuccess) return configured;
   const SmemPlan p = plan_smem(FMT == kFmtE4M3, BN, CG, a.experts);
   // no more CTAs (or pairs) than tiles there can be
   const int64_t groups = a.offsets == nullptr ? 1 : std::min(a.experts, a.rows);
   const int64_t tiles = ((a.rows + kGemmRows * CG - 1) / (kGemmRows * CG) + groups) * ((a.N + BN - 1) / BN);
   const int ctas = static_cast<int>(std::min<int64_t>(tiles, num_sms / CG));
-  return launch_clustered(kernel, dim3(ctas * CG), dim3(kThreads), p.bytes, stream, pdl, CG, m.x, m.x_part, m.w, m.y, a);
+  return launch_clustered(kernel, dim3(ctas * CG), dim3(gemm_threads(BN)), p.bytes, stream, pdl, CG, m.x, m.x_part, m.w, m.y, a);
 }
 
 template <int FMT, int DT>
@@ -870,7 +937,7 @@ cudaError_t launch_cut(const ExpertGemmCut& cut, const ExpertGemmMaps& m, const 
 cudaError_t launch_expert_gemm(int dtype, bool e4m3, const ExpertGemmCut& cut, const ExpertGemmMaps& maps,
                                const ExpertGemmArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
   if (cut.bn != 64 && cut.bn != 128 && cut.bn != 256) return cudaErrorInvalidValue;
-  if ((cut.pair == 2 || a.out == kOutCodes) && cut.bn != 256) return cudaErrorInvalidValue;
+  if ((cut.pair == 2 && cut.bn != 256) || (a.out == kOutCodes && cut.bn < kFp8Block)) return cudaErrorInvalidValue;
   if (e4m3)
     return dtype == kF16 ? launch_cut<kFmtE4M3, kF16>(cut, maps, a, num_sms, stream, pdl)
                          : launch_cut<kFmtE4M3, kBF16>(cut, maps, a, num_sms, stream, pdl);
@@ -900,7 +967,7 @@ ExpertGemmCut plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, b
   ExpertGemmCut best{1, 256};
   double least = 0.0;
   for (const Cut& c : kCuts) {
-    if (codes_out && c.bn != 256) continue;
+    if (codes_out && c.bn < kFp8Block) continue;
     const double tile_rows = kGemmRows * c.pair, workers = num_sms / c.pair;
     // ragged groups have half a tile more than their mean size
     double per_group = std::ceil(mean / tile_rows);

@@ -42,7 +42,7 @@ struct ExpertGemmMaps {
 };
 
 // How a call is cut: CTAs to a tile (1 of 128 rows, or a pair of 256) and weight
-// rows of a tile (64, 128 or 256; pairs and codes: 256).
+// rows of a tile (64, 128 or 256; pairs: 256; codes: 128 or 256).
 struct ExpertGemmCut {
   int pair, bn;
 };

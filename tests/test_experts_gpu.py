@@ -264,6 +264,41 @@ def test_expert_linear(cq, weights, name, n, k):
 
 
 @pytest.mark.parametrize("weights", ["16bit", "e4m3"])
+@pytest.mark.parametrize("experts,counts,n,k", [(40, 3, 2048, 1024), (40, 3, 1024, 1400), (24, 70, 1024, 640), (30, 40, 512, 2048),
+                                               (4, 700, 1024, 384), (6, 400, 2048, 512)])
+def test_expert_linear_many_tiles(cq, weights, experts, counts, n, k):
+    """Several tiles a CTA, of every width and pairing: the rings of copies, sums and scales go on from tile to tile."""
+    from nemotron_cuda import experts as ex
+    gen = rng_of(experts, counts, n, k)
+    sizes = [counts + (i * 7) % 5 - 2 for i in range(experts)]
+    x, off = values(gen, sum(sizes), k, spread=0.3), offsets_of(sizes)
+    if weights == "e4m3":
+        codes, scales = codes_of(gen, experts, n, k), scales_of(gen, experts, -(-n // 128), -(-k // 128)) / k ** 0.5
+        layer = ex.ExpertLinear.from_codes(codes, scales)
+        w, x64 = np.stack([weight_values(codes[e], scales[e]) for e in range(experts)]), row_values(x)
+    else:
+        weight = values(gen, experts, n, k, spread=0.2) / k ** 0.5
+        layer = ex.ExpertLinear.from_weight(weight)
+        w, x64 = f64(weight), f64(x)
+    y = layer.forward(x, off, act="silu")
+    want, mags = eo.experts(x64, w, off.cpu().numpy(), None, "silu")
+    close(y, want, mags, k, "bf16")
+    assert torch.equal(layer.forward(x, off, act="silu"), y)
+
+
+@pytest.mark.parametrize("rows,n,k", [(300, 8192, 512), (2500, 2048, 640), (700, 4096, 1152)])
+def test_fp8_linear_many_tiles(cq, rows, n, k):
+    from nemotron_cuda import fp8
+    gen = rng_of(rows, n, k)
+    x, codes, scales = values(gen, rows, k, spread=0.3), codes_of(gen, n, k), scales_of(gen, -(-n // 128), -(-k // 128)) / k ** 0.5
+    layer = fp8.Fp8Linear.from_codes(codes, scales)
+    y = layer.forward(x)
+    want, mags = eo.linear(row_values(x), weight_values(codes, scales))
+    close(y, want, mags, k, "bf16")
+    assert torch.equal(layer.forward(x), y)
+
+
+@pytest.mark.parametrize("weights", ["16bit", "e4m3"])
 @pytest.mark.parametrize("rows", [6, 200])
 def test_expert_linear_survives_wrong_offsets(cq, weights, rows):
     """Offsets outside the rows, or falling, are cut to the rows: no access out of range, good groups keep their values."""
@@ -402,7 +437,7 @@ def ffn_case(gen, weights, dtype, E, d, ff, tokens):
 @pytest.mark.parametrize("weights", ["16bit", "e4m3"])
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("tokens,E,top,d,ff", [(1, 4, 2, 128, 256), (14, 8, 2, 256, 1024), (33, 3, 3, 200, 333),
-                                               (130, 8, 2, 256, 520), (700, 5, 2, 384, 640)])
+                                               (130, 8, 2, 256, 520), (700, 5, 2, 384, 640), (900, 40, 2, 512, 1024)])
 def test_expert_feed_forward(cq, weights, dtype, tokens, E, top, d, ff):
     """Against the definition, by the 2-norm.  Beyond the roundings of z and y to T (and of h with 16-bit weights), each
     2^-9 (bf16) or 2^-12 (f16) in the mean, an f32 difference may bring a value of h to the next e4m3 code: a share of
