@@ -15,11 +15,9 @@
 // the epilogue of a tile overlaps the next tile's products.
 //
 // Wide tiles are bound by the copies from L2: a 128 x 256 tile takes 48 KB a k
-// block, 1100 cycles at the rate that all SMs have together.  So large groups
-// run on pairs of CTAs (cta_group::2): 256 rows, each CTA half of the weights'
-// tile in its shared memory, 32 KB a CTA.
+// block, 1100 cycles at the rate that all SMs have together.
 //
-// Persistent: a CTA or pair takes every W-th tile of all experts' tiles; the
+// Persistent: a CTA takes every W-th tile of all experts' tiles; the
 // tile list follows from the offsets, which only the device knows.
 //   warps 0, 2  copy tiles of x and of W (TMA, 128-byte swizzle) into a ring
 //   warp 1      issues tcgen05.mma
@@ -72,9 +70,9 @@ struct SmemPlan {
   int stage_bytes, stages, out_off, scale_off, list_off, bar_off, bytes;
 };
 
-__host__ __device__ inline SmemPlan plan_smem(bool e4m3, int bn, int pair, int experts) {
+__host__ __device__ inline SmemPlan plan_smem(bool e4m3, int bn, int experts) {
   SmemPlan p{};
-  p.stage_bytes = stage_blocks(bn) * (kXBytes + bn / pair * kRowBytes);
+  p.stage_bytes = stage_blocks(bn) * (kXBytes + bn * kRowBytes);
   const int list = (2 * (experts + 2) * 4 + 15) / 16 * 16;
   const int bars = (2 * kMaxStages + 2 * kGroups + 2 * kScaleSlots + 2) * 8 + 16;
   const int scales = e4m3 ? kScaleSlots * kScaleBytes : 0;
@@ -91,47 +89,28 @@ __host__ __device__ inline SmemPlan plan_smem(bool e4m3, int bn, int pair, int e
 
 // --------------------------------------------------------------- tcgen05
 
-template <int CG>
 __device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
-  if constexpr (CG == 2) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  } else {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
-template <int CG>
 __device__ __forceinline__ void tmem_release(uint32_t taddr, uint32_t cols) {
-  if constexpr (CG == 2)
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-  else
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
 }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-template <int FMT, int CG>
+template <int FMT>
 __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (FMT == kFmtE4M3 && CG == 2)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-  else if constexpr (FMT == kFmtE4M3)
+  if constexpr (FMT == kFmtE4M3)
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-  else if constexpr (CG == 2)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
   else
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// Arrives on the barrier at `bar` when the MMAs issued so far are done; with a
-// pair, on the barrier at that place in both CTAs.
-template <int CG>
+// Arrives on the barrier at `bar` when the MMAs issued so far are done.
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
-  if constexpr (CG == 2)
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
-  else
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // 32 lanes x 32 (or 16) columns: thread i of the warp gets its lane's columns.
@@ -182,27 +161,19 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
 }
 
 // Instruction descriptor: f32 sums, both operands K-major.
-template <int FMT, int CG>
+template <int FMT>
 __device__ __forceinline__ uint32_t mma_idesc(int n) {
   constexpr uint32_t type = FMT == kFmtBF16 ? 1u : 0u;  // f16 kind: 0 f16, 1 bf16; f8f6f4 kind: 0 e4m3
   return (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
-         (static_cast<uint32_t>(kGemmRows * CG >> 4) << 24);
+         (static_cast<uint32_t>(kGemmRows >> 4) << 24);
 }
 
-// TMA load into this CTA's shared memory, counted on the barrier at `bar`: of a
-// pair, the first CTA's.
-template <int CG>
+// TMA load into this CTA's shared memory, counted on the barrier at `bar`.
 __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, uint64_t policy) {
-  if constexpr (CG == 2)
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint "
-        "[%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar),
-        "l"(policy) : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
-        "[%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar),
-        "l"(policy) : "memory");
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+      "[%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar),
+      "l"(policy) : "memory");
 }
 
 // --------------------------------------------------------------- barriers
@@ -211,12 +182,6 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
 // products have a few hundred cycles a turn, and address arithmetic counts.
 __device__ __forceinline__ void arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// The same on a barrier of the pair's first CTA.  It publishes no memory (a
-// tensor-memory buffer has been read, which tcgen05.fence orders): release at
-// cluster scope would cost a fence of all outstanding stores for every k block.
-__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -432,14 +397,14 @@ __device__ __forceinline__ void set_sync(int set) {
 
 // --------------------------------------------------------------- kernel
 
-template <int FMT, int DT, int CG, int BN>
+template <int FMT, int DT, int BN>
 __global__ void __launch_bounds__(gemm_threads(BN), 1)
     expert_gemm_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap xmap_part,
                        const __grid_constant__ CUtensorMap wmap,
                        const __grid_constant__ CUtensorMap ymap, const ExpertGemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  const SmemPlan L = plan_smem(FMT == kFmtE4M3, BN, CG, a.experts);
+  const SmemPlan L = plan_smem(FMT == kFmtE4M3, BN, a.experts);
   const int stages = L.stages;
   // Tensor memory is two groups of accumulators that go back and forth between
   // the products and the epilogue: of kPer k blocks' partial sums each (e4m3),
@@ -464,8 +429,7 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
 
   // the same in all lanes, and known to be
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int rank = CG == 2 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
+  const int worker = blockIdx.x, workers = gridDim.x;
   const int tiles_n = (a.N + BN - 1) / BN;
   constexpr int kElems = FMT == kFmtE4M3 ? 128 : 64;  // values of a k block
   const int KB = (a.K + kElems - 1) / kElems;
@@ -484,23 +448,22 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
     init(kMaxStages, 2);
     init(kMaxStages, 1);
     init(kGroups, 1);
-    init(kGroups, CG * kSetWarps);
+    init(kGroups, kSetWarps);
     init(kScaleSlots, 32);
     init(kScaleSlots, kSetWarps);
     init(2, kSetWarps);
     fence_mbar_init();
   }
-  if (warp == 2) tmem_alloc<CG>(tmem_slot, kTmemCols);
+  if (warp == 2) tmem_alloc(tmem_slot, kTmemCols);
   // Weights are nobody's result, and the offsets may be known to be there: then
   // the weights' stream starts while the kernel before still runs.  What reads
   // rows or scales, or writes y, waits for it.
   if (warp == 3) {
     if (a.offsets != nullptr && !a.offsets_ready) pdl_wait();
-    build_list(a, list, kGemmRows * CG, tiles_n, lane);
+    build_list(a, list, kGemmRows, tiles_n, lane);
   }
   tc_fence_before();
   __syncthreads();
-  if (CG == 2) cluster_sync_all();  // the other CTA's barriers are ready
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int groups = a.offsets == nullptr ? 1 : a.experts;
@@ -524,34 +487,31 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
       int e = 0, issued = 0;
       Ring ring;
       for (int t = worker; t < total && ok; t += workers) {
-        const Tile tile = find_tile(list, t, kGemmRows * CG, tiles_n, BN, e);
-        const int m = tile.m0 + rank * kGemmRows, boxes = row_boxes(tile.end - m);
-        // both CTAs' bytes count on the first's barrier
-        const int all_boxes = CG == 2 ? row_boxes(tile.end - tile.m0) + row_boxes(tile.end - tile.m0 - kGemmRows) : boxes;
-        const int bytes = warp == 0 ? all_boxes * kBoxBytes : BN * kRowBytes;
-        const int w = tile.expert * a.N + tile.n0 + rank * (BN / CG);
+        const Tile tile = find_tile(list, t, kGemmRows, tiles_n, BN, e);
+        const int boxes = row_boxes(tile.end - tile.m0);
+        const int bytes = warp == 0 ? boxes * kBoxBytes : BN * kRowBytes;
+        const int w = tile.expert * a.N + tile.n0;
         for (int kb = 0; kb < KB; kb += kStageBlocks, ++issued) {
           if (!wait_phase(empty + ring.at * 8, ring.phase ^ 1u, a.status)) {
             ok = false;
             break;
           }
-          uint32_t bar = full + ring.at * 8;
-          if (CG == 2) bar = mapa_shared(bar, 0);
+          const uint32_t bar = full + ring.at * 8;
           const uint32_t dst = dst0 + ring.at * L.stage_bytes;
           const int blocks = min(kStageBlocks, KB - kb);
           if (elect_one()) {
-            if (CG == 1 || rank == 0) arrive_expect(full + ring.at * 8, blocks * bytes);
+            arrive_expect(bar, blocks * bytes);
 #pragma unroll
             for (int j = 0; j < kStageBlocks; ++j) {
               if (j >= blocks) break;
               const int k = (kb + j) * kElems;
               if (warp == 2) {
-                load_tile<CG>(dst + j * (BN / CG) * kRowBytes, &wmap, k, w, bar, keep);
+                load_tile(dst + j * BN * kRowBytes, &wmap, k, w, bar, keep);
               } else if (boxes == kGemmRows / kGemmBoxRows) {
-                load_tile<CG>(dst + j * kXBytes, &xmap, k, m, bar, keep);
+                load_tile(dst + j * kXBytes, &xmap, k, tile.m0, bar, keep);
               } else {
                 for (int b = 0; b < boxes; ++b)
-                  load_tile<CG>(dst + j * kXBytes + b * kBoxBytes, &xmap_part, k, m + b * kGemmBoxRows, bar, keep);
+                  load_tile(dst + j * kXBytes + b * kBoxBytes, &xmap_part, k, tile.m0 + b * kGemmBoxRows, bar, keep);
               }
             }
           }
@@ -559,11 +519,17 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
           ring.next(stages);
         }
       }
-      if (!ok && rank == 0)  // a wait ran out: let the copies in flight land before the CTA ends
+      // The last stages' releases come from the tensor cores and nobody else
+      // waits for them; the barriers have to be there until they have come.
+      for (int i = 0; i < stages && ok; ++i) {
+        ok = wait_phase(empty + ring.at * 8, ring.phase ^ 1u, a.status);
+        ring.next(stages);
+      }
+      if (!ok)  // a wait ran out: let the copies in flight land before the CTA ends
         for (int i = max(0, issued - stages); i < issued; ++i) wait_phase(full + i % stages * 8, (i / stages) & 1, a.status);
-    } else if (warp == 1 && rank == 0) {
+    } else if (warp == 1) {
       // ---------------------------------------------------------- products
-      const uint32_t idesc = mma_idesc<FMT, CG>(BN);
+      const uint32_t idesc = mma_idesc<FMT>(BN);
       // The tensor pipe queues few products, so this loop's scalar work has to
       // fit under them: the whole warp runs it, with values that are the same
       // in all lanes, and one lane issues; ring places by counters,
@@ -588,15 +554,15 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
             for (int j = 0; j < kStageBlocks; ++j) {
               if (j >= blocks) break;
               const uint64_t a0 = da + j * (kXBytes >> 4);
-              const uint64_t b0 = da + kStageBlocks * (kXBytes >> 4) + j * (BN / CG * kRowBytes >> 4);
+              const uint64_t b0 = da + kStageBlocks * (kXBytes >> 4) + j * (BN * kRowBytes >> 4);
               const uint32_t to = FMT == kFmtE4M3 ? d + j * BN : d;
-              tc_mma<FMT, CG>(to, a0, b0, idesc, FMT != kFmtE4M3 && (kb != 0 || j != 0));
-              tc_mma<FMT, CG>(to, a0 + 2, b0 + 2, idesc, 1);
-              tc_mma<FMT, CG>(to, a0 + 4, b0 + 4, idesc, 1);
-              tc_mma<FMT, CG>(to, a0 + 6, b0 + 6, idesc, 1);
+              tc_mma<FMT>(to, a0, b0, idesc, FMT != kFmtE4M3 && (kb != 0 || j != 0));
+              tc_mma<FMT>(to, a0 + 2, b0 + 2, idesc, 1);
+              tc_mma<FMT>(to, a0 + 4, b0 + 4, idesc, 1);
+              tc_mma<FMT>(to, a0 + 6, b0 + 6, idesc, 1);
             }
-            tc_commit<CG>(empty + ring.at * 8);
-            if (closes) tc_commit<CG>(acc_full + acc.at * 8);
+            tc_commit(empty + ring.at * 8);
+            if (closes) tc_commit(acc_full + acc.at * 8);
           }
           __syncwarp();
           ring.next(stages);
@@ -613,8 +579,8 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
       int e = 0;
       Ring ring;
       for (int t = worker; t < total && ok; t += workers) {
-        const Tile tile = find_tile(list, t, kGemmRows * CG, tiles_n, BN, e);
-        const int row0 = tile.m0 + rank * kGemmRows + lane;
+        const Tile tile = find_tile(list, t, kGemmRows, tiles_n, BN, e);
+        const int row0 = tile.m0 + lane;
         const float* sw = a.w_scales + static_cast<int64_t>(tile.expert) * NBLK * KB;
         const int blk0 = min(tile.n0 / kFp8Block, NBLK - 1), blk1 = min((tile.n0 + BN / 2) / kFp8Block, NBLK - 1);
         for (int kb = 0; kb < KB; kb += kScaleBlocks) {
@@ -656,11 +622,7 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
     const int tile_groups = FMT == kFmtE4M3 ? (KB + kPer - 1) / kPer : 1;  // of accumulators, per tile
     const int tile_slots = (KB + kScaleBlocks - 1) / kScaleBlocks;         // of scales, per tile
 
-    const uint32_t acc_empty0 = CG == 2 ? mapa_shared(acc_empty, 0) : acc_empty;
-    const auto hand_back = [&](int group) {
-      if (CG == 2) arrive_cluster(acc_empty0 + group * 8);
-      else arrive(acc_empty0 + group * 8);
-    };
+    const auto hand_back = [&](int group) { arrive(acc_empty + group * 8); };
 
     // rows of no expert are zeros
     if (a.out != kOutCodes) {
@@ -676,15 +638,15 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
 
     int e = 0;
     for (int t = worker + set * workers, seq = set; t < total && ok; t += kSets * workers, seq += kSets) {
-      const Tile tile = find_tile(list, t, kGemmRows * CG, tiles_n, BN, e);
+      const Tile tile = find_tile(list, t, kGemmRows, tiles_n, BN, e);
       Ring ring(seq * tile_groups, kGroups), scales(seq * tile_slots, kScaleSlots);
       // The sets' sums follow one another: a set that waited for its accumulators
       // while the other's are still to come would take a phase of theirs, of the
       // same parity, for its own.
       if (kSets == 2 && seq > 0) ok = wait_phase(token + set * 8, ((seq - 1) / 2) & 1, a.status);
-      const int64_t row = tile.m0 + rank * kGemmRows + local;
+      const int64_t row = tile.m0 + local;
       const bool live = row < tile.end;
-      const int row_w = tile.m0 + rank * kGemmRows + quarter * 32;  // the warp's first row
+      const int row_w = tile.m0 + quarter * 32;  // the warp's first row
       const bool idle = row_w >= tile.end;  // a warp without rows only hands buffers back
       const int n0 = tile.n0 + half * W;
       float acc[FMT == kFmtE4M3 ? W : 1];
@@ -902,85 +864,89 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (CG == 2) cluster_sync_all();  // neither CTA ends while the other signals its barriers
   if (warp == 2) {
     tc_fence_after();
-    tmem_release<CG>(tmem, kTmemCols);
+    tmem_release(tmem, kTmemCols);
   }
 }
 
-template <int FMT, int DT, int CG, int BN>
+template <int FMT, int DT, int BN>
 cudaError_t launch_typed(const ExpertGemmMaps& m, const ExpertGemmArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
-  auto kernel = expert_gemm_kernel<FMT, DT, CG, BN>;
+  auto kernel = expert_gemm_kernel<FMT, DT, BN>;
   static SharedMemoryOptIn opt_in;
   const cudaError_t configured = opt_in.ensure(reinterpret_cast<const void*>(kernel), kSmemLimit - kStaticBytes);
   if (configured != cudaSuccess) return configured;
-  const SmemPlan p = plan_smem(FMT == kFmtE4M3, BN, CG, a.experts);
-  // no more CTAs (or pairs) than tiles there can be
+  const SmemPlan p = plan_smem(FMT == kFmtE4M3, BN, a.experts);
+  // no more CTAs than tiles there can be
   const int64_t groups = a.offsets == nullptr ? 1 : std::min(a.experts, a.rows);
-  const int64_t tiles = ((a.rows + kGemmRows * CG - 1) / (kGemmRows * CG) + groups) * ((a.N + BN - 1) / BN);
-  const int ctas = static_cast<int>(std::min<int64_t>(tiles, num_sms / CG));
-  return launch_clustered(kernel, dim3(ctas * CG), dim3(gemm_threads(BN)), p.bytes, stream, pdl, CG, m.x, m.x_part, m.w, m.y, a);
+  const int64_t tiles = ((a.rows + kGemmRows - 1) / kGemmRows + groups) * ((a.N + BN - 1) / BN);
+  const int ctas = static_cast<int>(std::min<int64_t>(tiles, num_sms));
+  return launch(kernel, dim3(ctas), dim3(gemm_threads(BN)), p.bytes, stream, pdl, m.x, m.x_part, m.w, m.y, a);
 }
 
 template <int FMT, int DT>
-cudaError_t launch_cut(const ExpertGemmCut& cut, const ExpertGemmMaps& m, const ExpertGemmArgs& a, int num_sms,
-                       cudaStream_t stream, bool pdl) {
-  if (cut.pair == 2) return launch_typed<FMT, DT, 2, 256>(m, a, num_sms, stream, pdl);
-  if (cut.bn == 256) return launch_typed<FMT, DT, 1, 256>(m, a, num_sms, stream, pdl);
-  if (cut.bn == 128) return launch_typed<FMT, DT, 1, 128>(m, a, num_sms, stream, pdl);
-  return launch_typed<FMT, DT, 1, 64>(m, a, num_sms, stream, pdl);
+cudaError_t launch_cut(int bn, const ExpertGemmMaps& m, const ExpertGemmArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
+  if (bn == 256) return launch_typed<FMT, DT, 256>(m, a, num_sms, stream, pdl);
+  if (bn == 128) return launch_typed<FMT, DT, 128>(m, a, num_sms, stream, pdl);
+  return launch_typed<FMT, DT, 64>(m, a, num_sms, stream, pdl);
 }
 
 }  // namespace
 
-cudaError_t launch_expert_gemm(int dtype, bool e4m3, const ExpertGemmCut& cut, const ExpertGemmMaps& maps,
+cudaError_t launch_expert_gemm(int dtype, bool e4m3, int bn, const ExpertGemmMaps& maps,
                                const ExpertGemmArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
-  if (cut.bn != 64 && cut.bn != 128 && cut.bn != 256) return cudaErrorInvalidValue;
-  if ((cut.pair == 2 && cut.bn != 256) || (a.out == kOutCodes && cut.bn < kFp8Block)) return cudaErrorInvalidValue;
+  if (bn != 64 && bn != 128 && bn != 256) return cudaErrorInvalidValue;
+  if (a.out == kOutCodes && bn < kFp8Block) return cudaErrorInvalidValue;
   if (e4m3)
-    return dtype == kF16 ? launch_cut<kFmtE4M3, kF16>(cut, maps, a, num_sms, stream, pdl)
-                         : launch_cut<kFmtE4M3, kBF16>(cut, maps, a, num_sms, stream, pdl);
-  return dtype == kF16 ? launch_cut<kFmtF16, kF16>(cut, maps, a, num_sms, stream, pdl)
-                       : launch_cut<kFmtBF16, kBF16>(cut, maps, a, num_sms, stream, pdl);
+    return dtype == kF16 ? launch_cut<kFmtE4M3, kF16>(bn, maps, a, num_sms, stream, pdl)
+                         : launch_cut<kFmtE4M3, kBF16>(bn, maps, a, num_sms, stream, pdl);
+  return dtype == kF16 ? launch_cut<kFmtF16, kF16>(bn, maps, a, num_sms, stream, pdl)
+                       : launch_cut<kFmtBF16, kBF16>(bn, maps, a, num_sms, stream, pdl);
 }
 
-ExpertGemmCut plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, bool codes_out, int num_sms) {
-  // The cut with the least estimated time: waves of tiles, each of its k
-  // blocks' time and a tile's own.  A k block takes the longest of what the
-  // products and the epilogue need, its copies from L2 at the rate that all SMs
-  // have together, and its weights' share of the memory's rate (which the tiles
-  // of one group share: the second finds them in L2).  Cycles, fitted to
-  // measured calls: 8 to 16384 rows, 1 to 64 experts, n and k 512 to 4096.
+int plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, int act, int out, int num_sms) {
+  // The cut with the least estimated time, in cycles: the last pass over a tile
+  // (activation, codes, stores) and for each wave of tiles the sums of its k
+  // blocks, a wave's last pass beside the next wave's sums where two sets of
+  // epilogue warps take turns.  A k block takes the longer of a CTA's own time
+  // and its weights' share of the memory's rate (which the tiles of one group
+  // share: the second finds them in L2).  Fitted to nineteen calls of 16 to 16384
+  // rows, 1 to 64 experts, n and k 520 to 18944, each with all three cuts: the
+  // cut taken is the fastest of them or within 1 % for seventeen, 3 % (n 4096, k
+  // 1024, 16-bit) and 7 % (8192 rows, k 1024, e4m3) behind it for two.  Both sides:
+  //   64 rows, k 4096, n 1024, 8 experts, e4m3   14.1 us at 64, 18.3 at 128, 23.0 at 256
+  //   1792 rows, n 4096, k 1024, 32, e4m3, SiLU  46.5           43.8         70.4
+  //   8192 rows, n 2048, k 1024, 16, 16-bit      67.2           57.8         44.7
   struct Cut {
-    int pair, bn;
-    double block_e4m3, block_16, tile_e4m3, tile_16;
+    int bn;
+    double block_e4m3, block_16, last_e4m3, last_16;
   };
-  static constexpr Cut kCuts[] = {{1, 64, 250, 200, 3500, 2500},
-                                  {1, 128, 400, 350, 4500, 3000},
-                                  {1, 256, 800, 650, 6000, 2500},
-                                  {2, 256, 850, 650, 6000, 2500}};
-  constexpr double kMemoryBytes = 24.0, kL2Bytes = 43.0;  // a cycle and SM
+  static constexpr Cut kCuts[] = {{64, 515, 480, 4300, 300}, {128, 820, 780, 7400, 600}, {256, 1020, 1140, 9900, 800}};
+  constexpr double kMemoryBytes = 18.7;  // a cycle and SM
+  constexpr double kActivation = 1.44;   // of SiLU or codes on the last pass
   const int KB = (K + (e4m3 ? 127 : 63)) / (e4m3 ? 128 : 64);
+  const bool codes = out == kOutCodes;
   // experts that have rows, were the choice of expert even
   const double groups = experts * (1.0 - std::pow(1.0 - 1.0 / experts, rows)), mean = rows / groups;
-  ExpertGemmCut best{1, 256};
+  int best = 256;
   double least = 0.0;
   for (const Cut& c : kCuts) {
-    if (codes_out && c.bn < kFp8Block) continue;
-    const double tile_rows = kGemmRows * c.pair, workers = num_sms / c.pair;
+    if (codes && c.bn < kFp8Block) continue;
     // ragged groups have half a tile more than their mean size
-    double per_group = std::ceil(mean / tile_rows);
-    if (experts > 1 && mean > tile_rows / 2) per_group = mean / tile_rows + 0.5;
-    const double tiles = groups * per_group * ((N + c.bn - 1) / c.bn), busy = std::min(1.0, tiles / workers);
-    const double weights = static_cast<double>(c.bn / c.pair) * kRowBytes;
-    const double x = std::min(mean / c.pair, static_cast<double>(kGemmRows)) * kRowBytes;
-    const double block = std::max({e4m3 ? c.block_e4m3 : c.block_16, weights / kMemoryBytes * busy / per_group,
-                                   (weights + x) / kL2Bytes * busy});
-    const double time = std::ceil(tiles / workers) * (KB * block + (e4m3 ? c.tile_e4m3 : c.tile_16));
+    double per_group = std::ceil(mean / kGemmRows);
+    if (experts > 1 && mean > kGemmRows / 2) per_group = mean / kGemmRows + 0.5;
+    const double tiles = groups * per_group * ((N + c.bn - 1) / c.bn), busy = std::min(1.0, tiles / num_sms);
+    const double block = std::max(e4m3 ? c.block_e4m3 : c.block_16, c.bn * kRowBytes / kMemoryBytes * busy / per_group);
+    const double sums = KB * block;
+    const double last = (e4m3 ? c.last_e4m3 : c.last_16) * (codes || act == kActSilu ? kActivation : 1.0);
+    // (16-bit sums of the next tile begin while this one's are read)
+    double wave = std::max(sums, last);
+    if (e4m3) wave = epi_sets(c.bn) == 2 ? std::max(sums, (sums + last) / 2) : sums + last;
+    const double waves = std::max(1.0, std::ceil(tiles / num_sms - 1e-9));
+    const double time = sums + last + (waves - 1) * wave;
     if (least == 0.0 || time < least) {
       least = time;
-      best = {c.pair, c.bn};
+      best = c.bn;
     }
   }
   return best;

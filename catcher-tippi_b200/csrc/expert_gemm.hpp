@@ -34,21 +34,17 @@ struct ExpertGemmArgs {
 constexpr int kStoreRows = 32, kStoreBytes = 64;
 
 // Tensor maps of one call.  x, x_part: [rows, K], box 128 bytes x 128 and x 32
-// rows; w: [experts * N, K], box 128 bytes x bn / pair rows; all with the
+// rows; w: [experts * N, K], box 128 bytes x bn rows; all with the
 // 128-byte swizzle.  y: [rows, N] in its own type, box 64 bytes x 32 rows, 64-byte
 // swizzle, used where tile_store says that y's rows allow it (16-byte aligned).
 struct ExpertGemmMaps {
   CUtensorMap x, x_part, w, y;
 };
 
-// How a call is cut: CTAs to a tile (1 of 128 rows, or a pair of 256) and weight
-// rows of a tile (64, 128 or 256; pairs: 256; codes: 128 or 256).
-struct ExpertGemmCut {
-  int pair, bn;
-};
-
-cudaError_t launch_expert_gemm(int dtype, bool e4m3, const ExpertGemmCut& cut, const ExpertGemmMaps& maps,
-                               const ExpertGemmArgs& a, int num_sms, cudaStream_t stream, bool pdl);
-ExpertGemmCut plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, bool codes_out, int num_sms);
+// `bn`: weight rows of a tile, 64, 128 or 256 (codes: 128 or 256); what
+// plan_expert_gemm returns.
+cudaError_t launch_expert_gemm(int dtype, bool e4m3, int bn, const ExpertGemmMaps& maps, const ExpertGemmArgs& a,
+                               int num_sms, cudaStream_t stream, bool pdl);
+int plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, int act, int out, int num_sms);
 
 }  // namespace cq

@@ -215,18 +215,18 @@ void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, cons
   a.y_scales = out.scales;
   a.status = ctx.status;
   const bool codes = out.kind == cq::kOutCodes;
-  const cq::ExpertGemmCut cut = cq::plan_expert_gemm(e4m3(), rows, experts_, N_, K_, codes, ctx.num_sms);
+  const int bn = cq::plan_expert_gemm(e4m3(), rows, experts_, N_, K_, act, out.kind, ctx.num_sms);
   const int size = e4m3() ? 1 : 2, k = 128 / size;
   const int ysize = codes ? 1 : out.kind == cq::kOutF32 ? 4 : 2;
   a.tile_store = out.ld * ysize % 16 == 0 && (reinterpret_cast<uintptr_t>(out.y) & 15) == 0;
   cq::ExpertGemmMaps maps;
   maps.x = make_map_2d(from, size, rows, K_, ld, cq::kGemmRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
   maps.x_part = make_map_2d(from, size, rows, K_, ld, cq::kGemmBoxRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
-  maps.w = make_map_2d(weight_.get(), size, experts_ * N_, K_, ldw_, cut.bn / cut.pair, k, CU_TENSOR_MAP_SWIZZLE_128B);
+  maps.w = make_map_2d(weight_.get(), size, experts_ * N_, K_, ldw_, bn, k, CU_TENSOR_MAP_SWIZZLE_128B);
   maps.y = !a.tile_store ? maps.x
                          : make_map_2d(out.y, ysize, rows, codes ? static_cast<int>(out.ld) : N_, out.ld,
                                        cq::kStoreRows, cq::kStoreBytes / ysize, CU_TENSOR_MAP_SWIZZLE_64B);
-  check_cuda(cq::launch_expert_gemm(dtype_, e4m3(), cut, maps, a, ctx.num_sms, stream, pdl), "expert product");
+  check_cuda(cq::launch_expert_gemm(dtype_, e4m3(), bn, maps, a, ctx.num_sms, stream, pdl), "expert product");
 }
 
 void ExpertLinear::forward(const void* x, int64_t ldx, int rows, const int32_t* offsets, void* y, int64_t ldy, int act,
