@@ -27,9 +27,9 @@ size_t size_or_refuse(F&& f) {
   return guarded([&] { n = f(); }) == CQ_OK ? n : SIZE_MAX;
 }
 
-size_t rows_workspace(const ExpertLinear& layer, int32_t rows) {
+size_t rows_workspace(const ExpertLinear& layer, int32_t rows, bool grouped) {
   if (rows < 0) throw_invalid("negative row count");
-  return layer.workspace(rows);
+  return layer.workspace(rows, grouped);
 }
 
 }  // namespace
@@ -63,7 +63,7 @@ cq_status cq_fp8_linear_create_from_f32(const float* weight, const float* bias_o
 size_t cq_fp8_linear_workspace(const cq_fp8_linear* layer, int32_t rows) {
   return size_or_refuse([&] {
     need_handle(layer, "layer");
-    return rows_workspace(*layer->impl, rows);
+    return rows_workspace(*layer->impl, rows, false);
   });
 }
 
@@ -115,7 +115,7 @@ cq_status cq_expert_linear_create(const void* weight, const float* scales, const
 size_t cq_expert_linear_workspace(const cq_expert_linear* layer, int32_t rows) {
   return size_or_refuse([&] {
     need_handle(layer, "layer");
-    return rows_workspace(*layer->impl, rows);
+    return rows_workspace(*layer->impl, rows, true);
   });
 }
 

@@ -148,9 +148,9 @@ size_t ExpertLinear::staging_bytes(int64_t rows) const {
   return round_up(rows * ld, 256) + rows * (ld / kBlock) * sizeof(float);
 }
 
-size_t ExpertLinear::workspace(int rows) const {
-  // the streaming kernel of a single expert needs none
-  return experts_ == 1 && few_rows(rows, false) ? 0 : round_up(staging_bytes(rows), 256);
+size_t ExpertLinear::workspace(int rows, bool grouped) const {
+  // the streaming kernel needs none
+  return few_rows(rows, grouped) ? 0 : round_up(staging_bytes(rows), 256);
 }
 
 bool ExpertLinear::few_rows(int rows, bool grouped) const {
@@ -234,7 +234,7 @@ void ExpertLinear::forward(const void* x, int64_t ldx, int rows, const int32_t* 
   check_rows(x, ldx, rows, y, ldy, act);
   check_aligned(x, 2, "input");
   if (rows == 0) return;
-  check_workspace(workspace, workspace_bytes, this->workspace(rows));
+  check_workspace(workspace, workspace_bytes, this->workspace(rows, offsets != nullptr));
   DeviceGuard guard(device_);
   product({cq::kSourceT, x, ldx, nullptr, nullptr, rows}, rows, offsets, {cq::kOutT, y, ldy, nullptr}, act,
           workspace, stream);

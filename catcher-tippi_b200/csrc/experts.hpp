@@ -23,7 +23,8 @@ class ExpertLinear {
   static std::unique_ptr<ExpertLinear> from_f32(const float* weight, const float* bias, int output_dims,
                                                 int input_dims, cq_dtype dtype, int device);
 
-  size_t workspace(int rows) const;
+  // bytes of forward's workspace; `grouped`: with offsets
+  size_t workspace(int rows, bool grouped) const;
   // offsets null: all rows meet the only expert.
   void forward(const void* x, int64_t ldx, int rows, const int32_t* offsets, void* y, int64_t ldy, int act,
                void* workspace, size_t workspace_bytes, cudaStream_t stream) const;

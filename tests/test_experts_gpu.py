@@ -518,3 +518,29 @@ def test_calls_on_other_streams_and_in_a_graph(cq):
 
 def test_no_wait_ran_out(cq):
     assert cq.device_status(0) == 0
+
+
+@pytest.mark.parametrize("weights", ["16bit", "e4m3"])
+@pytest.mark.parametrize("rows", [1, 7, 32, 33])
+def test_expert_linear_of_one_expert(cq, weights, rows):
+    """One expert and few rows: the call says what workspace it needs, and refuses less."""
+    from nemotron_cuda import experts
+    gen = rng_of("one", weights, rows)
+    n, k = 200, 136
+    x, off = values(gen, rows, k), offsets_of([rows])
+    if weights == "e4m3":
+        codes, scales = codes_of(gen, 1, n, k), scales_of(gen, 1, 2, 2)
+        layer = experts.ExpertLinear.from_codes(codes, scales)
+        w, x64 = weight_values(codes[0], scales[0])[None], row_values(x)
+    else:
+        weight = values(gen, 1, n, k)
+        layer = experts.ExpertLinear.from_weight(weight)
+        w, x64 = f64(weight), f64(x)
+    need = cq.lib().cq_expert_linear_workspace(layer._h, rows)
+    assert need >= rows * k
+    y = torch.empty(rows, n, dtype=torch.bfloat16, device="cuda")
+    assert cq.lib().cq_expert_linear_forward(layer._h, x.data_ptr(), k, rows, off.data_ptr(), y.data_ptr(), n, 0, None, 0,
+                                             None) == cq.CQ_INVALID_ARGUMENT
+    layer.forward(x, off, y=y)
+    want, mags = eo.experts(x64, w, off.cpu().numpy(), None, "none")
+    close(y, want, mags, k, "bf16")
