@@ -1,4 +1,4 @@
-// The grouped product for few rows: see expert_gemv.cu.
+// The fp8 linear for few rows: see expert_gemv.cu.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -8,31 +8,28 @@
 
 namespace cq {
 
-// What the rows of x are: T or f32 (brought to e4m3 by the kernel where the
-// weights are), or e4m3 codes with their scales.
-enum ExpertSource : int { kSourceT = 0, kSourceF32 = 1, kSourceCodes = 2 };
+// What the rows of x are: T, brought to e4m3 on the way where the weights are, or
+// e4m3 codes with their scales.
+enum ExpertSource : int { kSourceT = 0, kSourceCodes = 1 };
+
+constexpr int kGemvMaxRows = 32;
 
 struct ExpertGemvArgs {
-  const void* x;
+  const void* x;  // codes: 16-byte aligned rows
   int64_t ldx;
-  const int32_t* row_index;  // row r is x row row_index[r]; outside [0, x_rows) it is zero; null: x row r
-  int x_rows;
   const float* x_scales;  // codes: [k blocks][rows]
   int rows;
-  const void* w;  // [experts][N][ldw], rows padded with zeros to 128 bytes
+  const void* w;  // codes [N][ldw], rows padded with zeros to 128 bytes
   int64_t ldw;
   const float* w_scales;
   const void* bias;
-  const int32_t* offsets;
-  int experts, N, K, act;
-  int y_f32;
+  int N, K, act;
   void* y;
   int64_t ldy;
 };
 
-// Whether the kernel can take the call (its rows fit shared memory).
-bool expert_gemv_fits(bool e4m3, int rows, int K);
-cudaError_t launch_expert_gemv(int dtype, bool e4m3, int source, const ExpertGemvArgs& a, int num_sms,
-                               cudaStream_t stream, bool pdl);
+// Whether the kernel can take the call: 1 to kGemvMaxRows rows that fit shared memory.
+bool expert_gemv_fits(int rows, int K);
+cudaError_t launch_expert_gemv(int dtype, int source, const ExpertGemvArgs& a, int num_sms, cudaStream_t stream, bool pdl);
 
 }  // namespace cq

@@ -154,7 +154,7 @@ size_t ExpertLinear::workspace(int rows, bool grouped) const {
 }
 
 bool ExpertLinear::few_rows(int rows, bool grouped) const {
-  return !grouped && rows <= 32 && cq::expert_gemv_fits(e4m3(), rows, K_);
+  return !grouped && e4m3() && cq::expert_gemv_fits(rows, K_);
 }
 
 void ExpertLinear::check_rows(const void* x, int64_t ldx, int rows, const void* y, int64_t ldy, int act) const {
@@ -170,11 +170,10 @@ void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, cons
                            cudaStream_t stream) const {
   DeviceContext& ctx = device_context(device_);
   const bool pdl = pdl_enabled();
-  if (out.kind != cq::kOutCodes && few_rows(rows, offsets != nullptr)) {
-    const cq::ExpertGemvArgs a{x.x,           x.ld,  x.row_index,        x.x_rows,     x.scales, rows,
-                               weight_.get(), ldw_,  scales_.as<float>(), bias_.get(), offsets,  experts_,
-                               N_,            K_,    act,                out.kind == cq::kOutF32, out.y,  out.ld};
-    check_cuda(cq::launch_expert_gemv(dtype_, e4m3(), x.source, a, ctx.num_sms, stream, pdl), "expert product");
+  if (few_rows(rows, offsets != nullptr)) {
+    const cq::ExpertGemvArgs a{x.x, x.ld, x.scales, rows, weight_.get(), ldw_, scales_.as<float>(), bias_.get(),
+                               N_,  K_,   act,      out.y, out.ld};
+    check_cuda(cq::launch_expert_gemv(dtype_, x.source, a, ctx.num_sms, stream, pdl), "expert product");
     return;
   }
   // rows as the tile copies take them: codes, or 16-byte aligned rows of T
@@ -186,8 +185,7 @@ void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, cons
     ld = round_up(K_, kBlock);
     float* s = reinterpret_cast<float*>(static_cast<char*>(staging) + round_up(rows * ld, 256));
     const cq::QuantizeRowsArgs q{x.x, x.ld, x.row_index, x.x_rows, rows, K_, static_cast<uint8_t*>(staging), ld, s};
-    check_cuda(cq::launch_quantize_rows(x.source == cq::kSourceF32 ? static_cast<int>(CQ_F32) : dtype_, q, stream, pdl),
-               "quantize rows");
+    check_cuda(cq::launch_quantize_rows(dtype_, q, stream, pdl), "quantize rows");
     from = staging;
     x_scales = s;
     staged = true;
@@ -350,8 +348,8 @@ struct FfnScratch {
   float* weight;
   void* route;
   size_t route_bytes;
-  void *x, *h_staged;  // the products' staging
-  void* h;             // up's result: T; f32 on its way to e4m3; or codes and scales
+  void* x;  // the first product's staging
+  void* h;  // up's result: T, or codes and scales
   int64_t ld_h;
   float* z;  // f32: the sum over a token's experts is rounded once
 };
@@ -368,10 +366,7 @@ FfnScratch take_ffn(Arena& arena, const ExpertLinear& up, const ExpertLinear& do
   s.route = arena.take<uint8_t>(s.route_bytes);
   s.x = arena.take<uint8_t>(up.staging_bytes(pairs));
   s.ld_h = round_up(up.output_dims(), 8);
-  const bool few = up.few_rows(static_cast<int>(pairs), true);
-  s.h_staged = up.e4m3() && few ? arena.take<uint8_t>(down.staging_bytes(pairs)) : nullptr;
-  s.h = up.e4m3() && !few ? arena.take<uint8_t>(down.staging_bytes(pairs))
-                          : arena.take<uint8_t>(pairs * s.ld_h * (up.e4m3() ? 4 : 2));
+  s.h = arena.take<uint8_t>(up.e4m3() ? down.staging_bytes(pairs) : pairs * s.ld_h * 2);
   s.z = arena.take<float>(pairs * down.output_dims());
   return s;
 }
@@ -420,9 +415,6 @@ void expert_ffn(const ExpertLinear& up, const ExpertLinear& down, const void* x,
   if (!up.e4m3()) {
     up.product(rows, pairs, s.offsets, {cq::kOutT, s.h, s.ld_h, nullptr}, act, s.x, stream);
     h.offsets_ready = true;  // a gather and the first product ran since the route
-  } else if (up.few_rows(pairs, true)) {
-    up.product(rows, pairs, s.offsets, {cq::kOutF32, s.h, s.ld_h, nullptr}, act, s.x, stream);
-    h.source = cq::kSourceF32;
   } else {
     // from f32 sums to codes inside the first product
     const int64_t ld = round_up(up.output_dims(), kBlock);
@@ -431,7 +423,7 @@ void expert_ffn(const ExpertLinear& up, const ExpertLinear& down, const void* x,
     h = {cq::kSourceCodes, s.h, ld, scales, nullptr, pairs};
     h.offsets_ready = true;  // the first product ran between the route and the second
   }
-  down.product(h, pairs, s.offsets, {cq::kOutF32, s.z, out, nullptr}, CQ_ACT_NONE, s.h_staged, stream);
+  down.product(h, pairs, s.offsets, {cq::kOutF32, s.z, out, nullptr}, CQ_ACT_NONE, nullptr, stream);
   const cq::CombineArgs c{s.z, out, s.position, s.weight, pairs, tokens, top, out, y, ldy, 1};
   check_cuda(cq::launch_combine(up.dtype(), c, stream, pdl_enabled()), "combine");
 }

@@ -38,7 +38,7 @@ class ExpertLinear {
   cq_dtype dtype() const { return dtype_; }
   int device() const { return device_; }
 
-  // Rows of a product: T, f32 (e4m3 weights only) or e4m3 codes with their
+  // Rows of a product: T, or e4m3 codes with their
   // scales [k blocks][rows], as cq::ExpertSource says; row r is x row
   // row_index[r] where that is given (T only).
   struct Rows {
