@@ -6,7 +6,7 @@
 // it looks at x.  The lane's bytes are used as the A fragment of mma.sync as
 // they come: which k a fragment slot holds does not matter as long as x, the B
 // fragment, is permuted alike, and both are read as the same 32 bytes of a
-// block.  mma.sync, not tcgen05: at 32 rows or fewer the products take less
+// block.  mma.sync, not tcgen05: at so few rows the products take less
 // than a tenth of the time of the weights' bytes, and this path has no
 // tensor-memory set-up and no copy into shared memory before it can start.
 //
@@ -29,7 +29,7 @@ namespace cq {
 namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
-constexpr int kMaxRows = kGemvMaxRows;
+constexpr int kMaxRows = kGemvMaxRows, kTiles = kMaxRows / 8;
 constexpr int kAhead = 4;       // k blocks a warp has in flight
 constexpr int kSmemMax = 200 * 1024;
 
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kThreads) expert_gemv_kernel(const ExpertGemvA
   const int n = a.rows, tiles = (n + 7) >> 3;
   stage_x<DT, SRC>(a, kb0, kb1, xs, pitch, sx);
   __syncthreads();
-  float acc[4][4] = {};
+  float acc[kTiles][4] = {};
   for (int b0 = wb0; b0 < wb1; b0 += kAhead) {
     if (b0 != wb0) {
 #pragma unroll
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kThreads) expert_gemv_kernel(const ExpertGemvA
       const int b = b0 + i - kb0;
       const float scale = __ldg(sw + b0 + i);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      for (int t = 0; t < kTiles; ++t) {
         if (t < tiles) {
           const uint4* xp = reinterpret_cast<const uint4*>(xs + (t * 8 + g) * pitch + b * 128 + q * 32);
           const uint4 x0 = xp[0], x1 = xp[1];
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) expert_gemv_kernel(const ExpertGemvA
   }
   // the slices' sums, row by row of the tile
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
+  for (int t = 0; t < kTiles; ++t) {
     if (t < tiles) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -285,8 +285,16 @@ cudaError_t launch_dtype(int source, const ExpertGemvArgs& a, int num_sms, cudaS
 
 }  // namespace
 
-bool expert_gemv_fits(int rows, int K) {
-  if (rows > kMaxRows) return false;
+bool expert_gemv_fits(int rows, int N, int K) {
+  // Every CTA brings the rows to e4m3 for itself, so the work beside the weights'
+  // stream is as rows * N * K, while tiles on the tensor cores start later and
+  // take a second launch (9.1 us of host time against 13.9).  us here / there:
+  //   rows          8          16          24          32
+  //   4096 x 1024   4.2/7.6    5.2/7.6     7.3/7.0     8.0/7.3
+  //   1024 x 4096   4.5/11.4   6.6/11.4    9.8/11.4    16.1/11.4
+  //   2048 x 2048   4.8/8.6    6.6/8.6     9.7/8.6     10.2/8.6
+  //   4096 x 4096   7.6/13.5   14.8/12.4   30.3/12.1   33.4/12.1
+  if (rows > kMaxRows || (rows > 8 && static_cast<int64_t>(N) * K > (1 << 23))) return false;
   const int KB = (K + kFp8Block - 1) / kFp8Block;
   int splits = 1;
   for (int s : {2, 4, 8})
@@ -296,7 +304,7 @@ bool expert_gemv_fits(int rows, int K) {
 }
 
 cudaError_t launch_expert_gemv(int dtype, int source, const ExpertGemvArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
-  if (!expert_gemv_fits(a.rows, a.K)) return cudaErrorInvalidValue;
+  if (!expert_gemv_fits(a.rows, a.N, a.K)) return cudaErrorInvalidValue;
   return dtype == kF16 ? launch_dtype<kF16>(source, a, num_sms, stream, pdl)
                        : launch_dtype<kBF16>(source, a, num_sms, stream, pdl);
 }

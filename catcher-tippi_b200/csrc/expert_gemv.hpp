@@ -12,7 +12,7 @@ namespace cq {
 // e4m3 codes with their scales.
 enum ExpertSource : int { kSourceT = 0, kSourceCodes = 1 };
 
-constexpr int kGemvMaxRows = 32;
+constexpr int kGemvMaxRows = 24;
 
 struct ExpertGemvArgs {
   const void* x;  // codes: 16-byte aligned rows
@@ -28,8 +28,8 @@ struct ExpertGemvArgs {
   int64_t ldy;
 };
 
-// Whether the kernel can take the call: 1 to kGemvMaxRows rows that fit shared memory.
-bool expert_gemv_fits(int rows, int K);
+// Whether the kernel takes the call: few rows, by measured times, that fit shared memory.
+bool expert_gemv_fits(int rows, int N, int K);
 cudaError_t launch_expert_gemv(int dtype, int source, const ExpertGemvArgs& a, int num_sms, cudaStream_t stream, bool pdl);
 
 }  // namespace cq

@@ -154,7 +154,7 @@ size_t ExpertLinear::workspace(int rows, bool grouped) const {
 }
 
 bool ExpertLinear::few_rows(int rows, bool grouped) const {
-  return !grouped && e4m3() && cq::expert_gemv_fits(rows, K_);
+  return !grouped && e4m3() && cq::expert_gemv_fits(rows, N_, K_);
 }
 
 void ExpertLinear::check_rows(const void* x, int64_t ldx, int rows, const void* y, int64_t ldy, int act) const {

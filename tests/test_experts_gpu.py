@@ -267,7 +267,7 @@ def test_expert_linear(cq, weights, name, n, k):
 @pytest.mark.parametrize("experts,counts,n,k", [(40, 3, 2048, 1024), (40, 3, 1024, 1400), (24, 70, 1024, 640), (30, 40, 512, 2048),
                                                (4, 700, 1024, 384), (6, 400, 2048, 512)])
 def test_expert_linear_many_tiles(cq, weights, experts, counts, n, k):
-    """Several tiles a CTA, of every width and pairing: the rings of copies, sums and scales go on from tile to tile."""
+    """Several tiles a CTA, of every width: the rings of copies, sums and scales go on from tile to tile."""
     from nemotron_cuda import experts as ex
     gen = rng_of(experts, counts, n, k)
     sizes = [counts + (i * 7) % 5 - 2 for i in range(experts)]
