@@ -171,22 +171,32 @@ __device__ __forceinline__ float fast_reciprocal(float v) {
 }
 constexpr float kLog2E = 1.4426950408889634f;
 
-// SiLU of two values, v / (1 + 2^(-v log2 e)): one reciprocal serves both,
-// 1 / a = b / (a b), as an epilogue of SiLUs is bound by the special-function
-// unit and by its instruction count.  -v log2 e is cut at 62, so that a b stays
-// below the range of the reciprocal: past it SiLU is under 1e-17 either way.  The approximate functions
-// are off by a few f32 ulps, far inside T's rounding step; values that a flush
-// of subnormals touches are 2^-126 next to 1.
+// 2^(v log2 e) for SiLU, v's sigmoid being that over one more than it.  The
+// exponent is cut at 62 above, where the sigmoid is 1 to the last bit; below,
+// the power goes to 0 by itself, and with it the factor of v: 0 from -88 on for
+// every finite v, NaN for -infinity, as the formula says.
+__device__ __forceinline__ float silu_power(float v) { return fast_exp2(fminf(kLog2E * v, 62.0f)); }
+
+// SiLU of two values, v p / (1 + p) with p = 2^(v log2 e): one reciprocal serves
+// both, 1 / a = b / (a b), as an epilogue of SiLUs is bound by the
+// special-function unit and by its instruction count.  a and b are at most 2^62,
+// so a b stays in the range of the reciprocal.  The largest error is that of the
+// rounded v log2 e: 2^-17 of the value next to v = -88, a few f32 ulps around 0,
+// both far inside T's rounding step.  Powers under 2^-126 are flushed to 0, values
+// under 2^-119.
 __device__ __forceinline__ void silu2(float& x, float& y) {
-  const float a = 1.0f + fast_exp2(fminf(-kLog2E * x, 62.0f)), b = 1.0f + fast_exp2(fminf(-kLog2E * y, 62.0f));
+  const float p = silu_power(x), q = silu_power(y), a = 1.0f + p, b = 1.0f + q;
   const float r = fast_reciprocal(a * b);
-  x *= r * b;
-  y *= r * a;
+  x *= p * (r * b);
+  y *= q * (r * a);
 }
 
-// act(v) in f32 for the fp8 and expert linears' epilogues.
+// act(v) in f32 for the few-row linear's last pass.
 __device__ __forceinline__ float activate(float v, int act) {
-  if (act == kActSilu) return v * fast_reciprocal(1.0f + fast_exp2(fminf(-kLog2E * v, 126.0f)));
+  if (act == kActSilu) {
+    const float p = silu_power(v);
+    return v * (p * fast_reciprocal(1.0f + p));
+  }
   if (act == kActRelu) return v < 0.0f ? 0.0f : v;
   return v;
 }
