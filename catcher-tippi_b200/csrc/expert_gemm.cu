@@ -12,7 +12,10 @@
 // warps multiply that partial sum by scale(x) * scale(w) and add it to f32
 // registers, while the tensor cores work on the next block in another
 // tensor-memory buffer.  16-bit: kind::f16 sums all of k in tensor memory, and
-// the epilogue of a tile overlaps the next tile's products.
+// the epilogue of a tile overlaps the next tile's products.  Rows of x that come
+// as the sum of two 16-bit parts (h of the feed-forward module) meet each k block
+// of the weights twice; narrow tiles have both parts in one stage, with one copy
+// of the weights.
 //
 // Wide tiles are bound by the copies from L2: a 128 x 256 tile takes 48 KB a k
 // block, 1100 cycles at the rate that all SMs have together.
@@ -176,6 +179,14 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
       "l"(policy) : "memory");
 }
 
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar,
+                                          uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+      "[%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z),
+      "r"(bar), "l"(policy) : "memory");
+}
+
 // --------------------------------------------------------------- barriers
 
 // Barriers go by their shared-memory addresses: the loops that issue copies and
@@ -314,10 +325,11 @@ __device__ __forceinline__ void store32(void* p, const uint32_t* w) {
 // (16-byte pieces in the 64-byte swizzle, free of bank conflicts) to one tile
 // store.  Whole sectors leave the SM in few requests; a store by each lane to
 // its own row touches 32 lines an instruction.  Where there are two buffers they
-// take turns, and a piece waits for the one before the last.
-template <int BUFFERS>
+// take turns, and a piece waits for the one before the last.  `PARTS`: y's map
+// has parts, of which this is one's.
+template <int BUFFERS, bool PARTS>
 __device__ __forceinline__ void store_piece(uint8_t* out_s, int& turn, int lane, const uint32_t* w,
-                                            const CUtensorMap* ymap, int n, int row) {
+                                            const CUtensorMap* ymap, int n, int row, int part) {
   uint8_t* buf = out_s + turn * kStageOut;
   if constexpr (BUFFERS == 2) {
     turn ^= 1;
@@ -333,8 +345,12 @@ __device__ __forceinline__ void store_piece(uint8_t* out_s, int& turn, int lane,
   fence_proxy_async_shared();
   __syncwarp();
   if (lane == 0) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
-                     reinterpret_cast<uint64_t>(ymap)), "r"(n), "r"(row), "r"(smem_u32(buf)) : "memory");
+    if constexpr (PARTS)
+      asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+                       reinterpret_cast<uint64_t>(ymap)), "r"(n), "r"(row), "r"(part), "r"(smem_u32(buf)) : "memory");
+    else
+      asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                       reinterpret_cast<uint64_t>(ymap)), "r"(n), "r"(row), "r"(smem_u32(buf)) : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   }
 }
@@ -432,7 +448,9 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
   const int worker = blockIdx.x, workers = gridDim.x;
   const int tiles_n = (a.N + BN - 1) / BN;
   constexpr int kElems = FMT == kFmtE4M3 ? 128 : 64;  // values of a k block
-  const int KB = (a.K + kElems - 1) / kElems;
+  const int parts = FMT == kFmtE4M3 ? 1 : a.x_parts;
+  const int KB = (a.K + kElems - 1) / kElems * parts;  // block kb: part kb % parts of x
+  const bool shared_w = kStageBlocks == 2 && parts == 2;  // a stage's two blocks are one block's parts
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&xmap);
@@ -498,20 +516,25 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
           }
           const uint32_t bar = full + ring.at * 8;
           const uint32_t dst = dst0 + ring.at * L.stage_bytes;
-          const int blocks = min(kStageBlocks, KB - kb);
+          const int blocks = warp == 2 && shared_w ? 1 : min(kStageBlocks, KB - kb);
           if (elect_one()) {
             arrive_expect(bar, blocks * bytes);
 #pragma unroll
             for (int j = 0; j < kStageBlocks; ++j) {
               if (j >= blocks) break;
-              const int k = (kb + j) * kElems;
+              const int part = parts == 2 ? (kb + j) & 1 : 0;
+              const int k = (parts == 2 ? (kb + j) >> 1 : kb + j) * kElems;
+              const auto load_x = [&](uint32_t to, const CUtensorMap* map, int row) {
+                if constexpr (FMT == kFmtE4M3) load_tile(to, map, k, row, bar, keep);
+                else load_tile(to, map, k, row, part, bar, keep);
+              };
               if (warp == 2) {
                 load_tile(dst + j * BN * kRowBytes, &wmap, k, w, bar, keep);
               } else if (boxes == kGemmRows / kGemmBoxRows) {
-                load_tile(dst + j * kXBytes, &xmap, k, tile.m0, bar, keep);
+                load_x(dst + j * kXBytes, &xmap, tile.m0);
               } else {
                 for (int b = 0; b < boxes; ++b)
-                  load_tile(dst + j * kXBytes + b * kBoxBytes, &xmap_part, k, tile.m0 + b * kGemmBoxRows, bar, keep);
+                  load_x(dst + j * kXBytes + b * kBoxBytes, &xmap_part, tile.m0 + b * kGemmBoxRows);
               }
             }
           }
@@ -536,6 +559,7 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
       // descriptors by adds (every address field stays below 2^14).
       const uint64_t base = sw128_desc(smem_u32(smem));
       const uint32_t stage_units = static_cast<uint32_t>(L.stage_bytes) >> 4;
+      const uint32_t w_step = shared_w ? 0 : BN * kRowBytes >> 4;  // from a stage's block of weights to the next
       Ring ring, acc;
       for (int t = worker; t < total && ok; t += workers) {
         int sub = 0;  // e4m3: every k block starts a sum of its own, kPer of them to a group
@@ -554,7 +578,7 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
             for (int j = 0; j < kStageBlocks; ++j) {
               if (j >= blocks) break;
               const uint64_t a0 = da + j * (kXBytes >> 4);
-              const uint64_t b0 = da + kStageBlocks * (kXBytes >> 4) + j * (BN * kRowBytes >> 4);
+              const uint64_t b0 = da + kStageBlocks * (kXBytes >> 4) + j * w_step;
               const uint32_t to = FMT == kFmtE4M3 ? d + j * BN : d;
               tc_mma<FMT>(to, a0, b0, idesc, FMT != kFmtE4M3 && (kb != 0 || j != 0));
               tc_mma<FMT>(to, a0 + 2, b0 + 2, idesc, 1);
@@ -624,8 +648,8 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
 
     const auto hand_back = [&](int group) { arrive(acc_empty + group * 8); };
 
-    // rows of no expert are zeros
-    if (a.out != kOutCodes) {
+    // rows of no expert are zeros (codes and parts are the module's own: it does not read those rows)
+    if (a.out == kOutT || a.out == kOutF32) {
       const int size = a.out == kOutF32 ? 4 : 2;
       for (int64_t r = list.start[groups] + static_cast<int64_t>(blockIdx.x); r < a.rows; r += gridDim.x) {
         char* p = reinterpret_cast<char*>(a.y) + r * a.ldy * size;
@@ -812,7 +836,7 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
               w[i] = e4m3x2_finite(v[0] * inv, v[1] * inv) | (e4m3x2_finite(v[2] * inv, v[3] * inv) << 16);
             }
             if (whole) {
-              store_piece<kOuts>(out_s, turn_out, lane, w, &ymap, n0 + h, row_w);
+              store_piece<kOuts, false>(out_s, turn_out, lane, w, &ymap, n0 + h, row_w, 0);
             } else if (live) {
               store_piece_by_lanes(w, reinterpret_cast<uint8_t*>(a.y) + row * a.ldy + n0 + h);
             }
@@ -832,27 +856,33 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
         take(c, v);
         if (n0 + c >= a.N) continue;
         finish(c, v);
-        // 64 bytes a piece: 16 f32 values, or 32 of T
+        // 64 bytes a piece: 16 f32 values, or 32 of T; of parts the low one second
         uint32_t w[16];
-        const int pieces = a.out == kOutF32 ? 2 : 1;
+        const int pieces = a.out == kOutT ? 1 : 2;
 #pragma unroll 1
         for (int p = 0; p < pieces; ++p) {
-          const int n = n0 + c + 16 * p;
+          const int n = n0 + c + (a.out == kOutF32 ? 16 * p : 0);
+          const int part = FMT != kFmtE4M3 && a.out == kOutParts ? p : 0;
           if (n >= a.N) break;
           if (a.out == kOutF32) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(p == 0 ? v[i] : v[16 + i]);
           } else {
+            if (part == 1) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) take_rest_t<DT>(w[i], v[2 * i], v[2 * i + 1]);
+            }
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = pack_t<DT>(v[2 * i], v[2 * i + 1]);
           }
+          uint8_t* y = reinterpret_cast<uint8_t*>(a.y) + part * (a.rows * a.ldy * size);
           if (whole) {
-            store_piece<kOuts>(out_s, turn_out, lane, w, &ymap, n, row_w);
+            store_piece<kOuts, FMT != kFmtE4M3>(out_s, turn_out, lane, w, &ymap, n, row_w, part);
           } else if (a.tile_store && n + kStoreBytes / size <= a.N) {
-            if (live) store_piece_by_lanes(w, reinterpret_cast<uint8_t*>(a.y) + (row * a.ldy + n) * size);
+            if (live) store_piece_by_lanes(w, y + (row * a.ldy + n) * size);
           } else {
-            store_piece_by_rows(out_s, lane, w, reinterpret_cast<uint8_t*>(a.y) + (row_w * a.ldy + n) * size,
-                                a.ldy * size, size, rows_w, min(kStoreBytes / size, a.N - n));
+            store_piece_by_rows(out_s, lane, w, y + (row_w * a.ldy + n) * size, a.ldy * size, size, rows_w,
+                                min(kStoreBytes / size, a.N - n));
           }
         }
       }
@@ -896,7 +926,8 @@ cudaError_t launch_cut(int bn, const ExpertGemmMaps& m, const ExpertGemmArgs& a,
 cudaError_t launch_expert_gemm(int dtype, bool e4m3, int bn, const ExpertGemmMaps& maps,
                                const ExpertGemmArgs& a, int num_sms, cudaStream_t stream, bool pdl) {
   if (bn != 64 && bn != 128 && bn != 256) return cudaErrorInvalidValue;
-  if (a.out == kOutCodes && bn < kFp8Block) return cudaErrorInvalidValue;
+  if (a.out == kOutCodes && (!e4m3 || bn < kFp8Block)) return cudaErrorInvalidValue;
+  if ((a.out == kOutParts || a.x_parts != 1) && e4m3) return cudaErrorInvalidValue;
   if (e4m3)
     return dtype == kF16 ? launch_cut<kFmtE4M3, kF16>(bn, maps, a, num_sms, stream, pdl)
                          : launch_cut<kFmtE4M3, kBF16>(bn, maps, a, num_sms, stream, pdl);
@@ -904,7 +935,7 @@ cudaError_t launch_expert_gemm(int dtype, bool e4m3, int bn, const ExpertGemmMap
                        : launch_cut<kFmtBF16, kBF16>(bn, maps, a, num_sms, stream, pdl);
 }
 
-int plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, int act, int out, int num_sms) {
+int plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, int x_parts, int act, int out, int num_sms) {
   // The cut with the least estimated time, in cycles: the last pass over a tile
   // (activation, codes, stores) and for each wave of tiles the sums of its k
   // blocks, a wave's last pass beside the next wave's sums where two sets of
@@ -924,7 +955,7 @@ int plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, int act, in
   static constexpr Cut kCuts[] = {{64, 515, 480, 4300, 300}, {128, 820, 780, 7400, 600}, {256, 1020, 1140, 9900, 800}};
   constexpr double kMemoryBytes = 18.7;  // a cycle and SM
   constexpr double kActivation = 1.44;   // of SiLU or codes on the last pass
-  const int KB = (K + (e4m3 ? 127 : 63)) / (e4m3 ? 128 : 64);
+  const int KB = (K + (e4m3 ? 127 : 63)) / (e4m3 ? 128 : 64) * x_parts;
   const bool codes = out == kOutCodes;
   // experts that have rows, were the choice of expert even
   const double groups = experts * (1.0 - std::pow(1.0 - 1.0 / experts, rows)), mean = rows / groups;

@@ -12,13 +12,16 @@ namespace cq {
 constexpr int kGemmRows = 128;  // rows of x per CTA
 constexpr int kGemmBoxRows = 32;  // rows of one copy where a tile is not full
 
-// What a value of y becomes: T, f32, or e4m3 codes with their scales.
-enum ExpertOut : int { kOutT = 0, kOutF32 = 1, kOutCodes = 2 };
+// What a value of y becomes: T, f32, e4m3 codes with their scales, or two of T
+// whose sum it is (16-bit weights): the high parts of all rows, and after them
+// what those leave.
+enum ExpertOut : int { kOutT = 0, kOutF32 = 1, kOutCodes = 2, kOutParts = 3 };
 
 struct ExpertGemmArgs {
   const float* x_scales;  // e4m3: [k blocks][rows]
   const float* w_scales;  // e4m3: [experts][n blocks][k blocks]
   const void* bias;       // T [experts][N] or null
+  int x_parts;            // 16-bit: 2 where x comes as kOutParts, else 1
   const int32_t* offsets; // null: all rows meet expert 0
   int offsets_ready;      // the kernel launched before this one began after what wrote the offsets was done
   int rows, experts, N, K, act;
@@ -37,6 +40,7 @@ constexpr int kStoreRows = 32, kStoreBytes = 64;
 // rows; w: [experts * N, K], box 128 bytes x bn rows; all with the
 // 128-byte swizzle.  y: [rows, N] in its own type, box 64 bytes x 32 rows, 64-byte
 // swizzle, used where tile_store says that y's rows allow it (16-byte aligned).
+// With 16-bit weights x, x_part and y have a third dimension, the parts.
 struct ExpertGemmMaps {
   CUtensorMap x, x_part, w, y;
 };
@@ -45,6 +49,6 @@ struct ExpertGemmMaps {
 // plan_expert_gemm returns.
 cudaError_t launch_expert_gemm(int dtype, bool e4m3, int bn, const ExpertGemmMaps& maps, const ExpertGemmArgs& a,
                                int num_sms, cudaStream_t stream, bool pdl);
-int plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, int act, int out, int num_sms);
+int plan_expert_gemm(bool e4m3, int rows, int experts, int N, int K, int x_parts, int act, int out, int num_sms);
 
 }  // namespace cq

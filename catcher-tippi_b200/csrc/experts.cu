@@ -206,6 +206,7 @@ void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, cons
   a.experts = experts_;
   a.N = N_;
   a.K = K_;
+  a.x_parts = x.parts;
   a.act = act;
   a.out = out.kind;
   a.y = out.y;
@@ -213,17 +214,24 @@ void ExpertLinear::product(const Rows& x, int rows, const int32_t* offsets, cons
   a.y_scales = out.scales;
   a.status = ctx.status;
   const bool codes = out.kind == cq::kOutCodes;
-  const int bn = cq::plan_expert_gemm(e4m3(), rows, experts_, N_, K_, act, out.kind, ctx.num_sms);
+  const int bn = cq::plan_expert_gemm(e4m3(), rows, experts_, N_, K_, x.parts, act, out.kind, ctx.num_sms);
   const int size = e4m3() ? 1 : 2, k = 128 / size;
   const int ysize = codes ? 1 : out.kind == cq::kOutF32 ? 4 : 2;
   a.tile_store = out.ld * ysize % 16 == 0 && (reinterpret_cast<uintptr_t>(out.y) & 15) == 0;
   cq::ExpertGemmMaps maps;
-  maps.x = make_map_2d(from, size, rows, K_, ld, cq::kGemmRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
-  maps.x_part = make_map_2d(from, size, rows, K_, ld, cq::kGemmBoxRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
+  // (16-bit: with the parts as a third dimension)
+  const auto rows_map = [&](const void* base, int elem, int parts, int cols, int64_t stride, int box_rows, int box_cols,
+                            CUtensorMapSwizzle swizzle) {
+    return e4m3() ? make_map_2d(base, elem, rows, cols, stride, box_rows, box_cols, swizzle)
+                  : make_map_3d(base, elem, parts, rows, cols, stride, box_rows, box_cols, swizzle);
+  };
+  maps.x = rows_map(from, size, x.parts, K_, ld, cq::kGemmRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
+  maps.x_part = rows_map(from, size, x.parts, K_, ld, cq::kGemmBoxRows, k, CU_TENSOR_MAP_SWIZZLE_128B);
   maps.w = make_map_2d(weight_.get(), size, experts_ * N_, K_, ldw_, bn, k, CU_TENSOR_MAP_SWIZZLE_128B);
   maps.y = !a.tile_store ? maps.x
-                         : make_map_2d(out.y, ysize, rows, codes ? static_cast<int>(out.ld) : N_, out.ld,
-                                       cq::kStoreRows, cq::kStoreBytes / ysize, CU_TENSOR_MAP_SWIZZLE_64B);
+                         : rows_map(out.y, ysize, out.kind == cq::kOutParts ? 2 : 1,
+                                    codes ? static_cast<int>(out.ld) : N_, out.ld, cq::kStoreRows,
+                                    cq::kStoreBytes / ysize, CU_TENSOR_MAP_SWIZZLE_64B);
   check_cuda(cq::launch_expert_gemm(dtype_, e4m3(), bn, maps, a, ctx.num_sms, stream, pdl), "expert product");
 }
 
@@ -349,7 +357,7 @@ struct FfnScratch {
   void* route;
   size_t route_bytes;
   void* x;  // the first product's staging
-  void* h;  // up's result: T, or codes and scales
+  void* h;  // up's result: two parts of T, or codes and scales
   int64_t ld_h;
   float* z;  // f32: the sum over a token's experts is rounded once
 };
@@ -366,7 +374,7 @@ FfnScratch take_ffn(Arena& arena, const ExpertLinear& up, const ExpertLinear& do
   s.route = arena.take<uint8_t>(s.route_bytes);
   s.x = arena.take<uint8_t>(up.staging_bytes(pairs));
   s.ld_h = round_up(up.output_dims(), 8);
-  s.h = arena.take<uint8_t>(up.e4m3() ? down.staging_bytes(pairs) : pairs * s.ld_h * 2);
+  s.h = arena.take<uint8_t>(up.e4m3() ? down.staging_bytes(pairs) : 2 * pairs * s.ld_h * 2);
   s.z = arena.take<float>(pairs * down.output_dims());
   return s;
 }
@@ -413,7 +421,10 @@ void expert_ffn(const ExpertLinear& up, const ExpertLinear& down, const void* x,
   const ExpertLinear::Rows rows{cq::kSourceT, x, ldx, nullptr, s.token, tokens};
   ExpertLinear::Rows h{cq::kSourceT, s.h, s.ld_h, nullptr, nullptr, pairs};
   if (!up.e4m3()) {
-    up.product(rows, pairs, s.offsets, {cq::kOutT, s.h, s.ld_h, nullptr}, act, s.x, stream);
+    // h as the sum of two values of T, so that it keeps twice T's fraction: one
+    // rounding of h to T alone was as large as that of y
+    up.product(rows, pairs, s.offsets, {cq::kOutParts, s.h, s.ld_h, nullptr}, act, s.x, stream);
+    h.parts = 2;
     h.offsets_ready = true;  // a gather and the first product ran since the route
   } else {
     // from f32 sums to codes inside the first product

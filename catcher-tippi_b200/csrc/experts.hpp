@@ -48,6 +48,7 @@ class ExpertLinear {
     const float* scales;
     const int32_t* row_index;
     int x_rows;
+    int parts = 1;  // 2: T as cq::kOutParts made it
     // the kernel that the product follows on the stream began after what wrote
     // the offsets was done (and says so to its dependents only then)
     bool offsets_ready = false;
@@ -56,7 +57,8 @@ class ExpertLinear {
   // tile copies take.
   size_t staging_bytes(int64_t rows) const;
   // What a product makes: a cq::ExpertOut; codes need y_scales [n blocks][rows]
-  // and rows padded to whole blocks, and rows that few_rows() does not take.
+  // and rows padded to whole blocks, and rows that few_rows() does not take; parts
+  // need 2 x rows rows.
   struct Out {
     int kind;
     void* y;

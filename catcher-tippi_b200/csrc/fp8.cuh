@@ -213,4 +213,18 @@ __device__ __forceinline__ uint32_t pack_t(float lo, float hi) {
   }
 }
 
+// Takes what pack_t made of lo and hi from them: 0 is left where that is not finite.
+template <int DT>
+__device__ __forceinline__ void take_rest_t(uint32_t packed, float& lo, float& hi) {
+  float a, b;
+  if constexpr (DT == kBF16) {
+    a = __uint_as_float(packed << 16), b = __uint_as_float(packed & 0xFFFF0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&packed));
+    a = f.x, b = f.y;
+  }
+  lo = fabsf(a) < INFINITY ? lo - a : 0.0f;
+  hi = fabsf(b) < INFINITY ? hi - b : 0.0f;
+}
+
 }  // namespace cq

@@ -147,6 +147,18 @@ CUtensorMap make_map_2d(const void* base, int elem_bytes, int rows, int cols, in
   return encode_map(dt, 2, base, dims, strides, box, swizzle);
 }
 
+CUtensorMap make_map_3d(const void* base, int elem_bytes, int parts, int rows, int cols, int64_t ld,
+                        int box_rows, int box_cols, CUtensorMapSwizzle swizzle) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows),
+                              static_cast<cuuint64_t>(parts)};
+  const cuuint64_t row = static_cast<cuuint64_t>(ld) * elem_bytes;
+  const cuuint64_t strides[2] = {row, row * rows};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1u};
+  const CUtensorMapDataType dt =
+      elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  return encode_map(dt, 3, base, dims, strides, box, swizzle);
+}
+
 cq::GemmActMaps make_act_maps(const void* base, int rows, int K, int ld, int tn) {
   cq::GemmActMaps m{};
   m.tn = tn;

@@ -59,6 +59,11 @@ class DeviceGuard {
 CUtensorMap make_map_2d(const void* base, int elem_bytes, int rows, int cols, int64_t ld,
                         int box_rows, int box_cols, CUtensorMapSwizzle swizzle);
 
+// `parts` such matrices of 2- or 4-byte elements one after another, box
+// [1, box_rows, box_cols].
+CUtensorMap make_map_3d(const void* base, int elem_bytes, int parts, int rows, int cols, int64_t ld,
+                        int box_rows, int box_cols, CUtensorMapSwizzle swizzle);
+
 // The K2 GEMM's activation maps over f16 [rows, K] with row stride ld.
 cq::GemmActMaps make_act_maps(const void* base, int rows, int K, int ld, int tn);
 

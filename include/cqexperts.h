@@ -113,8 +113,8 @@ size_t cq_expert_ffn_workspace(const cq_expert_linear *up, const cq_expert_linea
  * format, dtype and device; down's input is up's output and y has down's width.
  * x T [tokens, ldx], logits of logits_dtype [tokens, ld_logits], y T [tokens,
  * ldy]; y is zero for a token without an expert.  With e4m3 weights h goes
- * from f32 to e4m3 at once; with 16-bit weights it is rounded to T.  z stays in
- * f32.
+ * from f32 to e4m3 at once; with 16-bit weights it is the sum of two values of
+ * T, which keeps twice T's fraction (and T's range).  z stays in f32.
  */
 cq_status cq_expert_ffn_forward(cq_expert_linear *up, cq_expert_linear *down, const void *x,
                                 int64_t ldx, int32_t tokens, const void *logits, int64_t ld_logits,

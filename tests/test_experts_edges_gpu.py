@@ -90,3 +90,69 @@ def test_a_masked_value_of_h_leaves_its_block(cq, tokens):
     bound = (2.0 ** -4 + 2.0 ** -10) * np.abs(h) + scale * 2.0 ** -10 * (1 + 2.0 ** -10)
     for t in range(tokens):
         assert (np.abs(y[t] - h[t % E]) <= bound[t % E]).all()
+
+
+# ------------------------------------------------------------------ the 16-bit feed-forward module
+
+def module16(gen, dtype, E, d, ff, out, bias=True):
+    from nemotron_cuda import experts
+    w1, w2 = (values(gen, E, n, k, dtype=dtype, spread=0.2) / k ** 0.5 for n, k in ((ff, d), (out, ff)))
+    b1, b2 = (values(gen, E, n, dtype=dtype, spread=0.2) if bias else None for n in (ff, out))
+    return (experts.ExpertLinear.from_weight(w1, b1), experts.ExpertLinear.from_weight(w2, b2)), (w1, w2, b1, b2)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("tokens,E,top,d,ff,out,act", [
+    (1, 8, 2, 792, 1567, 792, "silu"), (14, 4, 2, 128, 64, 72, "relu"), (60, 3, 3, 200, 333, 104, "none"),
+    (300, 5, 2, 256, 1024, 256, "silu"), (900, 4, 2, 384, 2048, 512, "silu"), (3000, 3, 1, 136, 200, 1000, "relu")])
+def test_h_keeps_more_than_its_type(cq, dtype, tokens, E, top, d, ff, out, act):
+    """y is the definition's value rounded once.  h is held to 2^-17 (bf16) or 2^-22 (f16) of each value and the sums in f32
+    lose less, so y before its rounding is off by a small part of a step and few of its values come out at the
+    neighbour: their share is about twice that part, under 2^-6.  Bound: 2^-4.  With h rounded to T it would be near a half."""
+    from nemotron_cuda import experts
+    gen = rng_of("h", tokens, ff)
+    (up, down), (w1, w2, b1, b2) = module16(gen, dtype, E, d, ff, out)
+    x, z = values(gen, tokens, d, dtype=dtype, spread=0.3), torch.randn(tokens, E, device="cuda", generator=gen)
+    y = experts.ExpertFeedForward(up, down, top=top, act=act).forward(x, z)
+    expert, weight, offsets, token, position = eo.route(f64(z), top)
+    h, _ = eo.experts(f64(x)[token], f64(w1), offsets, f64(b1), act)
+    rows, _ = eo.experts(h, f64(w2), offsets, f64(b2))
+    want, _ = eo.combine(rows, position, weight)
+    want = torch.from_numpy(want).to(TYPES[dtype]).to("cuda")
+    assert y.isfinite().all()
+    assert (y != want).float().mean().item() <= 2.0 ** -4
+
+
+def test_h_past_the_range_of_its_type(cq):
+    """A value of h past f16's range is infinite, as a rounded one would be; the other tokens keep theirs."""
+    from nemotron_cuda import experts
+    up = experts.ExpertLinear.from_weight(torch.full((1, 1, 1), 300.0, dtype=torch.float16, device="cuda"))
+    down = experts.ExpertLinear.from_weight(torch.full((1, 1, 1), 0.25, dtype=torch.float16, device="cuda"))
+    x = torch.tensor([[2.0], [300.0], [-300.0], [1.5]], dtype=torch.float16, device="cuda")
+    y = experts.ExpertFeedForward(up, down, top=1, act="none").forward(x, torch.zeros(4, 1, device="cuda"))
+    assert y.flatten().tolist() == [150.0, float("inf"), -float("inf"), 112.5]
+
+
+@pytest.mark.parametrize("weights", ["16bit", "e4m3"])
+@pytest.mark.parametrize("tokens", [6, 300])
+def test_tokens_that_are_not_finite_stay_apart(cq, weights, tokens):
+    """Infinities and NaN in one token reach no other: of the module, and of its first linear alone."""
+    from nemotron_cuda import experts
+    gen = rng_of("apart", tokens)
+    E, d, ff = 4, 200, 328
+    if weights == "16bit":
+        (up, down), _ = module16(gen, "bf16", E, d, ff, d)
+    else:
+        up, down = (experts.ExpertLinear.from_codes(codes_of(gen, E, n, k), scales_of(gen, E, -(-n // 128), -(-k // 128)) / k ** 0.5)
+                    for n, k in ((ff, d), (d, ff)))
+    module = experts.ExpertFeedForward(up, down, top=2)
+    x, z = values(gen, tokens, d, spread=0.3), torch.randn(tokens, E, device="cuda", generator=gen)
+    r = experts.route(z, 2)
+    clean, rows = module.forward(x, z), up.forward(x[r.token.long()], r.offsets, act="silu")
+    bad = torch.zeros(tokens, dtype=torch.bool, device="cuda")
+    bad[1] = bad[4] = True
+    x[1, 7], x[4, 3], x[4, 150] = float("inf"), float("nan"), -float("inf")
+    y, y_rows = module.forward(x, z), up.forward(x[r.token.long()], r.offsets, act="silu")
+    assert torch.equal(y[~bad], clean[~bad]) and not y[bad].isfinite().any(1).all()
+    assert torch.equal(y_rows[~bad[r.token.long()]], rows[~bad[r.token.long()]])
+    assert y_rows[r.token == 4].isnan().all()
