@@ -660,14 +660,17 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
       }
     }
 
+    // A warp whose wait ran out (ok false) waits, sums and stores no more, but it
+    // goes through all of its tiles: the others may have seen that phase complete
+    // just in time, and meet it at the named barriers of every tile.
     int e = 0;
-    for (int t = worker + set * workers, seq = set; t < total && ok; t += kSets * workers, seq += kSets) {
+    for (int t = worker + set * workers, seq = set; t < total; t += kSets * workers, seq += kSets) {
       const Tile tile = find_tile(list, t, kGemmRows, tiles_n, BN, e);
       Ring ring(seq * tile_groups, kGroups), scales(seq * tile_slots, kScaleSlots);
       // The sets' sums follow one another: a set that waited for its accumulators
       // while the other's are still to come would take a phase of theirs, of the
       // same parity, for its own.
-      if (kSets == 2 && seq > 0) ok = wait_phase(token + set * 8, ((seq - 1) / 2) & 1, a.status);
+      if (kSets == 2 && seq > 0) ok = ok && wait_phase(token + set * 8, ((seq - 1) / 2) & 1, a.status);
       const int64_t row = tile.m0 + local;
       const bool live = row < tile.end;
       const int row_w = tile.m0 + quarter * 32;  // the warp's first row
@@ -689,12 +692,14 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
       if constexpr (FMT == kFmtE4M3) {
         for (int kb = 0; kb < KB; kb += kScaleBlocks) {
           ok = ok && wait_phase(scale_full + scales.at * 8, scales.phase, a.status);
+          if (!ok) break;
           const float* sx = scale_x + scales.at * kScaleBlocks * kGemmRows + local;
           const float* sw = scale_w + scales.at * 2 * kScaleBlocks + half;
           const int blocks = min(kScaleBlocks, KB - kb);
 #pragma unroll 1
           for (int i = 0; i < blocks; i += kPer) {
-            ok = ok && wait_phase(acc_full + ring.at * 8, ring.phase, a.status);
+            ok = wait_phase(acc_full + ring.at * 8, ring.phase, a.status);
+            if (!ok) break;
             tc_fence_after();
             const uint32_t src = lane_base + static_cast<uint32_t>(ring.at * kGroupCols);
             if (idle) {
@@ -733,6 +738,7 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
             }
             ring.next(kGroups);
           }
+          if (!ok) break;
           __syncwarp();
           if (lane == 0) arrive(scale_empty + scales.at * 8);
           scales.next(kScaleSlots);
@@ -741,8 +747,8 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
         ok = ok && wait_phase(acc_full + ring.at * 8, ring.phase, a.status);
         tc_fence_after();
       }
-      if (!ok) break;
-      if (kSets == 2 && lane == 0) arrive(token + (set ^ 1) * 8);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (kSets == 2 && ok && lane == 0) arrive(token + (set ^ 1) * 8);
 
       const uint32_t src = lane_base + static_cast<uint32_t>(ring.at * kGroupCols);
       const auto take = [&](int c, float(&v)[32]) {
@@ -788,7 +794,7 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
           // a row's block of 128 columns is one thread's, or two threads' halves:
           // its largest finite magnitude, then the codes (infinities made NaN)
           uint32_t top = 0;
-          if (!idle && n0 < a.N) {
+          if (ok && !idle && n0 < a.N) {
             float most = 0.0f;
 #pragma unroll
             for (int c = 0; c < W; c += 32) {
@@ -823,7 +829,7 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
             top = max(top, top_s[turn][set * 2 + (half ^ 1)][local]);
             turn ^= 1;
           }
-          if (idle || n0 >= a.N) continue;
+          if (!ok || idle || n0 >= a.N) continue;
           const int ex = fp8_scale_exponent(top);
           const float inv = pow2f(-ex);
           if (live && n0 % kFp8Block == 0) a.y_scales[static_cast<int64_t>(n0 / kFp8Block) * a.rows + row] = pow2f(ex);
@@ -844,6 +850,7 @@ __global__ void __launch_bounds__(gemm_threads(BN), 1)
           continue;
         }
       }
+      if (!ok) continue;
       if (idle || n0 >= a.N) {
         if constexpr (FMT != kFmtE4M3) {
           if (lane == 0) hand_back(ring.at);
