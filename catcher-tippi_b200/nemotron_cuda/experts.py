@@ -14,7 +14,8 @@ from typing import NamedTuple
 import torch
 
 from . import ACTS, DTYPES, _check, _ptr, lib
-from .fp8 import CODES, SIZE_MAX, TYPES, _allocating, _bytes, _Layer, _packed, _refuse, _rows_of, _stream_of, blocks
+from .fp8 import (CODES, SIZE_MAX, T_NAMES, TYPES, _allocating, _Layer, _packed, _refuse, _rows_of, _stream_of, _typed,
+                  blocks)
 
 FORMATS = {"16bit": 0, "e4m3": 1}
 
@@ -101,8 +102,8 @@ class ExpertLinear(_Layer):
     @classmethod
     def _create(cls, weight, scales, bias, format: str, dtype: str, device: int) -> "ExpertLinear":
         e, n, k = weight.shape
-        if bias is not None and _bytes(bias) != 2:
-            _refuse("the bias must be of the layer's 16-bit type")
+        if bias is not None:
+            _typed(bias, T_NAMES.get(dtype, dtype), "the bias")
         w, b = _packed(weight, e, n, k), None if bias is None else _packed(bias, e, n)
         s = None if scales is None else _packed(scales, e, blocks(n), blocks(k))
         h = ctypes.c_void_p()
@@ -121,8 +122,8 @@ class ExpertLinear(_Layer):
     @classmethod
     def from_codes(cls, codes, scales, bias=None, dtype: str = "bf16", device: int = 0) -> "ExpertLinear":
         """e4m3 codes [experts, N, K], scales f32 [experts, ceil(N / 128), ceil(K / 128)], bias T [experts, N] or None."""
-        if _bytes(codes) != 1 or _bytes(scales) != 4:
-            _refuse("codes must have one byte each and scales must be f32")
+        _typed(codes, "codes", "an array of codes")
+        _typed(scales, "float32", "an array of scales")
         return cls._create(codes, scales, bias, "e4m3", dtype, device)
 
     def forward(self, x, offsets, y=None, act: str = "none", stream=None):

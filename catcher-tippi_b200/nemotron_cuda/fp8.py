@@ -55,8 +55,21 @@ def _packed(a, *shape):
     return _contiguous(a)
 
 
-def _bytes(a) -> int:
-    return a.itemsize if isinstance(a, np.ndarray) else a.element_size()
+def _typed(a, name: str, what: str):
+    """Refuses an array argument of a layer whose type is not `name`: its bits would be read as another's."""
+    kind = a.dtype.name if isinstance(a, np.ndarray) else str(a.dtype).removeprefix("torch.")
+    if name == "codes":
+        fits = kind in ("uint8", "float8_e4m3fn")
+    elif isinstance(a, np.ndarray) and name in ("float16", "bfloat16"):
+        # numpy holds bf16, which it lacks, as raw 16-bit values
+        fits = a.itemsize == 2 and kind in (name, "uint16", "int16")
+    else:
+        fits = kind == name
+    if not fits:
+        _refuse(f"{what} has type {kind}, expected {'uint8 or float8_e4m3fn' if name == 'codes' else name}")
+
+
+T_NAMES = {"f16": "float16", "bf16": "bfloat16"}
 
 
 def blocks(n: int) -> int:
@@ -131,10 +144,10 @@ class Fp8Linear(_Layer):
         """codes [N, K] of one byte (torch float8_e4m3fn or uint8, or numpy uint8), scales f32
         [ceil(N / 128), ceil(K / 128)], bias T [N] or None; host or device arrays."""
         n, k = codes.shape
-        if _bytes(codes) != 1:
-            _refuse("codes must have one byte each")
-        if _bytes(scales) != 4 or (bias is not None and _bytes(bias) != 2):
-            _refuse("scales must be f32 and the bias of the layer's 16-bit type")
+        _typed(codes, "codes", "an array of codes")
+        _typed(scales, "float32", "an array of scales")
+        if bias is not None:
+            _typed(bias, T_NAMES.get(dtype, dtype), "the bias")
         c, s = _packed(codes, n, k), _packed(scales, blocks(n), blocks(k))
         b = None if bias is None else _packed(bias, n)
         h = ctypes.c_void_p()
@@ -145,8 +158,9 @@ class Fp8Linear(_Layer):
     def from_f32(cls, weight, bias=None, dtype: str = "bf16", device: int = 0) -> "Fp8Linear":
         """An f32 weight [N, K] and bias [N] (numpy or torch, host or device), brought to e4m3 on the device."""
         n, k = weight.shape
-        if _bytes(weight) != 4 or (bias is not None and _bytes(bias) != 4):
-            _refuse("weight and bias must be f32")
+        _typed(weight, "float32", "the weight")
+        if bias is not None:
+            _typed(bias, "float32", "the bias")
         w, b = _contiguous(weight), None if bias is None else _packed(bias, n)
         h = ctypes.c_void_p()
         _check(lib().cq_fp8_linear_create_from_f32(_ptr(w), _ptr(b), n, k, DTYPES[dtype], device, ctypes.byref(h)))
@@ -168,7 +182,9 @@ class Fp8Linear(_Layer):
         if codes.device != self._device or scales.device != self._device:
             _refuse(f"codes and scales must be on {self._device}")
         rows = codes.shape[0]
-        if codes.dim() != 2 or codes.shape[1] < self.input_dims or codes.stride(1) != 1 or _bytes(codes) != 1:
+        if codes.dtype is not torch.float8_e4m3fn and codes.dtype is not torch.uint8:
+            _refuse(f"codes have type {codes.dtype}, expected uint8 or float8_e4m3fn")
+        if codes.dim() != 2 or codes.shape[1] < self.input_dims or codes.stride(1) != 1:
             _refuse(f"codes must be rows of at least {self.input_dims} bytes, got shape {tuple(codes.shape)}")
         if scales.dtype != torch.float32 or tuple(scales.shape) != (blocks(self.input_dims), rows) or \
                 not scales.is_contiguous():
