@@ -14,7 +14,7 @@ from typing import NamedTuple
 import torch
 
 from . import ACTS, DTYPES, _check, _ptr, lib
-from .fp8 import (CODES, SIZE_MAX, T_NAMES, TYPES, _allocating, _Layer, _packed, _refuse, _rows_of, _stream_of, _typed,
+from .fp8 import (CODES, SIZE_MAX, T_NAMES, TYPES, _allocating, _check_output, _Layer, _packed, _refuse, _rows_of, _stream_of, _typed,
                   blocks)
 
 FORMATS = {"16bit": 0, "e4m3": 1}
@@ -82,9 +82,8 @@ def combine(z, position, weight, y=None, stream=None):
     if y is None:
         with _allocating(stream, z.device):
             y = z.new_empty((tokens, dims))
-    elif y.dtype != z.dtype or y.shape[0] != tokens:
-        _refuse(f"output must be {z.dtype} with {tokens} rows")
-    _rows_of(y, dims, "output")
+    else:
+        _check_output(y, z.dtype, tokens, dims, z.device)
     _check(lib().cq_expert_combine(z.data_ptr(), z.stride(0), rows, position.data_ptr(), weight.data_ptr(), tokens,
                                    top, dims, kind, y.data_ptr(), y.stride(0), _stream_of(stream, z.device)))
     return y

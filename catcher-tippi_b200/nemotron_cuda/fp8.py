@@ -84,6 +84,15 @@ def _rows_of(x, dims: int, what: str = "input"):
                 f"with strides {tuple(x.stride())}")
 
 
+def _check_output(y, dtype, rows: int, dims: int, device):
+    """Refuses a caller's output that the call could not write."""
+    if y.dtype != dtype or y.shape[0] != rows:
+        _refuse(f"output must be {dtype} with {rows} rows")
+    _rows_of(y, dims, "output")
+    if y.device != device:
+        _refuse(f"output is on {y.device}, the input on {device}")
+
+
 class _Layer:
     """A handle of the library and what its calls need to know."""
 
@@ -105,9 +114,7 @@ class _Layer:
             _refuse(f"input has type {x.dtype}, expected {self._type}")
         if y is None:
             return x.new_empty((x.shape[0], self.output_dims))
-        if y.dtype != self._type or y.shape[0] != x.shape[0]:
-            _refuse(f"output must be {self._type} with {x.shape[0]} rows")
-        _rows_of(y, self.output_dims, "output")
+        _check_output(y, self._type, x.shape[0], self.output_dims, x.device)
         return y
 
     def _workspace(self, entry, rows: int):
@@ -192,9 +199,8 @@ class Fp8Linear(_Layer):
         if y is None:
             with _allocating(stream, codes.device):
                 y = torch.empty((rows, self.output_dims), dtype=self._type, device=codes.device)
-        elif y.dtype != self._type or y.shape[0] != rows:
-            _refuse(f"output must be {self._type} with {rows} rows")
-        _rows_of(y, self.output_dims, "output")
+        else:
+            _check_output(y, self._type, rows, self.output_dims, codes.device)
         _check(lib().cq_fp8_linear_forward_codes(self._h, codes.data_ptr(), codes.stride(0), scales.data_ptr(), rows,
                                                  y.data_ptr(), y.stride(0), ACTS[act],
                                                  _stream_of(stream, codes.device)))

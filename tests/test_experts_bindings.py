@@ -54,3 +54,106 @@ def test_arrays_of_the_layer_s_types_reach_the_library(bias, monkeypatch):
         with pytest.raises(CQError, match="reached"):
             fp8.Fp8Linear.from_codes(codes, SCALES, bias, dtype="bf16")
     assert len(reached) == 3
+
+
+# ------------------------------------------------------------------ calls, on stand-ins for device tensors
+
+EMPTY = torch.empty
+
+
+class Rows:
+    """What the bindings ask of a device tensor."""
+
+    def __init__(self, *shape, dtype=torch.bfloat16, device=0, strides=None, requires_grad=False):
+        self.shape, self.dtype, self.device = torch.Size(shape), dtype, torch.device("cuda", device)
+        self.strides = strides or EMPTY(shape, device="meta").stride()
+        self.is_cuda, self.requires_grad = True, requires_grad
+
+    def dim(self):
+        return len(self.shape)
+
+    def stride(self, i=None):
+        return self.strides if i is None else self.strides[i]
+
+    def is_contiguous(self):
+        return EMPTY(self.shape, device="meta").as_strided(self.shape, self.strides).is_contiguous()
+
+    def element_size(self):
+        return self.dtype.itemsize
+
+    def data_ptr(self):
+        return 1 << 20
+
+    def new_empty(self, shape, dtype=None):
+        return Rows(*([shape] if isinstance(shape, int) else shape), dtype=dtype or self.dtype, device=self.device.index)
+
+    def as_strided(self, shape, strides, offset):
+        return Rows(*shape, dtype=self.dtype, strides=strides)
+
+    def view(self, dtype):
+        return Rows(*self.shape, dtype=dtype, strides=self.strides)
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The library as a list of the calls that reach it, each of which succeeds."""
+    seen = []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: seen.append((name, args)) or 0
+
+    for module in (fp8, experts):
+        monkeypatch.setattr(module, "lib", Library)
+    monkeypatch.setattr(fp8, "_raw_stream", lambda index: 77)
+    monkeypatch.setattr(torch, "empty", lambda shape, dtype, device: Rows(*([shape] if isinstance(shape, int) else shape), dtype=dtype))
+    experts._route_workspace.cache_clear()
+    yield seen
+    experts._route_workspace.cache_clear()
+
+
+def layer():
+    return fp8.Fp8Linear(None, 1, 8, 16, "bf16", 0)
+
+
+def expert_layer(n=8, k=16):
+    return experts.ExpertLinear(None, 2, n, k, "bf16", 0, format="e4m3")
+
+
+OFFSETS = Rows(3, dtype=torch.int32)
+PAIRS = dict(position=Rows(4, 2, dtype=torch.int32), weight=Rows(4, 2, dtype=torch.float32))
+
+
+def every_call(x=None, y=None, stream=None):
+    """Each call that takes rows, of 16 values and (combine's) of 8, with an output of 8."""
+    up, down = expert_layer(32, 16), expert_layer(8, 32)
+    x = x or Rows(4, 16)
+    yield lambda: layer().forward(x, y=y, stream=stream)
+    yield lambda: expert_layer().forward(x, OFFSETS, y=y, stream=stream)
+    yield lambda: experts.ExpertFeedForward(up, down, 2).forward(x, Rows(x.shape[0], 2, dtype=torch.float32), y=y, stream=stream)
+
+
+def codes_call(y=None, stream=None):
+    return layer().forward_codes(Rows(4, 128, dtype=torch.uint8), Rows(1, 4, dtype=torch.float32), y=y, stream=stream)
+
+
+def combine_call(y=None, stream=None):
+    return experts.combine(Rows(8, 8), **PAIRS, y=y, stream=stream)
+
+
+def test_calls_reach_the_library(calls):
+    y = Rows(4, 8)
+    for call in (*every_call(y=y), lambda: codes_call(y), lambda: combine_call(y)):
+        calls.clear()
+        assert call() is y
+        assert calls[-1][0].startswith("cq_")
+
+
+def test_an_output_on_another_device_is_refused(calls):
+    """It would be written as if it were local."""
+    y = Rows(4, 8, device=1)
+    for call in (*every_call(y=y), lambda: codes_call(y), lambda: combine_call(y)):
+        calls.clear()
+        with pytest.raises(CQError, match="output is on cuda:1, the input on cuda:0"):
+            call()
+        assert not any("forward" in name or "combine" in name for name, _ in calls)
