@@ -19,7 +19,8 @@ TYPES = {torch.float16: "f16", torch.bfloat16: "bf16", torch.float32: "f32"}
 # dtype -> the library's code, for the calls
 CODES = {t: DTYPES[name] for t, name in TYPES.items()}
 SIZE_MAX = ctypes.c_size_t(-1).value
-# the stream as a number, without building torch's Stream object (2 us a call)
+# the stream as a number, without building torch's Stream object (2 us a call); a
+# private name, which a torch may lack
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
@@ -29,7 +30,7 @@ def _refuse(message: str):
 
 def _stream_of(stream, device) -> int:
     if stream is None:
-        return _raw_stream(device.index)
+        return _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 

@@ -157,3 +157,17 @@ def test_an_output_on_another_device_is_refused(calls):
         with pytest.raises(CQError, match="output is on cuda:1, the input on cuda:0"):
             call()
         assert not any("forward" in name or "combine" in name for name, _ in calls)
+
+
+# ------------------------------------------------------------------ streams
+
+class OnStream:
+    cuda_stream = 99
+
+
+def test_the_current_stream_without_torch_s_short_way_to_it(calls, monkeypatch):
+    monkeypatch.setattr(fp8, "_raw_stream", None)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: OnStream)
+    for call in (*every_call(), codes_call, combine_call, lambda: experts.route(Rows(4, 8), 2), lambda: fp8.quantize_rows(Rows(4, 8))):
+        call()
+        assert calls[-1][1][-1] == 99
