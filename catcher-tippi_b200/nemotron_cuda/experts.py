@@ -14,7 +14,7 @@ from typing import NamedTuple
 import torch
 
 from . import ACTS, DTYPES, _check, _ptr, lib
-from .fp8 import (CODES, SIZE_MAX, T_NAMES, TYPES, _allocating, _check_output, _Layer, _packed, _refuse, _rows_of, _stream_of, _typed,
+from .fp8 import (CODES, SIZE_MAX, T_NAMES, TYPES, _allocating, _check_output, _Layer, _ld, _packed, _refuse, _rows_of, _stream_of, _typed,
                   blocks)
 
 FORMATS = {"16bit": 0, "e4m3": 1}
@@ -55,7 +55,7 @@ def route(logits, top: int, renormalize: bool = True, stream=None) -> Route:
     with _allocating(stream, device):
         ints = logits.new_empty(end + n // 4, dtype=torch.int32)
         at = ints.data_ptr()
-        _check(L.cq_route(logits.data_ptr(), logits.stride(0), kind, tokens, experts, top, int(renormalize), at, at + 4 * step,
+        _check(L.cq_route(logits.data_ptr(), _ld(logits), kind, tokens, experts, top, int(renormalize), at, at + 4 * step,
                           at + 16 * step, at + 12 * step, at + 8 * step, at + 4 * end if n else None, n,
                           _stream_of(stream, device)))
     pairs, across = (tokens, top), (top, 1)
@@ -84,8 +84,8 @@ def combine(z, position, weight, y=None, stream=None):
             y = z.new_empty((tokens, dims))
     else:
         _check_output(y, z.dtype, tokens, dims, z.device)
-    _check(lib().cq_expert_combine(z.data_ptr(), z.stride(0), rows, position.data_ptr(), weight.data_ptr(), tokens,
-                                   top, dims, kind, y.data_ptr(), y.stride(0), _stream_of(stream, z.device)))
+    _check(lib().cq_expert_combine(z.data_ptr(), _ld(z), rows, position.data_ptr(), weight.data_ptr(), tokens,
+                                   top, dims, kind, y.data_ptr(), _ld(y), _stream_of(stream, z.device)))
     return y
 
 
@@ -136,8 +136,8 @@ class ExpertLinear(_Layer):
         with _allocating(stream, x.device):
             y = self._output(x, y)
             keep, ws, n = self._workspace(L.cq_expert_linear_workspace, x.shape[0])
-            _check(L.cq_expert_linear_forward(self._h, x.data_ptr(), x.stride(0), x.shape[0], offsets.data_ptr(),
-                                              y.data_ptr(), y.stride(0), ACTS[act], ws, n,
+            _check(L.cq_expert_linear_forward(self._h, x.data_ptr(), _ld(x), x.shape[0], offsets.data_ptr(),
+                                              y.data_ptr(), _ld(y), ACTS[act], ws, n,
                                               _stream_of(stream, x.device)))
         return y
 
@@ -178,8 +178,8 @@ class ExpertFeedForward:
         with _allocating(stream, x.device):
             y = down._output(x, y)
             ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-            _check(lib().cq_expert_ffn_forward(up._h, down._h, x.data_ptr(), x.stride(0), tokens, logits.data_ptr(),
-                                               logits.stride(0), kind, self.top, int(self.renormalize),
-                                               ACTS[self.act], y.data_ptr(), y.stride(0), ws.data_ptr(), n,
+            _check(lib().cq_expert_ffn_forward(up._h, down._h, x.data_ptr(), _ld(x), tokens, logits.data_ptr(),
+                                               _ld(logits), kind, self.top, int(self.renormalize),
+                                               ACTS[self.act], y.data_ptr(), _ld(y), ws.data_ptr(), n,
                                                _stream_of(stream, x.device)))
         return y

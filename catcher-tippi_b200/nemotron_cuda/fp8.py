@@ -85,6 +85,11 @@ def _rows_of(x, dims: int, what: str = "input"):
                 f"with strides {tuple(x.stride())}")
 
 
+def _ld(x) -> int:
+    """The row stride for the library; that of a single row may be anything in torch (a transposed column has 1)."""
+    return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
+
+
 def _check_output(y, dtype, rows: int, dims: int, device):
     """Refuses a caller's output that the call could not write."""
     if y.dtype != dtype or y.shape[0] != rows:
@@ -181,7 +186,7 @@ class Fp8Linear(_Layer):
         with _allocating(stream, x.device):
             y = self._output(x, y)
             keep, ws, n = self._workspace(L.cq_fp8_linear_workspace, x.shape[0])
-            _check(L.cq_fp8_linear_forward(self._h, x.data_ptr(), x.stride(0), x.shape[0], y.data_ptr(), y.stride(0),
+            _check(L.cq_fp8_linear_forward(self._h, x.data_ptr(), _ld(x), x.shape[0], y.data_ptr(), _ld(y),
                                            ACTS[act], ws, n, _stream_of(stream, x.device)))
         return y
 
@@ -202,8 +207,8 @@ class Fp8Linear(_Layer):
                 y = torch.empty((rows, self.output_dims), dtype=self._type, device=codes.device)
         else:
             _check_output(y, self._type, rows, self.output_dims, codes.device)
-        _check(lib().cq_fp8_linear_forward_codes(self._h, codes.data_ptr(), codes.stride(0), scales.data_ptr(), rows,
-                                                 y.data_ptr(), y.stride(0), ACTS[act],
+        _check(lib().cq_fp8_linear_forward_codes(self._h, codes.data_ptr(), _ld(codes), scales.data_ptr(), rows,
+                                                 y.data_ptr(), _ld(y), ACTS[act],
                                                  _stream_of(stream, codes.device)))
         return y
 
@@ -220,8 +225,8 @@ def quantize_rows(x, stream=None):
     with _allocating(stream, x.device):
         codes = torch.empty((rows, BLOCK * blocks(k)), dtype=torch.float8_e4m3fn, device=x.device)
         scales = torch.empty((blocks(k), rows), dtype=torch.float32, device=x.device)
-    _check(lib().cq_fp8_quantize_rows(x.data_ptr(), x.stride(0), rows, k, DTYPES[kind], codes.data_ptr(),
-                                      codes.stride(0), scales.data_ptr(), _stream_of(stream, x.device)))
+    _check(lib().cq_fp8_quantize_rows(x.data_ptr(), _ld(x), rows, k, DTYPES[kind], codes.data_ptr(),
+                                      _ld(codes), scales.data_ptr(), _stream_of(stream, x.device)))
     return codes, scales
 
 

@@ -171,3 +171,26 @@ def test_the_current_stream_without_torch_s_short_way_to_it(calls, monkeypatch):
     for call in (*every_call(), codes_call, combine_call, lambda: experts.route(Rows(4, 8), 2), lambda: fp8.quantize_rows(Rows(4, 8))):
         call()
         assert calls[-1][1][-1] == 99
+
+
+# ------------------------------------------------------------------ strides
+
+def test_a_single_row_may_have_any_row_stride(calls):
+    """A transposed column is one row of neighbours with a row stride of 1; the library wants at least the width."""
+    x, y = Rows(1, 16, strides=(1, 1)), Rows(1, 8, strides=(1, 1))
+    for call, (of_x, of_y) in zip(every_call(x, y), ((2, 5), (2, 6), (3, 12))):
+        call()
+        assert calls[-1][1][of_x] == 16 and calls[-1][1][of_y] == 8
+    layer().forward_codes(Rows(1, 128, dtype=torch.uint8, strides=(1, 1)), Rows(1, 1, dtype=torch.float32), y=y)
+    assert calls[-1][1][2] == 128 and calls[-1][1][6] == 8
+    experts.combine(Rows(1, 8, strides=(1, 1)), Rows(1, 2, dtype=torch.int32), Rows(1, 2, dtype=torch.float32), y=y)
+    assert calls[-1][1][1] == 8 and calls[-1][1][10] == 8
+    experts.route(Rows(1, 8, strides=(1, 1)), 2)
+    assert calls[-1][1][1] == 8
+    fp8.quantize_rows(Rows(1, 8, strides=(1, 1)))
+    assert calls[-1][1][1] == 8
+    # wider strides stay, as do those of more rows
+    layer().forward(Rows(1, 16, strides=(24, 1)), y=Rows(1, 8, strides=(32, 1)))
+    assert calls[-1][1][2] == 24 and calls[-1][1][5] == 32
+    layer().forward(Rows(3, 16, strides=(20, 1)), y=Rows(3, 8, strides=(9, 1)))
+    assert calls[-1][1][2] == 20 and calls[-1][1][5] == 9
