@@ -3,7 +3,9 @@
 ``route`` chooses each token's experts and orders the (token, expert) pairs by
 expert, ``ExpertLinear`` multiplies rows so ordered by the weights of their
 expert, ``combine`` sums what each token's experts made, and
-``ExpertFeedForward`` is the feed-forward module of the four steps.
+``ExpertFeedForward`` is the feed-forward module of the four steps.  There is no
+backward pass: tensors that require a gradient are refused outside
+torch.no_grad().
 """
 from __future__ import annotations
 
@@ -14,7 +16,7 @@ from typing import NamedTuple
 import torch
 
 from . import ACTS, DTYPES, _check, _ptr, lib
-from .fp8 import (CODES, SIZE_MAX, T_NAMES, TYPES, _allocating, _check_output, _Layer, _ld, _packed, _refuse, _rows_of, _stream_of, _typed,
+from .fp8 import (CODES, SIZE_MAX, T_NAMES, TYPES, _allocating, _check_output, _Layer, _ld, _no_gradient, _packed, _refuse, _rows_of, _stream_of, _typed,
                   blocks)
 
 FORMATS = {"16bit": 0, "e4m3": 1}
@@ -79,6 +81,7 @@ def combine(z, position, weight, y=None, stream=None):
     if position.dtype != torch.int32 or weight.dtype != torch.float32 or not position.is_contiguous() or \
             not weight.is_contiguous() or position.device != z.device or weight.device != z.device:
         _refuse("positions must be int32 and weights f32, without gaps, on the device of the rows")
+    _no_gradient(weight, "an array of weights")
     if y is None:
         with _allocating(stream, z.device):
             y = z.new_empty((tokens, dims))

@@ -2,7 +2,8 @@
 
 ``Fp8Linear`` holds e4m3 weights with an f32 scale for each 128 x 128 block;
 ``forward`` brings the rows of x to e4m3 (a power-of-two scale for each 128
-values), multiplies and applies bias and activation in f32.
+values), multiplies and applies bias and activation in f32.  There is no backward
+pass: rows that require a gradient are refused outside torch.no_grad().
 """
 from __future__ import annotations
 
@@ -77,9 +78,16 @@ def blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
+def _no_gradient(x, what: str):
+    """Refuses what autograd follows: these operators have no backward pass, and the result would silently have none."""
+    if x.requires_grad and torch.is_grad_enabled():
+        _refuse(f"{what} requires a gradient, and there is no backward pass: call under torch.no_grad() or detach it")
+
+
 def _rows_of(x, dims: int, what: str = "input"):
     if not x.is_cuda:
         _refuse(f"{what} must be on the device, got {x.device}")
+    _no_gradient(x, what)
     if x.dim() != 2 or x.shape[1] != dims or (dims > 1 and x.stride(1) != 1):
         _refuse(f"{what} must be rows of {dims} values next to each other, got shape {tuple(x.shape)} "
                 f"with strides {tuple(x.stride())}")
@@ -202,6 +210,7 @@ class Fp8Linear(_Layer):
         if scales.dtype != torch.float32 or tuple(scales.shape) != (blocks(self.input_dims), rows) or \
                 not scales.is_contiguous():
             _refuse(f"scales must be f32 [{blocks(self.input_dims)}, {rows}] without gaps")
+        _no_gradient(scales, "an array of scales")
         if y is None:
             with _allocating(stream, codes.device):
                 y = torch.empty((rows, self.output_dims), dtype=self._type, device=codes.device)

@@ -194,3 +194,31 @@ def test_a_single_row_may_have_any_row_stride(calls):
     assert calls[-1][1][2] == 24 and calls[-1][1][5] == 32
     layer().forward(Rows(3, 16, strides=(20, 1)), y=Rows(3, 8, strides=(9, 1)))
     assert calls[-1][1][2] == 20 and calls[-1][1][5] == 9
+
+
+# ------------------------------------------------------------------ gradients
+
+def test_rows_that_require_a_gradient_are_refused(calls):
+    """There is no backward pass, and the result would not say so."""
+    def rows(*shape, dtype=torch.bfloat16):
+        return Rows(*shape, dtype=dtype, requires_grad=True)
+    made = list(every_call(rows(4, 16))) + [
+        lambda: experts.route(rows(4, 8, dtype=torch.float32), 2),
+        lambda: experts.combine(rows(8, 8), **PAIRS),
+        lambda: experts.combine(Rows(8, 8), PAIRS["position"], rows(4, 2, dtype=torch.float32)),
+        lambda: experts.ExpertFeedForward(expert_layer(32, 16), expert_layer(8, 32), 2).forward(
+            Rows(4, 16), rows(4, 2, dtype=torch.float32)),
+        lambda: layer().forward_codes(Rows(4, 128, dtype=torch.uint8), rows(1, 4, dtype=torch.float32)),
+        lambda: fp8.quantize_rows(rows(4, 8)),
+    ]
+    for call in made:
+        with pytest.raises(CQError, match="no backward pass"):
+            call()
+        with torch.no_grad():
+            call()
+
+
+def test_parameters_may_become_a_layer(calls):
+    """A layer copies its arrays, so a module's parameters are taken as they are."""
+    experts.ExpertLinear.from_weight(torch.nn.Parameter(torch.zeros(1, 4, 8, dtype=torch.bfloat16)))
+    assert calls[-1][0] == "cq_expert_linear_create"
