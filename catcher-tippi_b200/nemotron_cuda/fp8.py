@@ -50,10 +50,17 @@ def _contiguous(a):
     return np.ascontiguousarray(a) if isinstance(a, np.ndarray) else a.contiguous()
 
 
+def _fits32(shape, what: str):
+    """Refuses sizes that the library's 32-bit arguments would cut."""
+    if any(n > 0x7FFFFFFF for n in shape):
+        _refuse(f"{what} of shape {tuple(shape)}: sizes must fit 32 bits")
+
+
 def _packed(a, *shape):
     """An array argument of a layer: its shape checked, without gaps."""
     if tuple(a.shape) != shape:
         _refuse(f"array has shape {tuple(a.shape)}, expected {shape}")
+    _fits32(shape, "an array")
     return _contiguous(a)
 
 
@@ -91,6 +98,7 @@ def _rows_of(x, dims: int, what: str = "input"):
     if x.dim() != 2 or x.shape[1] != dims or (dims > 1 and x.stride(1) != 1):
         _refuse(f"{what} must be rows of {dims} values next to each other, got shape {tuple(x.shape)} "
                 f"with strides {tuple(x.stride())}")
+    _fits32(x.shape, what)
 
 
 def _ld(x) -> int:
@@ -182,7 +190,7 @@ class Fp8Linear(_Layer):
         _typed(weight, "float32", "the weight")
         if bias is not None:
             _typed(bias, "float32", "the bias")
-        w, b = _contiguous(weight), None if bias is None else _packed(bias, n)
+        w, b = _packed(weight, n, k), None if bias is None else _packed(bias, n)
         h = ctypes.c_void_p()
         _check(lib().cq_fp8_linear_create_from_f32(_ptr(w), _ptr(b), n, k, DTYPES[dtype], device, ctypes.byref(h)))
         return cls(h, 1, n, k, dtype, device)
@@ -207,6 +215,7 @@ class Fp8Linear(_Layer):
             _refuse(f"codes have type {codes.dtype}, expected uint8 or float8_e4m3fn")
         if codes.dim() != 2 or codes.shape[1] < self.input_dims or codes.stride(1) != 1:
             _refuse(f"codes must be rows of at least {self.input_dims} bytes, got shape {tuple(codes.shape)}")
+        _fits32(codes.shape, "codes")
         if scales.dtype != torch.float32 or tuple(scales.shape) != (blocks(self.input_dims), rows) or \
                 not scales.is_contiguous():
             _refuse(f"scales must be f32 [{blocks(self.input_dims)}, {rows}] without gaps")
@@ -244,6 +253,7 @@ def quantize_weight(w, stream=None):
     if not w.is_cuda or w.dim() != 2 or w.dtype != torch.float32 or not w.is_contiguous():
         _refuse("weight must be f32 [N, K] without gaps on the device")
     n, k = w.shape
+    _fits32(w.shape, "a weight")
     with _allocating(stream, w.device):
         codes = torch.empty((n, k), dtype=torch.float8_e4m3fn, device=w.device)
         scales = torch.empty((blocks(n), blocks(k)), dtype=torch.float32, device=w.device)

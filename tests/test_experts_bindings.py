@@ -222,3 +222,24 @@ def test_parameters_may_become_a_layer(calls):
     """A layer copies its arrays, so a module's parameters are taken as they are."""
     experts.ExpertLinear.from_weight(torch.nn.Parameter(torch.zeros(1, 4, 8, dtype=torch.bfloat16)))
     assert calls[-1][0] == "cq_expert_linear_create"
+
+
+# ------------------------------------------------------------------ sizes
+
+def test_sizes_past_32_bits_are_refused(calls):
+    """The library takes 32-bit sizes, and ctypes would cut larger ones without a word."""
+    many = (1 << 32) + 4
+    made = list(every_call(Rows(many, 16))) + [
+        lambda: experts.route(Rows(many, 8, dtype=torch.float32), 2),
+        lambda: experts.combine(Rows(many, 8), **PAIRS),
+        lambda: layer().forward_codes(Rows(many, 128, dtype=torch.uint8), Rows(1, many, dtype=torch.float32)),
+        lambda: fp8.quantize_rows(Rows(many, 8)),
+        lambda: fp8.quantize_weight(Rows(many, 1, dtype=torch.float32)),
+    ]
+    made += [lambda: fp8.Fp8Linear.from_codes(torch.zeros(1, 1, dtype=torch.uint8).expand(many, 1), SCALES),
+             lambda: fp8.Fp8Linear.from_f32(torch.zeros(1, 1).expand(many, 1))]
+    for call in made:
+        calls.clear()
+        with pytest.raises(CQError, match="32 bits"):
+            call()
+        assert not any("workspace" not in name for name, _ in calls)
