@@ -143,9 +143,12 @@ class _Layer:
         """(tensor that keeps the memory, pointer, bytes) for a call on `rows` rows."""
         n = self._sizes.get(rows)
         if n is None:
+            n = entry(self._h, rows)
+            if n == SIZE_MAX:
+                _check(-1)
             if len(self._sizes) > 256:
                 self._sizes.clear()
-            n = self._sizes[rows] = entry(self._h, rows)
+            self._sizes[rows] = n
         if n == 0:
             return None, None, 0
         w = torch.empty(n, dtype=torch.uint8, device=self._device)

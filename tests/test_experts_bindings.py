@@ -243,3 +243,18 @@ def test_sizes_past_32_bits_are_refused(calls):
         with pytest.raises(CQError, match="32 bits"):
             call()
         assert not any("workspace" not in name for name, _ in calls)
+
+
+# ------------------------------------------------------------------ layers that are closed
+
+def test_a_closed_layer_is_refused(calls, monkeypatch):
+    """By the library's own message, not by an allocation of the size that it answers for a refusal."""
+    import nemotron_cuda
+    for module in (fp8, experts):
+        monkeypatch.setattr(module, "lib", nemotron_cuda.lib)
+    for closed in (layer(), expert_layer()):
+        closed.close()
+        args = () if closed.experts == 1 else (OFFSETS,)
+        for _ in range(2):
+            with pytest.raises(CQError, match="layer must not be null"):
+                closed.forward(Rows(4, 16), *args)
