@@ -150,18 +150,18 @@ class ExpertFeedForward:
 
     def __init__(self, up: ExpertLinear, down: ExpertLinear, top: int, act: str = "silu", renormalize: bool = True):
         self.up, self.down, self.top, self.act, self.renormalize = up, down, top, act, renormalize
-        self._sizes: dict[int, int] = {}
+        self._sizes: dict[tuple[int, int], int] = {}
         self._workspace_bytes(0)  # the library's checks of the pair
 
     def _workspace_bytes(self, tokens: int) -> int:
-        n = self._sizes.get(tokens)
+        n = self._sizes.get((tokens, self.top))
         if n is None:
             n = lib().cq_expert_ffn_workspace(self.up._h, self.down._h, tokens, self.top)
             if n == SIZE_MAX:
                 _check(-1)
             if len(self._sizes) > 256:
                 self._sizes.clear()
-            self._sizes[tokens] = n
+            self._sizes[tokens, self.top] = n
         return n
 
     def forward(self, x, logits, y=None, stream=None):
@@ -173,7 +173,7 @@ class ExpertFeedForward:
         kind = CODES.get(logits.dtype)
         if kind is None or logits.shape[0] != tokens:
             _refuse(f"logits must be f32, f16 or bf16 with {tokens} rows, got {logits.dtype} {tuple(logits.shape)}")
-        if tokens > 0x7FFFFFFF // self.top:
+        if tokens * self.top > 0x7FFFFFFF:
             _refuse("tokens * top does not fit 32 bits")
         if logits.device != x.device:
             _refuse(f"logits are on {logits.device}, the input on {x.device}")

@@ -258,3 +258,28 @@ def test_a_closed_layer_is_refused(calls, monkeypatch):
         for _ in range(2):
             with pytest.raises(CQError, match="layer must not be null"):
                 closed.forward(Rows(4, 16), *args)
+
+
+# ------------------------------------------------------------------ the module's attributes
+
+def test_top_may_be_changed_between_calls(calls, monkeypatch):
+    """The workspace is the one of the call's own `top`."""
+    sizes = []
+
+    class Library:
+        def cq_expert_ffn_workspace(self, up, down, tokens, top):
+            return 1000 * top + tokens
+
+        def cq_expert_ffn_forward(self, *args):
+            sizes.append((args[8], args[-2]))
+            return 0
+
+        def __getattr__(self, name):
+            return lambda *args: 0
+
+    monkeypatch.setattr(experts, "lib", Library)
+    module = experts.ExpertFeedForward(expert_layer(32, 16), expert_layer(8, 32), 1)
+    for top in (1, 2, 1):
+        module.top = top
+        module.forward(Rows(4, 16), Rows(4, 2, dtype=torch.float32))
+    assert sizes == [(1, 1004), (2, 2004), (1, 1004)]
