@@ -156,3 +156,28 @@ def test_tokens_that_are_not_finite_stay_apart(cq, weights, tokens):
     assert torch.equal(y[~bad], clean[~bad]) and not y[bad].isfinite().any(1).all()
     assert torch.equal(y_rows[~bad[r.token.long()]], rows[~bad[r.token.long()]])
     assert y_rows[r.token == 4].isnan().all()
+
+
+# ------------------------------------------------------------------ refusals, each by its own message
+
+def test_refusals_of_a_forward_call(cq):
+    from nemotron_cuda import fp8
+    f = fp8.Fp8Linear.from_codes(torch.zeros(8, 16, dtype=torch.uint8, device="cuda"), torch.ones(1, 1, device="cuda"))
+    x, y = torch.zeros(40, 16, dtype=torch.bfloat16, device="cuda"), torch.zeros(40, 8, dtype=torch.bfloat16, device="cuda")
+    L = cq.lib()
+    need = L.cq_fp8_linear_workspace(f._h, 40)
+    ws = torch.zeros(need + 512, dtype=torch.uint8, device="cuda")
+    good = dict(x=x.data_ptr(), ldx=16, rows=40, y=y.data_ptr(), ldy=8, act=0, ws=ws.data_ptr(), n=need)
+    for change, needle in ((dict(ws=None), "workspace has 0 bytes, expected"), (dict(n=need - 1), f"workspace has {need - 1} bytes, expected"),
+                           (dict(ws=ws.data_ptr() + 16), "256-byte aligned"), (dict(act=3), "unknown activation 3"),
+                           (dict(ldx=15), "input row stride 15"), (dict(ldy=7), "output row stride 7"),
+                           (dict(rows=-1), "negative row count"), (dict(x=None), "must not be null"), (dict(y=None), "must not be null"),
+                           (dict(x=x.data_ptr() + 1), "input must be aligned"), (dict(y=y.data_ptr() + 1), "output must be aligned")):
+        a = good | change
+        status = L.cq_fp8_linear_forward(f._h, a["x"], a["ldx"], a["rows"], a["y"], a["ldy"], a["act"], a["ws"], a["n"], None)
+        assert status == cq.CQ_INVALID_ARGUMENT and needle in cq.last_error(), (change, cq.last_error())
+    torch.cuda.synchronize()
+
+
+def test_no_wait_ran_out(cq):
+    assert cq.device_status(0) == 0
