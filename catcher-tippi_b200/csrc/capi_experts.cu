@@ -90,7 +90,7 @@ void cq_fp8_linear_destroy(cq_fp8_linear* layer) { delete layer; }
 cq_status cq_fp8_quantize_rows(const void* x, int64_t ldx, int32_t rows, int32_t cols, cq_dtype dtype, uint8_t* codes,
                                int64_t ld, float* scales, void* stream) {
   return guarded([&] {
-    quantize_rows(x, ldx, nullptr, rows, rows, cols, dtype, codes, ld, scales, as_stream(stream));
+    quantize_rows(x, ldx, rows, cols, dtype, codes, ld, scales, as_stream(stream));
   });
 }
 

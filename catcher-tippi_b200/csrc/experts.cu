@@ -259,8 +259,8 @@ void ExpertLinear::forward_codes(const uint8_t* codes, int64_t ld, const float* 
           nullptr, stream);
 }
 
-void quantize_rows(const void* x, int64_t ldx, const int32_t* row_index, int x_rows, int rows, int cols,
-                   cq_dtype dtype, uint8_t* codes, int64_t ld, float* scales, cudaStream_t stream) {
+void quantize_rows(const void* x, int64_t ldx, int rows, int cols, cq_dtype dtype, uint8_t* codes, int64_t ld,
+                   float* scales, cudaStream_t stream) {
   check_dtype(dtype);
   if (rows < 0 || cols < 1 || cols > kMaxDims) throw_invalid("invalid shape " + std::to_string(rows) + "x" + std::to_string(cols));
   if (ldx < cols) throw_invalid("input row stride " + std::to_string(ldx) + " is smaller than " + std::to_string(cols));
@@ -272,7 +272,7 @@ void quantize_rows(const void* x, int64_t ldx, const int32_t* row_index, int x_r
   check_aligned(codes, 16, "codes");
   check_aligned(scales, 4, "scales");
   DeviceGuard guard(device_of(codes, "codes"));
-  const cq::QuantizeRowsArgs q{x, ldx, row_index, x_rows, rows, cols, codes, ld, scales};
+  const cq::QuantizeRowsArgs q{x, ldx, nullptr, rows, rows, cols, codes, ld, scales};
   check_cuda(cq::launch_quantize_rows(dtype, q, stream, pdl_enabled()), "quantize rows");
 }
 

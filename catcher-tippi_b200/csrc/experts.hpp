@@ -84,9 +84,9 @@ class ExpertLinear {
   DeviceBuffer weight_, scales_, bias_;
 };
 
-// x rows -> e4m3 (cq_fp8_quantize_rows), and with row_index a gather.
-void quantize_rows(const void* x, int64_t ldx, const int32_t* row_index, int x_rows, int rows, int cols,
-                   cq_dtype dtype, uint8_t* codes, int64_t ld, float* scales, cudaStream_t stream);
+// x rows -> e4m3 (cq_fp8_quantize_rows).
+void quantize_rows(const void* x, int64_t ldx, int rows, int cols, cq_dtype dtype, uint8_t* codes, int64_t ld,
+                   float* scales, cudaStream_t stream);
 
 // f32 weight -> e4m3 by blocks of 128 x 128 (cq_fp8_quantize_weight).
 void quantize_weight(const float* w, int rows, int cols, uint8_t* codes, float* scales, cudaStream_t stream);

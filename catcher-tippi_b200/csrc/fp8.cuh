@@ -2,8 +2,6 @@
 // linears' kernels.
 #pragma once
 
-#include <cuda_fp8.h>
-
 #include "common.cuh"
 
 namespace cq {
@@ -151,12 +149,6 @@ __device__ __forceinline__ Raw8<T> load_row8(const void* row, int k, int cols, b
   r.u[0] = make_uint4(b[0], b[1], b[2], b[3]);
   if constexpr (T == kF32) r.u[1] = make_uint4(b[4], b[5], b[6], b[7]);
   return r;
-}
-
-__device__ __forceinline__ float e4m3_to_float(uint8_t code) {
-  __nv_fp8_e4m3 v;
-  v.__x = code;
-  return static_cast<float>(v);
 }
 
 __device__ __forceinline__ float fast_exp2(float v) {
