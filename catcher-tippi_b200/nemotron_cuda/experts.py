@@ -16,7 +16,7 @@ from typing import NamedTuple
 import torch
 
 from . import ACTS, DTYPES, _check, _ptr, lib
-from .fp8 import (CODES, SIZE_MAX, T_NAMES, TYPES, _allocating, _check_output, _Layer, _ld, _no_gradient, _packed, _refuse, _rows_of, _stream_of, _typed,
+from .fp8 import (CODES, SIZE_MAX, T_NAMES, TYPES, _allocating, _check_output, _Layer, _no_gradient, _packed, _refuse, _rows_of, _stream_of, _typed,
                   blocks)
 
 FORMATS = {"16bit": 0, "e4m3": 1}
@@ -43,8 +43,8 @@ def route(logits, top: int, renormalize: bool = True, stream=None) -> Route:
     """Router logits torch [tokens, experts] (f32, f16 or bf16) -> each token's `top` best experts and the order of pairs."""
     if logits.dim() != 2:
         _refuse(f"logits must be [tokens, experts], got shape {tuple(logits.shape)}")
-    tokens, experts = logits.shape
-    _rows_of(logits, experts, "logits")
+    experts = logits.shape[1]
+    tokens, ld = _rows_of(logits, experts, "logits")
     kind = CODES.get(logits.dtype)
     if kind is None:
         _refuse(f"logits have type {logits.dtype}, expected f32, f16 or bf16")
@@ -57,7 +57,7 @@ def route(logits, top: int, renormalize: bool = True, stream=None) -> Route:
     with _allocating(stream, device):
         ints = logits.new_empty(end + n // 4, dtype=torch.int32)
         at = ints.data_ptr()
-        _check(L.cq_route(logits.data_ptr(), _ld(logits), kind, tokens, experts, top, int(renormalize), at, at + 4 * step,
+        _check(L.cq_route(logits.data_ptr(), ld, kind, tokens, experts, top, int(renormalize), at, at + 4 * step,
                           at + 16 * step, at + 12 * step, at + 8 * step, at + 4 * end if n else None, n,
                           _stream_of(stream, device)))
     pairs, across = (tokens, top), (top, 1)
@@ -72,23 +72,24 @@ def combine(z, position, weight, y=None, stream=None):
     if z.dim() != 2 or position.dim() != 2 or tuple(weight.shape) != tuple(position.shape):
         _refuse(f"expected rows, and positions and weights [tokens, top]; got shapes {tuple(z.shape)}, "
                 f"{tuple(position.shape)} and {tuple(weight.shape)}")
-    rows, dims = z.shape
+    dims = z.shape[1]
     tokens, top = position.shape
-    _rows_of(z, dims, "rows")
+    rows, ldz = _rows_of(z, dims, "rows")
     kind = CODES.get(z.dtype)
     if kind is None or z.dtype is torch.float32:
         _refuse(f"rows have type {z.dtype}, expected f16 or bf16")
     if position.dtype != torch.int32 or weight.dtype != torch.float32 or not position.is_contiguous() or \
             not weight.is_contiguous() or position.device != z.device or weight.device != z.device:
         _refuse("positions must be int32 and weights f32, without gaps, on the device of the rows")
-    _no_gradient(weight, "an array of weights")
+    if weight.requires_grad:
+        _no_gradient(weight, "an array of weights")
     if y is None:
         with _allocating(stream, z.device):
-            y = z.new_empty((tokens, dims))
+            y, ldy = z.new_empty((tokens, dims)), dims
     else:
-        _check_output(y, z.dtype, tokens, dims, z.device)
-    _check(lib().cq_expert_combine(z.data_ptr(), _ld(z), rows, position.data_ptr(), weight.data_ptr(), tokens,
-                                   top, dims, kind, y.data_ptr(), _ld(y), _stream_of(stream, z.device)))
+        ldy = _check_output(y, z.dtype, tokens, dims, z.device)
+    _check(lib().cq_expert_combine(z.data_ptr(), ldz, rows, position.data_ptr(), weight.data_ptr(), tokens,
+                                   top, dims, kind, y.data_ptr(), ldy, _stream_of(stream, z.device)))
     return y
 
 
@@ -130,18 +131,17 @@ class ExpertLinear(_Layer):
 
     def forward(self, x, offsets, y=None, act: str = "none", stream=None):
         """x torch [rows, K] of T, offsets int32 [experts + 1] on the device -> y [rows, N], zeros from offsets[-1] on."""
-        _rows_of(x, self.input_dims)
+        rows, ldx = _rows_of(x, self.input_dims)
         if offsets.dtype != torch.int32 or tuple(offsets.shape) != (self.experts + 1,) or \
                 not offsets.is_contiguous() or offsets.device != self._device:
             _refuse(f"offsets must be int32 [{self.experts + 1}] on {self._device}, got {offsets.dtype} "
                     f"{tuple(offsets.shape)} on {offsets.device}")
         L = lib()
         with _allocating(stream, x.device):
-            y = self._output(x, y)
-            keep, ws, n = self._workspace(L.cq_expert_linear_workspace, x.shape[0])
-            _check(L.cq_expert_linear_forward(self._h, x.data_ptr(), _ld(x), x.shape[0], offsets.data_ptr(),
-                                              y.data_ptr(), _ld(y), ACTS[act], ws, n,
-                                              _stream_of(stream, x.device)))
+            y, ldy = self._output(x, rows, y)
+            keep, ws, n = self._workspace(L.cq_expert_linear_workspace, rows)
+            _check(L.cq_expert_linear_forward(self._h, x.data_ptr(), ldx, rows, offsets.data_ptr(), y.data_ptr(), ldy,
+                                              ACTS[act], ws, n, _stream_of(stream, x.device)))
         return y
 
 
@@ -167,11 +167,10 @@ class ExpertFeedForward:
     def forward(self, x, logits, y=None, stream=None):
         """x torch [tokens, K] of T, logits [tokens, experts] (f32, f16 or bf16) -> y [tokens, N]."""
         up, down = self.up, self.down
-        _rows_of(x, up.input_dims)
-        _rows_of(logits, up.experts, "logits")
-        tokens = x.shape[0]
+        tokens, ldx = _rows_of(x, up.input_dims)
+        logit_rows, ld = _rows_of(logits, up.experts, "logits")
         kind = CODES.get(logits.dtype)
-        if kind is None or logits.shape[0] != tokens:
+        if kind is None or logit_rows != tokens:
             _refuse(f"logits must be f32, f16 or bf16 with {tokens} rows, got {logits.dtype} {tuple(logits.shape)}")
         if tokens * self.top > 0x7FFFFFFF:
             _refuse("tokens * top does not fit 32 bits")
@@ -179,10 +178,9 @@ class ExpertFeedForward:
             _refuse(f"logits are on {logits.device}, the input on {x.device}")
         n = self._workspace_bytes(tokens)
         with _allocating(stream, x.device):
-            y = down._output(x, y)
+            y, ldy = down._output(x, tokens, y)
             ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-            _check(lib().cq_expert_ffn_forward(up._h, down._h, x.data_ptr(), _ld(x), tokens, logits.data_ptr(),
-                                               _ld(logits), kind, self.top, int(self.renormalize),
-                                               ACTS[self.act], y.data_ptr(), _ld(y), ws.data_ptr(), n,
-                                               _stream_of(stream, x.device)))
+            _check(lib().cq_expert_ffn_forward(up._h, down._h, x.data_ptr(), ldx, tokens, logits.data_ptr(), ld,
+                                               kind, self.top, int(self.renormalize), ACTS[self.act], y.data_ptr(), ldy,
+                                               ws.data_ptr(), n, _stream_of(stream, x.device)))
         return y

@@ -91,28 +91,30 @@ def _no_gradient(x, what: str):
         _refuse(f"{what} requires a gradient, and there is no backward pass: call under torch.no_grad() or detach it")
 
 
-def _rows_of(x, dims: int, what: str = "input"):
+def _rows_of(x, dims: int, what: str = "input") -> tuple[int, int]:
+    """(rows, row stride) of device rows for the library, which asks for a stride of at least the width; that of a
+    single row may be anything in torch (a transposed column has 1)."""
     if not x.is_cuda:
         _refuse(f"{what} must be on the device, got {x.device}")
-    _no_gradient(x, what)
-    if x.dim() != 2 or x.shape[1] != dims or (dims > 1 and x.stride(1) != 1):
-        _refuse(f"{what} must be rows of {dims} values next to each other, got shape {tuple(x.shape)} "
-                f"with strides {tuple(x.stride())}")
-    _fits32(x.shape, what)
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 2 or shape[1] != dims or (dims > 1 and strides[1] != 1):
+        _refuse(f"{what} must be rows of {dims} values next to each other, got shape {tuple(shape)} "
+                f"with strides {tuple(strides)}")
+    if x.requires_grad:
+        _no_gradient(x, what)
+    rows = shape[0]
+    if rows > 0x7FFFFFFF:
+        _fits32(shape, what)
+    return rows, strides[0] if rows > 1 else max(strides[0], dims)
 
 
-def _ld(x) -> int:
-    """The row stride for the library; that of a single row may be anything in torch (a transposed column has 1)."""
-    return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
-
-
-def _check_output(y, dtype, rows: int, dims: int, device):
-    """Refuses a caller's output that the call could not write."""
+def _check_output(y, dtype, rows: int, dims: int, device) -> int:
+    """The row stride of a caller's output, which is refused where the call could not write it."""
     if y.dtype != dtype or y.shape[0] != rows:
         _refuse(f"output must be {dtype} with {rows} rows")
-    _rows_of(y, dims, "output")
     if y.device != device:
         _refuse(f"output is on {y.device}, the input on {device}")
+    return _rows_of(y, dims, "output")[1]
 
 
 class _Layer:
@@ -129,15 +131,15 @@ class _Layer:
         self._device = torch.device("cuda", device)
         self._sizes: dict[int, int] = {}
 
-    def _output(self, x, y):
+    def _output(self, x, rows: int, y):
+        """(the call's output, its row stride), made where the caller gave none."""
         if x.device != self._device:
             _refuse(f"input is on {x.device}, the layer on {self._device}")
         if x.dtype != self._type:
             _refuse(f"input has type {x.dtype}, expected {self._type}")
         if y is None:
-            return x.new_empty((x.shape[0], self.output_dims))
-        _check_output(y, self._type, x.shape[0], self.output_dims, x.device)
-        return y
+            return x.new_empty((rows, self.output_dims)), self.output_dims
+        return y, _check_output(y, self._type, rows, self.output_dims, x.device)
 
     def _workspace(self, entry, rows: int):
         """(tensor that keeps the memory, pointer, bytes) for a call on `rows` rows."""
@@ -200,37 +202,35 @@ class Fp8Linear(_Layer):
 
     def forward(self, x, y=None, act: str = "none", stream=None):
         """x torch [rows, K] of T on the layer's device -> y [rows, N]."""
-        _rows_of(x, self.input_dims)
+        rows, ldx = _rows_of(x, self.input_dims)
         L = lib()
         with _allocating(stream, x.device):
-            y = self._output(x, y)
-            keep, ws, n = self._workspace(L.cq_fp8_linear_workspace, x.shape[0])
-            _check(L.cq_fp8_linear_forward(self._h, x.data_ptr(), _ld(x), x.shape[0], y.data_ptr(), _ld(y),
-                                           ACTS[act], ws, n, _stream_of(stream, x.device)))
+            y, ldy = self._output(x, rows, y)
+            keep, ws, n = self._workspace(L.cq_fp8_linear_workspace, rows)
+            _check(L.cq_fp8_linear_forward(self._h, x.data_ptr(), ldx, rows, y.data_ptr(), ldy, ACTS[act], ws, n,
+                                           _stream_of(stream, x.device)))
         return y
 
     def forward_codes(self, codes, scales, y=None, act: str = "none", stream=None):
         """forward on rows that quantize_rows made: codes [rows, >= K], scales [ceil(K / 128), rows]."""
         if codes.device != self._device or scales.device != self._device:
             _refuse(f"codes and scales must be on {self._device}")
-        rows = codes.shape[0]
         if codes.dtype is not torch.float8_e4m3fn and codes.dtype is not torch.uint8:
             _refuse(f"codes have type {codes.dtype}, expected uint8 or float8_e4m3fn")
         if codes.dim() != 2 or codes.shape[1] < self.input_dims or codes.stride(1) != 1:
             _refuse(f"codes must be rows of at least {self.input_dims} bytes, got shape {tuple(codes.shape)}")
-        _fits32(codes.shape, "codes")
+        rows, ldc = _rows_of(codes, codes.shape[1], "codes")
         if scales.dtype != torch.float32 or tuple(scales.shape) != (blocks(self.input_dims), rows) or \
                 not scales.is_contiguous():
             _refuse(f"scales must be f32 [{blocks(self.input_dims)}, {rows}] without gaps")
         _no_gradient(scales, "an array of scales")
         if y is None:
             with _allocating(stream, codes.device):
-                y = torch.empty((rows, self.output_dims), dtype=self._type, device=codes.device)
+                y, ldy = torch.empty((rows, self.output_dims), dtype=self._type, device=codes.device), self.output_dims
         else:
-            _check_output(y, self._type, rows, self.output_dims, codes.device)
-        _check(lib().cq_fp8_linear_forward_codes(self._h, codes.data_ptr(), _ld(codes), scales.data_ptr(), rows,
-                                                 y.data_ptr(), _ld(y), ACTS[act],
-                                                 _stream_of(stream, codes.device)))
+            ldy = _check_output(y, self._type, rows, self.output_dims, codes.device)
+        _check(lib().cq_fp8_linear_forward_codes(self._h, codes.data_ptr(), ldc, scales.data_ptr(), rows,
+                                                 y.data_ptr(), ldy, ACTS[act], _stream_of(stream, codes.device)))
         return y
 
 
@@ -238,16 +238,16 @@ def quantize_rows(x, stream=None):
     """x torch [rows, K] (f16, bf16 or f32) -> (e4m3 codes [rows, 128 ceil(K / 128)], scales f32 [ceil(K / 128), rows])."""
     if x.dim() != 2:
         _refuse(f"input must be rows, got shape {tuple(x.shape)}")
-    rows, k = x.shape
-    _rows_of(x, k)
+    k = x.shape[1]
+    rows, ldx = _rows_of(x, k)
     kind = TYPES.get(x.dtype)
     if kind is None:
         _refuse(f"input has type {x.dtype}, expected f16, bf16 or f32")
     with _allocating(stream, x.device):
         codes = torch.empty((rows, BLOCK * blocks(k)), dtype=torch.float8_e4m3fn, device=x.device)
         scales = torch.empty((blocks(k), rows), dtype=torch.float32, device=x.device)
-    _check(lib().cq_fp8_quantize_rows(x.data_ptr(), _ld(x), rows, k, DTYPES[kind], codes.data_ptr(),
-                                      _ld(codes), scales.data_ptr(), _stream_of(stream, x.device)))
+    _check(lib().cq_fp8_quantize_rows(x.data_ptr(), ldx, rows, k, DTYPES[kind], codes.data_ptr(),
+                                      codes.stride(0), scales.data_ptr(), _stream_of(stream, x.device)))
     return codes, scales
 
 
