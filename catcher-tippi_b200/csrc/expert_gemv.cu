@@ -15,8 +15,11 @@
 // CTA's shared memory.  Each CTA brings its slice of the rows of x to e4m3
 // itself (a few KB from L2), which saves a launch.
 //
-// 14 rows, n 4096, k 1024 (4.2 MB of weights, 0.66 us of memory): 5.2 us, most
-// of it the launch, the first loads' latency and the join; 8.6 us with the call.
+// n 4096, k 1024 (4.2 MB of weights, 0.66 us of memory), each call on weights that
+// are not in L2: 3.6 us for one row, 4.2 for 8, 5.3 for 14 (4.7 where they come as
+// codes, so 0.6 us are their way to e4m3).  One row's time is the launch, the
+// first loads' latency and the join; what the others add is each CTA's own work on its
+// slice of the rows.  The INT8 linear takes 3.5 us for the 14.
 #include "expert_gemv.hpp"
 
 #include <algorithm>
@@ -288,12 +291,15 @@ cudaError_t launch_dtype(int source, const ExpertGemvArgs& a, int num_sms, cudaS
 bool expert_gemv_fits(int rows, int N, int K) {
   // Every CTA brings the rows to e4m3 for itself, so the work beside the weights'
   // stream is as rows * N * K, while tiles on the tensor cores start later and
-  // take a second launch (9.1 us of host time against 13.9).  us here / there:
-  //   rows          8          16          24          32
-  //   4096 x 1024   4.2/7.6    5.2/7.6     7.3/7.0     8.0/7.3
-  //   1024 x 4096   4.5/11.4   6.6/11.4    9.8/11.4    16.1/11.4
-  //   2048 x 2048   4.8/8.6    6.6/8.6     9.7/8.6     10.2/8.6
-  //   4096 x 4096   7.6/13.5   14.8/12.4   30.3/12.1   33.4/12.1
+  // take a second launch.  us on the GPU here / there (n x k):
+  //   rows          8          16          24
+  //   4096 x 1024   4.2/7.6    5.5/7.4     7.4/7.3
+  //   1024 x 4096   4.6/12.0   6.5/12.0    9.7/12.0
+  //   2048 x 2048   4.7/8.8    6.5/8.8     9.6/8.8
+  //   4096 x 4096   8.4/13.9   14.8/12.4   30.3/12.1
+  // A call from Python takes 7.7 us of host time here and 12.2 there, so that up to
+  // 24 rows it is the faster one here at each of the first three; replayed from a graph,
+  // 17 to 24 rows lose up to a tenth at 2048 x 2048 by that.
   if (rows > kMaxRows || (rows > 8 && static_cast<int64_t>(N) * K > (1 << 23))) return false;
   const int KB = (K + kFp8Block - 1) / kFp8Block;
   int splits = 1;
